@@ -48,7 +48,8 @@ enum w4a16_status {
   W4A16_ERR_KERNEL = -7     /* a kernel gave up on a bounded wait (w4a16_read_device_error) */
 };
 
-enum w4a16_dtype { W4A16_DTYPE_F32 = 0, W4A16_DTYPE_F16 = 1 };
+/* W4A16_DTYPE_BF16 is a type of the paged-cache and logits entries only. */
+enum w4a16_dtype { W4A16_DTYPE_F32 = 0, W4A16_DTYPE_F16 = 1, W4A16_DTYPE_BF16 = 2 };
 enum w4a16_packing { W4A16_PACK_INTERLEAVED = 0, W4A16_PACK_SIMPLE = 1 };
 enum w4a16_prologue { W4A16_PROLOGUE_NONE = 0, W4A16_PROLOGUE_RMSNORM = 1, W4A16_PROLOGUE_SWIGLU = 2 };
 
@@ -359,6 +360,162 @@ size_t w4a16_gemm_workspace_bytes(int M, int N, int K);
 int w4a16_gemm(const uint8_t* packed, const float* scale, int group, const void* x,
                const float* bias, int M, int N, int K, void* y, int out_dtype, void* workspace,
                size_t workspace_bytes, w4a16_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Serving several sequences over a paged key-value cache (no counterpart in the reference,
+ * whose decode is batch 1 through the Hugging Face cache: benchmarks/end_to_end.py:24-42).
+ * A page holds page_size consecutive positions of one sequence for every kv head; a page
+ * table lists each sequence's pages in order.  Rows, tokens and requests are launched
+ * asynchronously and read their indices on the device, so every entry can be captured in a
+ * CUDA graph and replayed with new ones.
+ * ------------------------------------------------------------------------- */
+
+/* One layer's pages.  Position r of kv head g in page p starts at element
+ * p * page_stride + g * head_stride + r * token_stride of k and of v; head_dim elements are
+ * contiguous.  dtype W4A16_DTYPE_F16 or W4A16_DTYPE_BF16; head_dim 64, 128 or 256; page_size
+ * a power of two, 1..4096; strides positive multiples of 8; k and v 16-byte aligned. */
+typedef struct {
+  void* k;
+  void* v;
+  int dtype, pages, kv_heads, page_size, head_dim;
+  long long page_stride, head_stride, token_stride;
+} w4a16_page_pool;
+
+/* Page tables: int32 ids[s * stride + i] is the page of positions [i * page_size,
+ * (i + 1) * page_size) of sequence s; s < sequences, i < width; -1 past the last page. */
+typedef struct {
+  const int32_t* ids;
+  int sequences, width;
+  long long stride;
+} w4a16_page_tables;
+
+/* Writes new keys and values into the cache, with the rotary embedding of q and k.  For
+ * token t at position p = positions[t] of sequence s = seqs[t] (seqs NULL: sequence t):
+ *   q_out[t] = rotary(q[t]);  k pages = rotary(k[t]);  v pages = v[t]
+ * q, q_out [tokens][heads][head_dim], k, v [tokens][kv_heads][head_dim] of the pool's dtype,
+ * with *_stride elements from one token to the next (multiples of 8), 16-byte aligned.  q_out
+ * may be q.  cos_t, sin_t: fp32 [angle_rows][head_dim] rotate-half tables, or both NULL for no
+ * rotation.  heads == 0 (q, q_out NULL) writes the cache only.  Rounded once, from fp32.
+ *   p < 0: padding, nothing is written to the cache, the token's q_out is zero.
+ *   p past the tables, the angles or the pool, or s outside the tables: nothing is written
+ *   to the cache, the token's q_out is NaN.
+ * Each (sequence, position) at most once per call. */
+int w4a16_paged_append(const void* q, long long q_stride, const void* k, long long k_stride,
+                       const void* v, long long v_stride, const int32_t* positions,
+                       const int32_t* seqs, int tokens, int heads, const w4a16_page_tables* tables,
+                       const float* cos_t, const float* sin_t, int angle_rows,
+                       const w4a16_page_pool* pool, void* q_out, long long q_out_stride,
+                       w4a16_stream_t stream);
+
+/* Attention of one query token per row over its sequence's pages:
+ *   out[t][h] = softmax_j(scale * q[t][h] . K[j][g]) V[j][g],  j < lengths[t],
+ *   g = h / (heads / kv_heads), K and V of sequence seqs[t] (seqs NULL: sequence t).
+ * q, out [rows][heads][head_dim] of the pool's dtype with a stride of q_stride / out_stride
+ * elements (multiples of 8) between rows, 16-byte aligned; heads a multiple of kv_heads.
+ * Several rows may name one sequence (a prompt's tokens with growing lengths).  A length <= 0
+ * gives zeros; a length past the tables, a sequence outside them or a page outside the pool
+ * gives NaN.  Scores, softmax and sums in fp32; the probabilities are rounded to the pool's
+ * dtype for the product with V.  workspace: w4a16_paged_attention_workspace_bytes bytes of
+ * scratch, 16-byte aligned, whose content does not matter before or after the call; calls that
+ * may overlap on the GPU need their own.  The length of each row is read on the device and the
+ * rows' positions are shared out evenly over the GPU, so neither the tables' width nor unequal
+ * lengths cost time. */
+size_t w4a16_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* lengths,
+                          const int32_t* seqs, int rows, int heads, const w4a16_page_tables* tables,
+                          const w4a16_page_pool* pool, float scale, void* out, long long out_stride,
+                          void* workspace, size_t workspace_bytes, w4a16_stream_t stream);
+
+/* The bookkeeping of a paged cache, all int32 device memory:
+ *   tables  [sequences][width] (stride elements between rows), lengths [sequences],
+ *   refs    [pages]: the number of table entries that hold the page, 0 for a free one.
+ * Whole pages may be shared between sequences; a partly filled page belongs to one. */
+typedef struct {
+  int32_t* tables;
+  int32_t* lengths;
+  int32_t* refs;
+  int sequences, width, pages, page_size;
+  long long table_stride;
+} w4a16_page_state;
+
+/* The contents of the pages: `layers` pools for k and v, page p of layer l at
+ * l * layer_stride + p * page_stride bytes, page_bytes of them contiguous.  All multiples of
+ * 16, k and v 16-byte aligned. */
+typedef struct {
+  void* k;
+  void* v;
+  int layers, pages;
+  long long layer_stride, page_stride, page_bytes;
+} w4a16_page_blocks;
+
+/* extend: sequence seqs[i] grows by counts[i] positions and receives the lowest free pages
+ * that it needs for them.  fork: sequence dst[i], which must be empty, becomes a copy of
+ * src[i]: whole pages are shared, a partly filled last page is copied (in every layer) to the
+ * lowest free page.  free: sequence seqs[i] gives up every page in its row and becomes empty
+ * (pages whose refs reach 0 are free).  n requests (1..1024; free: any number), served in
+ * order; all of them see the state from before the call.  ok[i] (int32) is 1, or 0 for a
+ * request that was refused and changed nothing: an index out of range, a negative count, more
+ * positions than the table row holds, the same seqs / dst index as an earlier request, a dst
+ * that is not empty or equals its src, or, from the first request on that no longer fits the free pages, every
+ * request that needs one.  scratch: w4a16_pages_fork_scratch_bytes(n), 16-byte aligned. */
+int w4a16_pages_extend(const w4a16_page_state* state, const int32_t* seqs, const int32_t* counts,
+                       int n, int32_t* ok, w4a16_stream_t stream);
+size_t w4a16_pages_fork_scratch_bytes(int n);
+int w4a16_pages_fork(const w4a16_page_state* state, const w4a16_page_blocks* blocks,
+                     const int32_t* src, const int32_t* dst, int n, int32_t* ok, void* scratch,
+                     size_t scratch_bytes, w4a16_stream_t stream);
+int w4a16_pages_free(const w4a16_page_state* state, const int32_t* seqs, int n, int32_t* ok,
+                     w4a16_stream_t stream);
+
+/* Copies page src[i] to page dst[i] in every layer of k and v (int32 device lists).  A pair
+ * with an index outside [0, pages) is skipped.  No page may be in both lists or twice in dst. */
+int w4a16_pages_copy(const w4a16_page_blocks* blocks, const int32_t* src, const int32_t* dst, int n,
+                     w4a16_stream_t stream);
+
+/* Moves the live pages (refs > 0) to the front of the pool: with L of them, the k-th live
+ * page at or above L is copied to the k-th free page below L and no other page moves.
+ * tables_out [entries] = tables with the new page numbers, refs_out likewise (each may be
+ * its input), *moved = pages moved.  scratch: w4a16_pages_compact_scratch_bytes(pages),
+ * 16-byte aligned. */
+size_t w4a16_pages_compact_scratch_bytes(int pages);
+int w4a16_pages_compact(const w4a16_page_blocks* blocks, const int32_t* tables, int32_t* tables_out,
+                        long long entries, const int32_t* refs, int32_t* refs_out, int32_t* moved,
+                        void* scratch, size_t scratch_bytes, w4a16_stream_t stream);
+
+/* What is done to a step's logits before the next token is chosen (no counterpart in the
+ * reference, which takes the argmax of the raw logits: benchmarks/end_to_end.py:33-37).  Per
+ * row b and token v, in fp32, rounded once to dtype:
+ *   x = logits[b][v]
+ *   v among tokens[b][0..total):              x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   c = occurrences in tokens[b][prompt..total):  x = x - frequency[b] * c - presence[b] * (c > 0)
+ *   x = x + bias[v] + the values of the row's pairs (bias_ids, bias_values) with id v
+ *   bit v % 32 of mask[b][v / 32] is 0:       x = -inf
+ * NULL leaves a part out (total_lens NULL: all `history` tokens; prompt_lens NULL: no prompt).
+ * Tokens and ids outside [0, vocab) are skipped; lengths are clamped to [0, history]. */
+typedef struct {
+  const void* logits;       /* [rows][vocab], row stride `stride` elements */
+  void* out;                /* the same layout by out_stride; may be logits itself */
+  int dtype;                /* W4A16_DTYPE_F32, F16 or BF16 */
+  int rows, vocab;
+  long long stride, out_stride;
+  const void* tokens;       /* int32 (token_bytes 4) or int64 (8) [rows][history] */
+  int token_bytes, history;
+  long long token_stride;
+  const int32_t* prompt_lens;   /* [rows] */
+  const int32_t* total_lens;    /* [rows] */
+  const float* repetition;      /* [rows] */
+  const float* frequency;       /* [rows] */
+  const float* presence;        /* [rows] */
+  const float* bias;            /* fp32 [vocab], or [rows][vocab] by bias_stride (0: one for all) */
+  long long bias_stride;
+  const int32_t* bias_ids;      /* [rows][pairs] */
+  const float* bias_values;     /* [rows][pairs] */
+  int pairs;
+  const int32_t* mask;          /* [rows][ceil(vocab / 32)] words by mask_stride (0: one row for all) */
+  long long mask_stride;
+} w4a16_logits_desc;
+
+int w4a16_process_logits(const w4a16_logits_desc* desc, w4a16_stream_t stream);
 
 /* Reads and clears the error word that kernels set when a bounded wait runs out
  * (0 = none; 1 = a weight copy did not land in time; 2 = another rank's flag did not

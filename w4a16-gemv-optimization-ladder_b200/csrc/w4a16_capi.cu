@@ -125,6 +125,148 @@ int ladder(const uint8_t* packed, const float* scale, const void* vec, float* ou
                      W4A16_DTYPE_F32, nullptr, nullptr, 0, stream);
 }
 
+// ---- paged cache: shared checks ----
+
+int check_pool(const w4a16_page_pool* p, w4a16::PagedPool* out) {
+  if (!p || !p->k || !p->v) {
+    set_error("null page pool");
+    return W4A16_ERR_NULL;
+  }
+  if (p->dtype != W4A16_DTYPE_F16 && p->dtype != W4A16_DTYPE_BF16) {
+    set_error("page pool dtype code %d is not fp16 or bf16", p->dtype);
+    return W4A16_ERR_DTYPE;
+  }
+  if (p->pages <= 0 || p->kv_heads <= 0 || p->page_size <= 0 || p->page_size > 4096 ||
+      (p->page_size & (p->page_size - 1)) != 0 ||
+      (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)) {
+    set_error("unsupported page pool: pages %d kv_heads %d page_size %d head_dim %d (page_size a power of "
+              "two up to 4096, head_dim 64, 128 or 256)", p->pages, p->kv_heads, p->page_size, p->head_dim);
+    return W4A16_ERR_SHAPE;
+  }
+  if (p->page_stride <= 0 || p->head_stride <= 0 || p->token_stride <= 0 || p->page_stride % 8 ||
+      p->head_stride % 8 || p->token_stride % 8 || !aligned(p->k, 16) || !aligned(p->v, 16)) {
+    set_error("page pool strides must be positive multiples of 8 elements (page %lld head %lld token %lld), k and v "
+              "16-byte aligned", p->page_stride, p->head_stride, p->token_stride);
+    return W4A16_ERR_ALIGN;
+  }
+  out->k = p->k;
+  out->v = p->v;
+  out->dtype = p->dtype;
+  out->pages = p->pages;
+  out->kv_heads = p->kv_heads;
+  out->head_dim = p->head_dim;
+  out->page_shift = __builtin_ctz((unsigned)p->page_size);
+  out->page_stride = p->page_stride;
+  out->head_stride = p->head_stride;
+  out->token_stride = p->token_stride;
+  return W4A16_OK;
+}
+
+int check_tables(const w4a16_page_tables* t, w4a16::PagedTables* out) {
+  if (!t || !t->ids) {
+    set_error("null page tables");
+    return W4A16_ERR_NULL;
+  }
+  if (t->sequences <= 0 || t->width <= 0 || t->stride < 0) {
+    set_error("bad page tables: %d sequences, width %d, stride %lld", t->sequences, t->width, t->stride);
+    return W4A16_ERR_SHAPE;
+  }
+  if (!aligned(t->ids, 4)) {
+    set_error("page tables must be 4-byte aligned");
+    return W4A16_ERR_ALIGN;
+  }
+  out->ids = t->ids;
+  out->rows = t->sequences;
+  out->width = t->width;
+  out->stride = t->stride;
+  return W4A16_OK;
+}
+
+int check_state(const w4a16_page_state* s, w4a16::PagesState* out) {
+  if (!s || !s->tables || !s->lengths || !s->refs) {
+    set_error("null page state");
+    return W4A16_ERR_NULL;
+  }
+  if (s->sequences <= 0 || s->width <= 0 || s->pages <= 0 || s->page_size <= 0 || s->page_size > 4096 ||
+      (s->page_size & (s->page_size - 1)) != 0 || s->table_stride < s->width) {
+    set_error("bad page state: %d sequences, width %d, stride %lld, %d pages of %d (page_size a power of two up to 4096)",
+              s->sequences, s->width, s->table_stride, s->pages, s->page_size);
+    return W4A16_ERR_SHAPE;
+  }
+  if (!aligned(s->tables, 4) || !aligned(s->lengths, 4) || !aligned(s->refs, 4)) {
+    set_error("page state must be 4-byte aligned");
+    return W4A16_ERR_ALIGN;
+  }
+  out->tables = s->tables;
+  out->lengths = s->lengths;
+  out->refs = s->refs;
+  out->sequences = s->sequences;
+  out->width = s->width;
+  out->pages = s->pages;
+  out->page_shift = __builtin_ctz((unsigned)s->page_size);
+  out->table_stride = s->table_stride;
+  return W4A16_OK;
+}
+
+int check_blocks(const w4a16_page_blocks* b, w4a16::PageBlocks* out) {
+  if (!b || !b->k || !b->v) {
+    set_error("null page blocks");
+    return W4A16_ERR_NULL;
+  }
+  if (b->layers <= 0 || b->pages <= 0 || b->page_bytes <= 0 || b->page_stride < b->page_bytes || b->layer_stride < 0) {
+    set_error("bad page blocks: %d layers of %d pages, layer stride %lld, page stride %lld, %lld bytes a page", b->layers,
+              b->pages, b->layer_stride, b->page_stride, b->page_bytes);
+    return W4A16_ERR_SHAPE;
+  }
+  if (!aligned(b->k, 16) || !aligned(b->v, 16) || b->page_bytes % 16 || b->page_stride % 16 || b->layer_stride % 16) {
+    set_error("page blocks must be 16-byte aligned, sizes and strides multiples of 16");
+    return W4A16_ERR_ALIGN;
+  }
+  out->k = b->k;
+  out->v = b->v;
+  out->layers = b->layers;
+  out->pages = b->pages;
+  out->layer_stride = b->layer_stride;
+  out->page_stride = b->page_stride;
+  out->page_bytes = b->page_bytes;
+  return W4A16_OK;
+}
+
+// n requests with their lists: 0 is a no-op for the caller to return.
+int check_requests(int n, int most, const void* a, const void* b, const void* ok) {
+  if (n < 0 || n > most) {
+    set_error("%d requests (0..%d in one call)", n, most);
+    return W4A16_ERR_SHAPE;
+  }
+  if (n == 0) return W4A16_OK;
+  if (!a || !b || !ok) {
+    set_error("null pointer argument");
+    return W4A16_ERR_NULL;
+  }
+  if (!aligned(a, 4) || !aligned(b, 4) || !aligned(ok, 4)) {
+    set_error("request lists must be 4-byte aligned");
+    return W4A16_ERR_ALIGN;
+  }
+  return W4A16_OK;
+}
+
+int check_scratch(const void* scratch, size_t bytes, size_t need) {
+  if (need == 0) return W4A16_OK;
+  if (!scratch) {
+    set_error("null scratch");
+    return W4A16_ERR_NULL;
+  }
+  if (!aligned(scratch, 16)) {
+    set_error("scratch must be 16-byte aligned");
+    return W4A16_ERR_ALIGN;
+  }
+  if (bytes < need) {
+    set_error("scratch of %zu bytes is smaller than the %zu needed", bytes, need);
+    return W4A16_ERR_WORKSPACE;
+  }
+  return W4A16_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -607,6 +749,241 @@ int w4a16_decode_step(w4a16_decode_plan plan, const int64_t* token, const int64_
                                    reinterpret_cast<const long long*>(token),
                                    reinterpret_cast<const long long*>(pos), k_cache, v_cache, logits,
                                    reinterpret_cast<cudaStream_t>(stream));
+}
+
+int w4a16_paged_append(const void* q, long long q_stride, const void* k, long long k_stride,
+                       const void* v, long long v_stride, const int32_t* positions,
+                       const int32_t* seqs, int tokens, int heads, const w4a16_page_tables* tables,
+                       const float* cos_t, const float* sin_t, int angle_rows,
+                       const w4a16_page_pool* pool, void* q_out, long long q_out_stride,
+                       w4a16_stream_t stream) {
+  w4a16::PagedPool pl;
+  w4a16::PagedTables tb;
+  int rc = check_pool(pool, &pl);
+  if (rc == W4A16_OK) rc = check_tables(tables, &tb);
+  if (rc != W4A16_OK) return rc;
+  if (tokens < 0 || heads < 0 || (cos_t == nullptr) != (sin_t == nullptr) || (cos_t && angle_rows <= 0)) {
+    set_error("bad shape: %d tokens, %d heads, %d rows of angles (cos and sin together)", tokens, heads, angle_rows);
+    return W4A16_ERR_SHAPE;
+  }
+  if (tokens == 0) return W4A16_OK;
+  if (!k || !v || !positions || (heads && (!q || !q_out))) {
+    set_error("null pointer argument");
+    return W4A16_ERR_NULL;
+  }
+  if (q_stride % 8 || k_stride % 8 || v_stride % 8 || q_out_stride % 8 || q_stride < 0 || k_stride < 0 || v_stride < 0 ||
+      (heads && tokens > 1 && q_out_stride < (long long)heads * pl.head_dim) || !aligned(k, 16) || !aligned(v, 16) ||
+      (heads && (!aligned(q, 16) || !aligned(q_out, 16))) || !aligned(positions, 4) || (seqs && !aligned(seqs, 4)) ||
+      (cos_t && (!aligned(cos_t, 16) || !aligned(sin_t, 16)))) {
+    set_error("q, k, v, q_out and the angles must be 16-byte aligned with strides of multiples of 8 elements, indices 4");
+    return W4A16_ERR_ALIGN;
+  }
+  w4a16::PagedAppend a;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_out = q_out;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_out_stride = q_out_stride;
+  a.positions = positions;
+  a.seqs = seqs;
+  a.cos_t = cos_t;
+  a.sin_t = sin_t;
+  a.angle_rows = angle_rows;
+  a.tokens = tokens;
+  a.heads = heads;
+  return w4a16::launch_paged_append(a, pl, tb, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t w4a16_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
+  return w4a16::paged_attention_workspace_bytes(heads, kv_heads, head_dim);
+}
+
+int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* lengths,
+                          const int32_t* seqs, int rows, int heads, const w4a16_page_tables* tables,
+                          const w4a16_page_pool* pool, float scale, void* out, long long out_stride,
+                          void* workspace, size_t workspace_bytes, w4a16_stream_t stream) {
+  w4a16::PagedPool pl;
+  w4a16::PagedTables tb;
+  int rc = check_pool(pool, &pl);
+  if (rc == W4A16_OK) rc = check_tables(tables, &tb);
+  if (rc != W4A16_OK) return rc;
+  if (rows < 0 || heads <= 0 || heads % pl.kv_heads) {
+    set_error("bad shape: %d rows, %d heads over %d kv heads", rows, heads, pl.kv_heads);
+    return W4A16_ERR_SHAPE;
+  }
+  if (rows == 0) return W4A16_OK;
+  if (!q || !lengths || !out) {
+    set_error("null pointer argument");
+    return W4A16_ERR_NULL;
+  }
+  if (q_stride % 8 || out_stride % 8 || q_stride < 0 || (rows > 1 && out_stride < (long long)heads * pl.head_dim) ||
+      !aligned(q, 16) || !aligned(out, 16) || !aligned(lengths, 4) || (seqs && !aligned(seqs, 4))) {
+    set_error("q and out must be 16-byte aligned with strides of multiples of 8 elements, indices 4");
+    return W4A16_ERR_ALIGN;
+  }
+  rc = check_scratch(workspace, workspace_bytes, w4a16::paged_attention_workspace_bytes(heads, pl.kv_heads, pl.head_dim));
+  if (rc != W4A16_OK) return rc;
+  w4a16::PagedAttention a;
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.lengths = lengths;
+  a.seqs = seqs;
+  a.rows = rows;
+  a.heads = heads;
+  a.scale = scale;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return w4a16::launch_paged_attention(a, pl, tb, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int w4a16_pages_extend(const w4a16_page_state* state, const int32_t* seqs, const int32_t* counts,
+                       int n, int32_t* ok, w4a16_stream_t stream) {
+  w4a16::PagesState st;
+  int rc = check_state(state, &st);
+  if (rc == W4A16_OK) rc = check_requests(n, w4a16::kPagesMaxRequests, seqs, counts, ok);
+  if (rc != W4A16_OK || n == 0) return rc;
+  return w4a16::launch_pages_extend(st, seqs, counts, n, ok, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t w4a16_pages_fork_scratch_bytes(int n) { return n > 0 ? (size_t)n * 8 : 0; }
+
+int w4a16_pages_fork(const w4a16_page_state* state, const w4a16_page_blocks* blocks,
+                     const int32_t* src, const int32_t* dst, int n, int32_t* ok, void* scratch,
+                     size_t scratch_bytes, w4a16_stream_t stream) {
+  w4a16::PagesState st;
+  w4a16::PageBlocks b;
+  int rc = check_state(state, &st);
+  if (rc == W4A16_OK) rc = check_blocks(blocks, &b);
+  if (rc == W4A16_OK) rc = check_requests(n, w4a16::kPagesMaxRequests, src, dst, ok);
+  if (rc != W4A16_OK || n == 0) return rc;
+  if (st.pages != b.pages) {
+    set_error("the page state has %d pages, the blocks %d", st.pages, b.pages);
+    return W4A16_ERR_SHAPE;
+  }
+  rc = check_scratch(scratch, scratch_bytes, w4a16_pages_fork_scratch_bytes(n));
+  if (rc != W4A16_OK) return rc;
+  return w4a16::launch_pages_fork(st, b, src, dst, n, ok, scratch, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int w4a16_pages_free(const w4a16_page_state* state, const int32_t* seqs, int n, int32_t* ok,
+                     w4a16_stream_t stream) {
+  w4a16::PagesState st;
+  int rc = check_state(state, &st);
+  if (rc == W4A16_OK) rc = check_requests(n, 1 << 20, seqs, seqs, ok);
+  if (rc != W4A16_OK || n == 0) return rc;
+  return w4a16::launch_pages_free(st, seqs, n, ok, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int w4a16_pages_copy(const w4a16_page_blocks* blocks, const int32_t* src, const int32_t* dst, int n,
+                     w4a16_stream_t stream) {
+  w4a16::PageBlocks b;
+  int rc = check_blocks(blocks, &b);
+  if (rc == W4A16_OK) rc = check_requests(n, 1 << 30, src, dst, src);
+  if (rc != W4A16_OK || n == 0) return rc;
+  return w4a16::launch_pages_copy(b, src, dst, n, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t w4a16_pages_compact_scratch_bytes(int pages) {
+  return pages > 0 ? w4a16::pages_compact_scratch_bytes(pages) : 0;
+}
+
+int w4a16_pages_compact(const w4a16_page_blocks* blocks, const int32_t* tables, int32_t* tables_out,
+                        long long entries, const int32_t* refs, int32_t* refs_out, int32_t* moved,
+                        void* scratch, size_t scratch_bytes, w4a16_stream_t stream) {
+  w4a16::PageBlocks b;
+  int rc = check_blocks(blocks, &b);
+  if (rc != W4A16_OK) return rc;
+  if (entries < 0) {
+    set_error("%lld table entries", entries);
+    return W4A16_ERR_SHAPE;
+  }
+  if (!refs || !refs_out || !moved || (entries && (!tables || !tables_out))) {
+    set_error("null pointer argument");
+    return W4A16_ERR_NULL;
+  }
+  if (!aligned(refs, 4) || !aligned(refs_out, 4) || !aligned(moved, 4) || (entries && (!aligned(tables, 4) || !aligned(tables_out, 4)))) {
+    set_error("tables, refs and moved must be 4-byte aligned");
+    return W4A16_ERR_ALIGN;
+  }
+  rc = check_scratch(scratch, scratch_bytes, w4a16::pages_compact_scratch_bytes(b.pages));
+  if (rc != W4A16_OK) return rc;
+  return w4a16::launch_pages_compact(b, tables, tables_out, entries, refs, refs_out, moved, scratch,
+                                     reinterpret_cast<cudaStream_t>(stream));
+}
+
+int w4a16_process_logits(const w4a16_logits_desc* d, w4a16_stream_t stream) {
+  if (!d) {
+    set_error("null description");
+    return W4A16_ERR_NULL;
+  }
+  if (d->dtype != W4A16_DTYPE_F32 && d->dtype != W4A16_DTYPE_F16 && d->dtype != W4A16_DTYPE_BF16) {
+    set_error("unknown logits dtype code %d", d->dtype);
+    return W4A16_ERR_DTYPE;
+  }
+  if (d->tokens && d->token_bytes != 4 && d->token_bytes != 8) {
+    set_error("tokens of %d bytes (4 or 8)", d->token_bytes);
+    return W4A16_ERR_DTYPE;
+  }
+  if (d->rows < 0 || d->vocab < 0 || d->history < 0 || d->pairs < 0 || d->stride < 0 || d->bias_stride < 0 ||
+      d->mask_stride < 0 || d->token_stride < 0 || (d->rows > 1 && d->out_stride < d->vocab)) {
+    set_error("bad shape: rows %d vocab %d history %d pairs %d or a negative or overlapping stride", d->rows, d->vocab,
+              d->history, d->pairs);
+    return W4A16_ERR_SHAPE;
+  }
+  if (d->rows == 0 || d->vocab == 0) return W4A16_OK;
+  if (!d->logits || !d->out || (d->pairs && (!d->bias_ids || !d->bias_values))) {
+    set_error("null pointer argument");
+    return W4A16_ERR_NULL;
+  }
+  const size_t size = d->dtype == W4A16_DTYPE_F32 ? 4 : 2;
+  if (!aligned(d->logits, size) || !aligned(d->out, size) || (d->tokens && !aligned(d->tokens, d->token_bytes)) ||
+      (d->prompt_lens && !aligned(d->prompt_lens, 4)) || (d->total_lens && !aligned(d->total_lens, 4)) ||
+      (d->repetition && !aligned(d->repetition, 4)) || (d->frequency && !aligned(d->frequency, 4)) ||
+      (d->presence && !aligned(d->presence, 4)) || (d->bias && !aligned(d->bias, 4)) ||
+      (d->pairs && (!aligned(d->bias_ids, 4) || !aligned(d->bias_values, 4))) || (d->mask && !aligned(d->mask, 4))) {
+    set_error("a pointer is not aligned to its element size");
+    return W4A16_ERR_ALIGN;
+  }
+  {  // in place exactly, or apart
+    const uintptr_t i0 = reinterpret_cast<uintptr_t>(d->logits), o0 = reinterpret_cast<uintptr_t>(d->out);
+    const uintptr_t i1 = i0 + ((size_t)(d->rows - 1) * d->stride + d->vocab) * size;
+    const uintptr_t o1 = o0 + ((size_t)(d->rows - 1) * d->out_stride + d->vocab) * size;
+    if (i0 < o1 && o0 < i1 && !(i0 == o0 && (d->rows == 1 || d->stride == d->out_stride))) {
+      set_error("out overlaps logits without being them");
+      return W4A16_ERR_SHAPE;
+    }
+  }
+  w4a16::LogitsProblem p;
+  p.logits = d->logits;
+  p.out = d->out;
+  p.dtype = d->dtype;
+  p.rows = d->rows;
+  p.vocab = d->vocab;
+  p.stride = d->stride;
+  p.out_stride = d->out_stride;
+  p.tokens = d->history ? d->tokens : nullptr;
+  p.token_bytes = d->token_bytes;
+  p.history = d->history;
+  p.token_stride = d->token_stride;
+  p.prompt_lens = d->prompt_lens;
+  p.total_lens = d->total_lens;
+  p.repetition = d->repetition;
+  p.frequency = d->frequency;
+  p.presence = d->presence;
+  p.bias = d->bias;
+  p.bias_stride = d->bias_stride;
+  p.bias_ids = d->bias_ids;
+  p.bias_values = d->bias_values;
+  p.pairs = d->pairs;
+  p.mask = d->mask;
+  p.mask_stride = d->mask_stride;
+  return w4a16::launch_process_logits(p, reinterpret_cast<cudaStream_t>(stream));
 }
 
 const char* w4a16_status_string(int status) {

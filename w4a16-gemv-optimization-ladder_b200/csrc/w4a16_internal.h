@@ -128,6 +128,97 @@ int read_gemm_error(int* code, cudaStream_t stream);
 int decode_plan_timeline(DecodePlan* plan, int enable, unsigned long long* host, size_t capacity,
                          size_t* count, cudaStream_t stream);
 
+// ---- serving over a paged key-value cache (w4a16_paged.cu, w4a16_pages.cu) ----
+// One layer's pages; strides in elements.
+struct PagedPool {
+  void* k = nullptr;
+  void* v = nullptr;
+  int dtype = W4A16_DTYPE_F16;  // F16 or BF16
+  int pages = 0, kv_heads = 0, head_dim = 0, page_shift = 0;
+  long long page_stride = 0, head_stride = 0, token_stride = 0;
+};
+// The pages of every sequence: ids[s * stride + i], i < width, s < rows.
+struct PagedTables {
+  const int* ids = nullptr;
+  int rows = 0, width = 0;
+  long long stride = 0;
+};
+struct PagedAppend {
+  const void* q = nullptr;
+  const void* k = nullptr;
+  const void* v = nullptr;
+  void* q_out = nullptr;
+  long long q_stride = 0, k_stride = 0, v_stride = 0, q_out_stride = 0;  // elements per token
+  const int* positions = nullptr;
+  const int* seqs = nullptr;     // null: token t is sequence t
+  const float* cos_t = nullptr;  // null: no rotation
+  const float* sin_t = nullptr;
+  int angle_rows = 0, tokens = 0, heads = 0;
+};
+struct PagedAttention {
+  const void* q = nullptr;
+  void* out = nullptr;
+  long long q_stride = 0, out_stride = 0;  // elements per row
+  const int* lengths = nullptr;
+  const int* seqs = nullptr;  // null: row t is sequence t
+  int rows = 0, heads = 0;
+  float scale = 0.f;
+  void* workspace = nullptr;
+  size_t workspace_bytes = 0;
+};
+int launch_paged_append(const PagedAppend& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream);
+size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+int launch_paged_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream);
+
+constexpr int kPagesMaxRequests = 1024;  // requests of one extend / fork call
+struct PagesState {
+  int* tables = nullptr;
+  int* lengths = nullptr;
+  int* refs = nullptr;
+  int sequences = 0, width = 0, pages = 0, page_shift = 0;
+  long long table_stride = 0;
+};
+// The pages' bytes: page p of layer l starts at l * layer_stride + p * page_stride (bytes).
+struct PageBlocks {
+  void* k = nullptr;
+  void* v = nullptr;
+  int layers = 0, pages = 0;
+  long long layer_stride = 0, page_stride = 0, page_bytes = 0;
+};
+int launch_pages_extend(const PagesState& st, const int* seqs, const int* counts, int n, int* ok, cudaStream_t stream);
+int launch_pages_fork(const PagesState& st, const PageBlocks& b, const int* src, const int* dst, int n, int* ok, void* scratch,
+                      cudaStream_t stream);
+int launch_pages_free(const PagesState& st, const int* seqs, int n, int* ok, cudaStream_t stream);
+int launch_pages_copy(const PageBlocks& b, const int* src, const int* dst, int n, cudaStream_t stream);
+size_t pages_compact_scratch_bytes(int pages);
+int launch_pages_compact(const PageBlocks& b, const int* tables, int* tables_out, long long entries, const int* refs, int* refs_out,
+                         int* moved, void* scratch, cudaStream_t stream);
+
+// Penalties, biases and grammar masks on logits (w4a16_logits.cu).
+struct LogitsProblem {
+  const void* logits = nullptr;
+  void* out = nullptr;
+  int dtype = W4A16_DTYPE_F32;  // F32, F16 or BF16
+  int rows = 0, vocab = 0;
+  long long stride = 0, out_stride = 0;
+  const void* tokens = nullptr;  // int32 or int64 [rows][history]
+  int token_bytes = 4, history = 0;
+  long long token_stride = 0;
+  const int* prompt_lens = nullptr;
+  const int* total_lens = nullptr;
+  const float* repetition = nullptr;
+  const float* frequency = nullptr;
+  const float* presence = nullptr;
+  const float* bias = nullptr;  // [vocab], or [rows][vocab] by bias_stride
+  long long bias_stride = 0;
+  const int* bias_ids = nullptr;
+  const float* bias_values = nullptr;
+  int pairs = 0;
+  const int* mask = nullptr;  // bit v % 32 of word v / 32: token v is allowed
+  long long mask_stride = 0;
+};
+int launch_process_logits(const LogitsProblem& p, cudaStream_t stream);
+
 // Thread-local description of the last failure, for w4a16_last_error_string().
 void set_error(const char* fmt, ...);
 // SM count of the current device (cached per device).

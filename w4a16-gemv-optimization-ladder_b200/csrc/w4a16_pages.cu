@@ -1,0 +1,293 @@
+// Bookkeeping of a paged key-value cache on the device, so that a captured serving loop can
+// grow, fork, free and compact its sequences without the host:
+//   tables  int32 [sequences][width]  the pages of each sequence in order, -1 past the last
+//   lengths int32 [sequences]         positions held
+//   refs    int32 [pages]             number of table entries that hold the page (0: free)
+// Whole pages may be shared by several sequences; a partly filled page belongs to one.
+//
+// extend and fork first run one CTA that serves the requests in order with the lowest free
+// pages (k_pages_plan); what is proportional to table widths or page contents is done by
+// grid-wide kernels (k_pages_apply, k_page_moves).
+#include <cuda_runtime.h>
+
+#include "w4a16_internal.h"
+
+namespace w4a16 {
+
+namespace {
+
+constexpr int kPlanThreads = kPagesMaxRequests;  // one thread per request
+
+// Exclusive prefix sum over the CTA; *total gets the sum.  `sh` holds 33 values; callable
+// again after the next __syncthreads.
+__device__ __forceinline__ int block_prefix(int v, int* sh, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += n;
+  }
+  if (lane == 31) sh[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    const int n = (int)(blockDim.x >> 5);
+    int w = lane < n ? sh[lane] : 0, s = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += x;
+    }
+    sh[lane] = s - w;
+    if (lane == 31) sh[32] = s;
+  }
+  __syncthreads();
+  *total = sh[32];
+  return sh[warp] + inc - v;
+}
+
+// Serves the requests of one call in order.  extend (src == nullptr): sequence seqs[i] grows by
+// counts[i] positions.  fork: seqs[i] (empty) becomes a copy of src[i]; it needs a page of its
+// own for src's partly filled one.  Request i is refused (ok 0, nothing changed) when its
+// arguments are out of range, when an earlier request names the same seqs[i], or when the
+// free pages do not suffice for all requests up to it.
+__global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st, const int* __restrict__ seqs,
+                                                             const int* __restrict__ src, const int* __restrict__ counts,
+                                                             int n, int* __restrict__ ok, int2* __restrict__ moves) {
+  __shared__ int sh[33], named[kPlanThreads], cum[kPlanThreads], first[kPlanThreads];
+  const int i = threadIdx.x;
+  const int seq = i < n ? seqs[i] : -1;
+  named[i] = seq;
+  __syncthreads();
+  const int mask = (1 << st.page_shift) - 1;
+  const long long cap = (long long)st.width << st.page_shift;
+  bool valid = i < n && seq >= 0 && seq < st.sequences;
+  for (int j = 0; valid && j < i; ++j) valid = named[j] != seq;
+  int need = 0, length = 0, from = 0, grown = 0;
+  if (valid) {
+    length = st.lengths[seq];
+    if (src) {
+      from = src[i];
+      valid = from >= 0 && from < st.sequences && from != seq && length == 0;
+      if (valid) {
+        grown = st.lengths[from];
+        valid = grown >= 0 && grown <= cap;
+        need = valid && (grown & mask) ? 1 : 0;
+        length = grown & ~mask;  // the first position that needs a page of its own
+      }
+    } else {
+      const int c = counts[i];
+      valid = c >= 0 && length >= 0 && (long long)length + c <= cap;
+      if (valid) {
+        grown = length + c;
+        need = (int)(((long long)grown + mask) >> st.page_shift) - (int)(((long long)length + mask) >> st.page_shift);
+      }
+    }
+  }
+  if (!valid) need = 0;
+  int wanted;
+  const int before = block_prefix(need, sh, &wanted);
+  cum[i] = before + need;
+  first[i] = (int)(((long long)length + mask) >> st.page_shift);  // table column of the request's first new page
+  __syncthreads();
+  // the lowest free pages, as many as are wanted: rank -> request -> table entry.  Which
+  // requests are served is known once the free pages are counted, so count, then hand out.
+  int found = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int have = 0;
+    for (int p0 = 0; p0 < st.pages && have < wanted; p0 += kPlanThreads) {
+      const int p = p0 + i;
+      const bool free = p < st.pages && st.refs[p] == 0;
+      int got;
+      const int rank = have + block_prefix(free ? 1 : 0, sh, &got);
+      __syncthreads();
+      if (pass == 1 && free && rank < wanted) {
+        int lo = 0, hi = kPlanThreads - 1;  // the first request whose running sum exceeds rank
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (cum[mid] > rank) hi = mid; else lo = mid + 1;
+        }
+        if (cum[lo] <= found) {
+          const int k = rank - (lo ? cum[lo - 1] : 0);
+          st.refs[p] = 1;
+          if (moves) {
+            const int f = src[lo];
+            moves[lo] = make_int2(st.tables[(size_t)f * st.table_stride + first[lo]], p);
+          }
+          st.tables[(size_t)named[lo] * st.table_stride + first[lo] + k] = p;
+        }
+      }
+      have += got;
+    }
+    if (pass == 0) found = have;
+  }
+  if (i < n) {
+    const bool served = valid && (need == 0 || cum[i] <= found);
+    ok[i] = served ? 1 : 0;
+    if (served) st.lengths[seq] = grown;
+    if (moves && !(served && need)) moves[i] = make_int2(-1, -1);
+  }
+}
+
+// Shares the whole pages of fork's sources: one CTA row per request.
+__global__ void __launch_bounds__(256) k_pages_share(const PagesState st, const int* __restrict__ src, const int* __restrict__ dst,
+                                                     const int* __restrict__ ok) {
+  const int i = blockIdx.y;
+  if (!ok[i]) return;
+  const int whole = st.lengths[dst[i]] >> st.page_shift;  // set by the plan; a source may be another request's dst
+  const int* from = st.tables + (size_t)src[i] * st.table_stride;
+  int* to = st.tables + (size_t)dst[i] * st.table_stride;
+  for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < whole; c += gridDim.x * blockDim.x) {
+    const int p = from[c];
+    to[c] = p;
+    if (p >= 0 && p < st.pages) atomicAdd(st.refs + p, 1);
+  }
+}
+
+// Frees sequences: one CTA per request; the first request that names a sequence counts.
+__global__ void __launch_bounds__(256) k_pages_free(const PagesState st, const int* __restrict__ seqs, int n, int* __restrict__ ok) {
+  const int i = blockIdx.x;
+  const int seq = seqs[i];
+  int again = 0;
+  for (int j = threadIdx.x; j < i; j += blockDim.x) again |= seqs[j] == seq;
+  again = __syncthreads_or(again);
+  const bool valid = seq >= 0 && seq < st.sequences && !again;
+  if (threadIdx.x == 0) ok[i] = valid ? 1 : 0;
+  if (!valid) return;
+  int* row = st.tables + (size_t)seq * st.table_stride;
+  for (int c = threadIdx.x; c < st.width; c += blockDim.x) {
+    const int p = row[c];
+    if (p >= 0 && p < st.pages) atomicSub(st.refs + p, 1);
+    row[c] = -1;
+  }
+  if (threadIdx.x == 0) st.lengths[seq] = 0;
+}
+
+// Compaction plan, one CTA: with L live pages, the k-th live page at or above L moves to the
+// k-th free page below it.  Sources and destinations are disjoint, and no page moves that
+// does not have to.
+__global__ void __launch_bounds__(1024) k_compact_plan(const int* refs, int pages, int* refs_out, int* __restrict__ where,
+                                                       int2* __restrict__ moves, int* __restrict__ moved) {
+  __shared__ int sh[33];
+  const int per = (pages + 1023) / 1024, p0 = min(pages, (int)threadIdx.x * per), p1 = min(pages, p0 + per);
+  int live = 0;
+  for (int p = p0; p < p1; ++p) live += refs[p] > 0;
+  int total;
+  block_prefix(live, sh, &total);
+  __syncthreads();
+  int high = 0, holes = 0;
+  for (int p = p0; p < p1; ++p) {
+    const bool l = refs[p] > 0;
+    high += l && p >= total;
+    holes += !l && p < total;
+  }
+  int count, same;
+  int hk = block_prefix(high, sh, &count);
+  __syncthreads();
+  int ok = block_prefix(holes, sh, &same);
+  for (int p = p0; p < p1; ++p) {
+    const int r = refs[p];
+    if (r > 0 && p >= total) moves[hk++].x = p;
+    if (r <= 0 && p < total) moves[ok++].y = p;
+  }
+  __syncthreads();  // the moves are visible to the CTA
+  if (refs_out != refs)
+    for (int p = threadIdx.x; p < pages; p += 1024) refs_out[p] = refs[p];
+  for (int p = threadIdx.x; p < pages; p += 1024) where[p] = p;
+  __syncthreads();
+  for (int k = threadIdx.x; k < count; k += 1024) {
+    const int2 m = moves[k];
+    where[m.x] = m.y;
+    refs_out[m.y] = refs[m.x];
+    refs_out[m.x] = 0;
+  }
+  if (threadIdx.x == 0) *moved = count;
+}
+
+__global__ void __launch_bounds__(256) k_tables_remap(const int* tables, int* out, long long n, const int* __restrict__ where, int pages) {
+  for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (long long)gridDim.x * blockDim.x) {
+    const int p = tables[e];
+    out[e] = p >= 0 && p < pages ? where[p] : p;
+  }
+}
+
+// Copies whole pages of every layer, k and v: moves are pairs (src, dst), or two lists.  A pair
+// with an index outside [0, pages) is skipped.  Item = (pair, layer, pool); 16 bytes a thread.
+__global__ void __launch_bounds__(256) k_page_moves(const PageBlocks b, const int2* __restrict__ pairs, const int* __restrict__ src,
+                                                    const int* __restrict__ dst, int n, const int* __restrict__ count) {
+  if (count) n = min(n, *count);
+  const long long items = 2LL * n * b.layers;
+  for (long long e = blockIdx.x; e < items; e += gridDim.x) {
+    const int which = (int)(e & 1), layer = (int)((e >> 1) % b.layers), i = (int)((e >> 1) / b.layers);
+    const int f = pairs ? pairs[i].x : src[i], t = pairs ? pairs[i].y : dst[i];
+    if (f < 0 || f >= b.pages || t < 0 || t >= b.pages || f == t) continue;
+    uint8_t* base = static_cast<uint8_t*>(which ? b.v : b.k) + (size_t)layer * b.layer_stride;
+    const uint4* from = reinterpret_cast<const uint4*>(base + (size_t)f * b.page_stride);
+    uint4* to = reinterpret_cast<uint4*>(base + (size_t)t * b.page_stride);
+    const long long words = b.page_bytes / 16;
+    for (long long w = threadIdx.x; w < words; w += 256) to[w] = from[w];
+  }
+}
+
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return W4A16_OK;
+  set_error("%s launch failed: %s", what, cudaGetErrorString(e));
+  return W4A16_ERR_CUDA;
+}
+
+int launch_moves(const PageBlocks& b, const int2* pairs, const int* src, const int* dst, int n, const int* count, cudaStream_t stream) {
+  int sms = 0;
+  const int rc = current_sm_count(&sms);
+  if (rc != W4A16_OK) return rc;
+  const long long items = 2LL * n * b.layers, most = (long long)sms * 8;
+  k_page_moves<<<(unsigned)(items < most ? items : most), 256, 0, stream>>>(b, pairs, src, dst, n, count);
+  return launched("k_page_moves");
+}
+
+}  // namespace
+
+int launch_pages_extend(const PagesState& st, const int* seqs, const int* counts, int n, int* ok, cudaStream_t stream) {
+  k_pages_plan<<<1, kPlanThreads, 0, stream>>>(st, seqs, nullptr, counts, n, ok, nullptr);
+  return launched("k_pages_plan");
+}
+
+int launch_pages_fork(const PagesState& st, const PageBlocks& b, const int* src, const int* dst, int n, int* ok, void* scratch,
+                      cudaStream_t stream) {
+  int2* moves = static_cast<int2*>(scratch);
+  k_pages_plan<<<1, kPlanThreads, 0, stream>>>(st, dst, src, nullptr, n, ok, moves);
+  int rc = launched("k_pages_plan");
+  if (rc != W4A16_OK) return rc;
+  const int blocks = (st.width + 1023) / 1024;
+  k_pages_share<<<dim3(blocks, n), 256, 0, stream>>>(st, src, dst, ok);
+  rc = launched("k_pages_share");
+  return rc == W4A16_OK ? launch_moves(b, moves, nullptr, nullptr, n, nullptr, stream) : rc;
+}
+
+int launch_pages_free(const PagesState& st, const int* seqs, int n, int* ok, cudaStream_t stream) {
+  k_pages_free<<<n, 256, 0, stream>>>(st, seqs, n, ok);
+  return launched("k_pages_free");
+}
+
+int launch_pages_copy(const PageBlocks& b, const int* src, const int* dst, int n, cudaStream_t stream) {
+  return launch_moves(b, nullptr, src, dst, n, nullptr, stream);
+}
+
+size_t pages_compact_scratch_bytes(int pages) { return (size_t)pages * 12; }
+
+int launch_pages_compact(const PageBlocks& b, const int* tables, int* tables_out, long long entries, const int* refs, int* refs_out,
+                         int* moved, void* scratch, cudaStream_t stream) {
+  int2* moves = static_cast<int2*>(scratch);
+  int* where = reinterpret_cast<int*>(moves + b.pages);
+  k_compact_plan<<<1, 1024, 0, stream>>>(refs, b.pages, refs_out, where, moves, moved);
+  int rc = launched("k_compact_plan");
+  if (rc != W4A16_OK) return rc;
+  if (entries > 0) {
+    const long long blocks = (entries + 255) / 256;
+    k_tables_remap<<<(unsigned)(blocks < 1024 ? blocks : 1024), 256, 0, stream>>>(tables, tables_out, entries, where, b.pages);
+    rc = launched("k_tables_remap");
+  }
+  return rc == W4A16_OK ? launch_moves(b, moves, nullptr, nullptr, b.pages, moved, stream) : rc;
+}
+
+}  // namespace w4a16

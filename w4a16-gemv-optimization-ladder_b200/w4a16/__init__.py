@@ -28,6 +28,17 @@ from .kernels import (
 )
 from . import ops  # noqa: F401  (registers torch.ops.w4a16.*)
 from .checkpoint import load_quantized, save_quantized
+from .logits import process_logits
+from .paged import (
+    PagedKVCache,
+    compact_pages,
+    copy_pages,
+    extend_sequences,
+    fork_sequences,
+    free_sequences,
+    paged_append,
+    paged_attention,
+)
 from .linear import W4A16Linear, replace_linear_with_w4a16
 from .quant import (
     dequant_ref,
@@ -50,4 +61,7 @@ __all__ = [
     "dequant_int4", "gemm", "quantize_pack", "unpack_int4", "reserve_workspace", "save_quantized",
     "load_quantized",
     "read_device_error",
+    # serving several sequences
+    "PagedKVCache", "paged_append", "paged_attention", "extend_sequences", "fork_sequences", "free_sequences",
+    "compact_pages", "copy_pages", "process_logits",
 ]

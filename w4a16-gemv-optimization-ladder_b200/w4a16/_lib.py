@@ -15,6 +15,7 @@ ENV_LIB = "W4A16_B200_LIB"
 W4A16_OK = 0
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2
 PACK_INTERLEAVED = 0
 PACK_SIMPLE = 1
 PROLOGUE_NONE = 0
@@ -27,6 +28,41 @@ _p = ctypes.c_void_p
 _i = ctypes.c_int
 _u = ctypes.c_uint
 _sz = ctypes.c_size_t
+_ll = ctypes.c_longlong
+
+
+
+class PagePool(ctypes.Structure):
+    """w4a16_page_pool of include/w4a16_b200.h."""
+    _fields_ = [("k", _p), ("v", _p), ("dtype", _i), ("pages", _i), ("kv_heads", _i), ("page_size", _i),
+                ("head_dim", _i), ("page_stride", _ll), ("head_stride", _ll), ("token_stride", _ll)]
+
+
+class PageTables(ctypes.Structure):
+    """w4a16_page_tables."""
+    _fields_ = [("ids", _p), ("sequences", _i), ("width", _i), ("stride", _ll)]
+
+
+class PageState(ctypes.Structure):
+    """w4a16_page_state."""
+    _fields_ = [("tables", _p), ("lengths", _p), ("refs", _p), ("sequences", _i), ("width", _i), ("pages", _i),
+                ("page_size", _i), ("table_stride", _ll)]
+
+
+class PageBlocks(ctypes.Structure):
+    """w4a16_page_blocks."""
+    _fields_ = [("k", _p), ("v", _p), ("layers", _i), ("pages", _i), ("layer_stride", _ll), ("page_stride", _ll),
+                ("page_bytes", _ll)]
+
+
+class LogitsDesc(ctypes.Structure):
+    """w4a16_logits_desc."""
+    _fields_ = [("logits", _p), ("out", _p), ("dtype", _i), ("rows", _i), ("vocab", _i), ("stride", _ll),
+                ("out_stride", _ll), ("tokens", _p), ("token_bytes", _i), ("history", _i), ("token_stride", _ll),
+                ("prompt_lens", _p), ("total_lens", _p), ("repetition", _p), ("frequency", _p), ("presence", _p),
+                ("bias", _p), ("bias_stride", _ll), ("bias_ids", _p), ("bias_values", _p), ("pairs", _i),
+                ("mask", _p), ("mask_stride", _ll)]
+
 
 _REF_SIG = [_p, _p, _p, _p, _i, _i, _p]
 SIGNATURES = {
@@ -64,6 +100,17 @@ SIGNATURES = {
     "w4a16_quantize_pack": ([_p, _i, _i, _i, _i, _i, _p, _p, _i, _p], _i),
     "w4a16_gemm": ([_p, _p, _i, _p, _p, _i, _i, _i, _p, _i, _p, ctypes.c_size_t, _p], _i),
     "w4a16_gemm_workspace_bytes": ([_i, _i, _i], ctypes.c_size_t),
+    "w4a16_paged_append": ([_p, _ll, _p, _ll, _p, _ll, _p, _p, _i, _i, _p, _p, _p, _i, _p, _p, _ll, _p], _i),
+    "w4a16_paged_attention": ([_p, _ll, _p, _p, _i, _i, _p, _p, ctypes.c_float, _p, _ll, _p, _sz, _p], _i),
+    "w4a16_paged_attention_workspace_bytes": ([_i, _i, _i], _sz),
+    "w4a16_pages_extend": ([_p, _p, _p, _i, _p, _p], _i),
+    "w4a16_pages_fork": ([_p, _p, _p, _p, _i, _p, _p, _sz, _p], _i),
+    "w4a16_pages_fork_scratch_bytes": ([_i], _sz),
+    "w4a16_pages_free": ([_p, _p, _i, _p, _p], _i),
+    "w4a16_pages_copy": ([_p, _p, _p, _i, _p], _i),
+    "w4a16_pages_compact": ([_p, _p, _p, _ll, _p, _p, _p, _p, _sz, _p], _i),
+    "w4a16_pages_compact_scratch_bytes": ([_i], _sz),
+    "w4a16_process_logits": ([_p, _p], _i),
     "w4a16_read_device_error": ([ctypes.POINTER(ctypes.c_int), _p], _i),
     "w4a16_status_string": ([_i], ctypes.c_char_p),
     "w4a16_last_error_string": ([], ctypes.c_char_p),

@@ -1,0 +1,326 @@
+"""Serving several sequences over a paged key-value cache.
+
+The reference decodes one sequence through the Hugging Face cache (benchmarks/end_to_end.py:
+24-42), and decode_attention here holds one sequence's cache as one block.  With several
+sequences of different lengths the cache is cut into pages of `page_size` positions:
+
+    k_pages, v_pages  fp16 or bf16 [pages, kv_heads, page_size, head_dim] (one layer's pool; any
+                      strides with the last dimension contiguous, so [pages, page_size, kv_heads,
+                      head_dim] storage is passed as its transpose(1, 2))
+    tables            int32 [sequences, width]: the pages of each sequence in order, -1 past the last
+    lengths           int32 [sequences]: positions held
+    refs              int32 [pages]: table entries that hold the page, 0 for a free one
+
+    paged_append      rotary embedding of new q and k, k and v written into their pages
+    paged_attention   attention of one new token per row over its sequence's pages
+    extend_sequences, fork_sequences, free_sequences, compact_pages, copy_pages
+                      the pages' bookkeeping, on the device
+    PagedKVCache      the tensors above for all layers of a model, with the calls as methods
+
+Everything is read on the device, launched on the current stream and can be captured in a CUDA
+graph; nothing is kept between calls.  Wrong dtypes, devices, shapes or layouts raise
+RuntimeError before anything is launched; indices are checked in the kernels (a bad page, position
+or sequence gives NaN, is skipped, or is refused, as each function says).
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .kernels import _need, _ptr, _stream
+
+_POOL_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _is_cuda(t):
+    return isinstance(t, torch.Tensor) and t.is_cuda
+
+
+def _pool(k_pages, v_pages):
+    """The C description of one layer's pool, checked."""
+    _need(_is_cuda(k_pages) and k_pages.dim() == 4 and k_pages.dtype in _POOL_DTYPES,
+          "k_pages must be an fp16 or bf16 CUDA tensor [pages, kv_heads, page_size, head_dim]")
+    _need(isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype == k_pages.dtype
+          and v_pages.shape == k_pages.shape and v_pages.stride() == k_pages.stride(),
+          "v_pages must have the device, dtype, shape and strides of k_pages")
+    pages, kv_heads, page_size, head_dim = k_pages.shape
+    sp, sh, st, sd = k_pages.stride()
+    _need(sd == 1, "the last dimension of the pages must be contiguous")
+    # a dimension of one entry may carry any stride
+    return _lib.PagePool(k_pages.data_ptr(), v_pages.data_ptr(), _POOL_DTYPES[k_pages.dtype], pages, kv_heads, page_size,
+                         head_dim, sp if pages > 1 else 8, sh if kv_heads > 1 else 8, st if page_size > 1 else 8)
+
+
+def _tables(tables, dev):
+    _need(isinstance(tables, torch.Tensor) and tables.device == dev and tables.dtype == torch.int32 and tables.dim() == 2
+          and (tables.stride(1) == 1 or tables.shape[1] <= 1),
+          f"tables must be an int32 [sequences, width] tensor on {dev} with contiguous rows")
+    return _lib.PageTables(tables.data_ptr(), tables.shape[0], tables.shape[1], tables.stride(0))
+
+
+def _index(t, n, name, dev):
+    _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == torch.int32 and t.dim() == 1
+          and t.is_contiguous() and (n is None or t.shape[0] == n),
+          f"{name} must be a contiguous int32 [{'n' if n is None else n}] tensor on {dev}")
+    return t.data_ptr()
+
+
+def _tokens(t, n, heads, head_dim, dtype, name, dev):
+    """(address, elements between tokens) of a [tokens, heads, head_dim] tensor whose tokens are
+    contiguous blocks (rows of a wider projection output will do)."""
+    _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == dtype and t.dim() == 3
+          and t.shape == (n, heads, head_dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim),
+          f"{name} must be a {dtype} [{n}, {heads}, {head_dim}] tensor on {dev}, contiguous within a token")
+    return t.data_ptr(), t.stride(0) if n > 1 else heads * head_dim
+
+
+def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=None, seqs=None, out=None):
+    """Rotary embedding of new tokens' q and k, and the write of k and v into the cache's pages.
+
+    q          [tokens, heads, head_dim] of the pool's dtype (rows of a wider tensor will do: the
+               q, k, v slices of one projection's output), or None to write the cache only
+    k, v       [tokens, kv_heads, head_dim]
+    positions  int32 [tokens]: each token's position in its sequence; negative for a padding token,
+               which writes nothing and whose q comes back zero
+    seqs       int32 [tokens]: each token's row of `tables` (default: token t is sequence t)
+    cos, sin   fp32 [>= positions, head_dim] rotate-half tables (both None: no rotation)
+    out        where the rotated q goes (default a new tensor; q itself will do)
+
+    Returns out.  A position past the tables' width or the angles, a sequence outside `tables` or a
+    page outside the pool writes nothing to the cache and gives NaN.  A (sequence, position) may
+    occur once per call."""
+    pool = _pool(k_pages, v_pages)
+    dev, dtype, d = k_pages.device, k_pages.dtype, k_pages.shape[3]
+    _need(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
+    n, kvh = k.shape[0], k_pages.shape[1]
+    kp, ks = _tokens(k, n, kvh, d, dtype, "k", dev)
+    vp, vs = _tokens(v, n, kvh, d, dtype, "v", dev)
+    pos = _index(positions, n, "positions", dev)
+    sq = _index(seqs, n, "seqs", dev) if seqs is not None else None
+    tab = _tables(tables, dev)
+    _need((cos is None) == (sin is None), "cos and sin go together")
+    if cos is not None:
+        for name, t in (("cos", cos), ("sin", sin)):
+            _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == torch.float32 and t.dim() == 2
+                  and t.shape == cos.shape and t.shape[1] == d and t.is_contiguous(),
+                  f"{name} must be a contiguous fp32 [positions, {d}] tensor on {dev}")
+    heads, qp, qs, op, os_ = 0, None, 0, None, 0
+    if q is not None:
+        _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [tokens, heads, head_dim]")
+        heads = q.shape[1]
+        qp, qs = _tokens(q, n, heads, d, dtype, "q", dev)
+        if out is None:
+            out = torch.empty((n, heads, d), dtype=dtype, device=dev)
+        op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
+    if n == 0:
+        return out
+    with torch.cuda.device(dev):
+        status = _lib.lib().w4a16_paged_append(
+            qp, qs, kp, ks, vp, vs, pos, sq, n, heads, ctypes.byref(tab), _ptr(cos), _ptr(sin),
+            cos.shape[0] if cos is not None else 0, ctypes.byref(pool), op, os_, _stream(dev))
+    _lib.check(status, "w4a16_paged_append")
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=None, out=None, workspace=None):
+    """Attention of one query token per row over the pages of its sequence:
+    out[t, h] = softmax_j(scale * q[t, h] . K[j, g]) V[j, g] over j < lengths[t], g = h // (heads // kv_heads).
+
+    q        [rows, heads, head_dim] of the pool's dtype (rows of a wider tensor will do)
+    lengths  int32 [rows]: positions each row attends to, its own token's included
+    seqs     int32 [rows]: each row's row of `tables` (default: row t is sequence t); several rows may
+             name one sequence, as the tokens of a prompt do with growing lengths
+    scale    default head_dim ** -0.5
+    workspace  a uint8 CUDA tensor of at least w4a16_paged_attention_workspace_bytes; default: one
+             allocated for the call, so calls on several streams or in several graphs do not share it
+
+    Returns out [rows, heads, head_dim].  A row of length <= 0 is zero; a length past the tables'
+    width, a sequence outside `tables` or a page outside the pool gives NaN."""
+    pool = _pool(k_pages, v_pages)
+    dev, dtype = k_pages.device, k_pages.dtype
+    kvh, d = k_pages.shape[1], k_pages.shape[3]
+    _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [rows, heads, head_dim]")
+    n, heads = q.shape[0], q.shape[1]
+    qp, qs = _tokens(q, n, heads, d, dtype, "q", dev)
+    _need(heads > 0 and heads % kvh == 0, f"{heads} query heads are not a multiple of {kvh} kv heads")
+    lens = _index(lengths, n, "lengths", dev)
+    sq = _index(seqs, n, "seqs", dev) if seqs is not None else None
+    tab = _tables(tables, dev)
+    if out is None:
+        out = torch.empty((n, heads, d), dtype=dtype, device=dev)
+    op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
+    if n == 0:
+        return out
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        if workspace is None:
+            workspace = torch.empty(L.w4a16_paged_attention_workspace_bytes(heads, kvh, d), dtype=torch.uint8, device=dev)
+        else:
+            _need(isinstance(workspace, torch.Tensor) and workspace.device == dev and workspace.dtype == torch.uint8
+                  and workspace.is_contiguous(), f"workspace must be a contiguous uint8 tensor on {dev}")
+        status = L.w4a16_paged_attention(qp, qs, lens, sq, n, heads, ctypes.byref(tab), ctypes.byref(pool),
+                                         float(d ** -0.5 if scale is None else scale), op, os_, workspace.data_ptr(),
+                                         workspace.numel(), _stream(dev))
+    _lib.check(status, "w4a16_paged_attention")
+    return out
+
+
+# ------------------------------------------------------------------------------ page bookkeeping
+
+def _state(tables, lengths, refs, page_size):
+    _need(_is_cuda(tables) and tables.dtype == torch.int32 and tables.dim() == 2 and tables.is_contiguous(),
+          "tables must be a contiguous int32 [sequences, width] CUDA tensor")
+    dev = tables.device
+    _index(lengths, tables.shape[0], "lengths", dev)
+    _index(refs, None, "refs", dev)
+    return _lib.PageState(tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), tables.shape[0], tables.shape[1],
+                          refs.shape[0], page_size, tables.shape[1])
+
+
+def _blocks(k_pages, v_pages):
+    """The C description of the pages' bytes in all layers, checked: [layers, pages, ...] or one
+    layer's [pages, kv_heads, page_size, head_dim], every page one dense block."""
+    _need(_is_cuda(k_pages) and k_pages.dim() in (4, 5), "k_pages must be a CUDA tensor [layers, pages, kv_heads, page_size, "
+          "head_dim] or [pages, kv_heads, page_size, head_dim]")
+    _need(isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype == k_pages.dtype
+          and v_pages.shape == k_pages.shape and v_pages.stride() == k_pages.stride(),
+          "v_pages must have the device, dtype, shape and strides of k_pages")
+    size, shape, stride = k_pages.element_size(), k_pages.shape, k_pages.stride()
+    layers, ls = (shape[0], stride[0]) if len(shape) == 5 else (1, 0)
+    pages, ps = shape[-4], stride[-4]
+    elements = 1
+    for st, n in sorted(zip(stride[-3:], shape[-3:])):  # dense in some order of its dimensions
+        _need(n == 1 or st == elements, "a page must be one dense block")
+        elements *= n
+    return _lib.PageBlocks(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, ls * size if layers > 1 else 0,
+                           (ps if pages > 1 else elements) * size, elements * size)
+
+
+def extend_sequences(tables, lengths, refs, seqs, counts, *, page_size):
+    """Sequence seqs[i] grows by counts[i] positions (int32 [n], n <= 1024) and receives the lowest free
+    pages that it needs for them; tables, lengths and refs are updated in place.
+
+    Returns ok, int32 [n]: 1, or 0 for a request that was refused and changed nothing (an index or
+    count out of range, more positions than the table's row holds, a sequence named by an earlier
+    request of the call, or no pages left: requests are served in order, and from the first that does
+    not fit on all that need pages are refused)."""
+    st = _state(tables, lengths, refs, page_size)
+    dev = tables.device
+    s = _index(seqs, None, "seqs", dev)
+    n = seqs.shape[0]
+    c = _index(counts, n, "counts", dev)
+    ok = torch.empty(n, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        status = _lib.lib().w4a16_pages_extend(ctypes.byref(st), s, c, n, ok.data_ptr(), _stream(dev))
+    _lib.check(status, "w4a16_pages_extend")
+    return ok
+
+
+def fork_sequences(k_pages, v_pages, tables, lengths, refs, src, dst):
+    """Sequence dst[i], which must be empty, becomes a copy of src[i] (int32 [n], n <= 1024): whole
+    pages are shared, a partly filled last page is copied in every layer to the lowest free page.
+    k_pages, v_pages: [layers, pages, kv_heads, page_size, head_dim] (or one layer's four dimensions).
+
+    Returns ok, int32 [n], as extend_sequences does; a dst that is not empty, is its own src or was
+    named by an earlier request is refused.  All requests see the state from before the call."""
+    b = _blocks(k_pages, v_pages)
+    st = _state(tables, lengths, refs, k_pages.shape[-2])
+    dev = tables.device
+    _need(k_pages.device == dev and refs.shape[0] == k_pages.shape[-4], f"refs must have one entry per page and k_pages be on {dev}")
+    s = _index(src, None, "src", dev)
+    n = src.shape[0]
+    t = _index(dst, n, "dst", dev)
+    ok = torch.empty(n, dtype=torch.int32, device=dev)
+    L = _lib.lib()
+    need = L.w4a16_pages_fork_scratch_bytes(n)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        status = L.w4a16_pages_fork(ctypes.byref(st), ctypes.byref(b), s, t, n, ok.data_ptr(), scratch.data_ptr(), need,
+                                    _stream(dev))
+    _lib.check(status, "w4a16_pages_fork")
+    return ok
+
+
+def free_sequences(tables, lengths, refs, seqs):
+    """Sequence seqs[i] (int32 [n]) gives up every page in its row and becomes empty; a page that no
+    row holds any more is free.  Returns ok, int32 [n]: 0 for an index out of range or named before."""
+    st = _state(tables, lengths, refs, 1)
+    dev = tables.device
+    s = _index(seqs, None, "seqs", dev)
+    n = seqs.shape[0]
+    ok = torch.empty(n, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        status = _lib.lib().w4a16_pages_free(ctypes.byref(st), s, n, ok.data_ptr(), _stream(dev))
+    _lib.check(status, "w4a16_pages_free")
+    return ok
+
+
+def copy_pages(k_pages, v_pages, src, dst):
+    """Copies page src[i] to page dst[i] in every layer (int32 [n]).  A pair with an index outside
+    the pool is skipped.  No page may be in both lists, or twice in dst."""
+    b = _blocks(k_pages, v_pages)
+    dev = k_pages.device
+    s = _index(src, None, "src", dev)
+    n = src.shape[0]
+    t = _index(dst, n, "dst", dev)
+    with torch.cuda.device(dev):
+        status = _lib.lib().w4a16_pages_copy(ctypes.byref(b), s, t, n, _stream(dev))
+    _lib.check(status, "w4a16_pages_copy")
+
+
+def compact_pages(k_pages, v_pages, tables, refs, *, inplace=True):
+    """Moves the live pages (refs > 0) to the front of the pool: with L of them, the k-th live page at
+    or above L goes to the k-th free page below L, and no other page moves.
+
+    Returns (tables, refs, moved): the tables and refs with the new page numbers (updated in place, or
+    new tensors with inplace=False), and the number of pages moved, int32 [1] on the device."""
+    b = _blocks(k_pages, v_pages)
+    dev = k_pages.device
+    _need(isinstance(tables, torch.Tensor) and tables.device == dev and tables.dtype == torch.int32 and tables.is_contiguous(),
+          f"tables must be a contiguous int32 tensor on {dev}")
+    r = _index(refs, k_pages.shape[-4], "refs", dev)
+    new_tables, new_refs = (tables, refs) if inplace else (torch.empty_like(tables), torch.empty_like(refs))
+    moved = torch.empty(1, dtype=torch.int32, device=dev)
+    L = _lib.lib()
+    need = L.w4a16_pages_compact_scratch_bytes(refs.shape[0])
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        status = L.w4a16_pages_compact(ctypes.byref(b), tables.data_ptr(), new_tables.data_ptr(), tables.numel(), r,
+                                       new_refs.data_ptr(), moved.data_ptr(), scratch.data_ptr(), need, _stream(dev))
+    _lib.check(status, "w4a16_pages_compact")
+    return new_tables, new_refs, moved
+
+
+class PagedKVCache:
+    """The paged cache of a model: k and v [layers, pages, kv_heads, page_size, head_dim], and the page
+    tables of `sequences` sequences of at most `max_len` positions."""
+
+    def __init__(self, layers, pages, sequences, max_len, *, kv_heads, head_dim, page_size=16, dtype=torch.float16,
+                 device="cuda"):
+        if page_size < 1 or page_size & (page_size - 1):
+            raise ValueError(f"page_size {page_size} is not a power of two")
+        dev = torch.device(device)
+        self.page_size = page_size
+        self.k = torch.zeros(layers, pages, kv_heads, page_size, head_dim, dtype=dtype, device=dev)
+        self.v = torch.zeros_like(self.k)
+        self.tables = torch.full((sequences, -(-max_len // page_size)), -1, dtype=torch.int32, device=dev)
+        self.lengths = torch.zeros(sequences, dtype=torch.int32, device=dev)
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
+
+    def extend(self, seqs, counts):
+        return extend_sequences(self.tables, self.lengths, self.refs, seqs, counts, page_size=self.page_size)
+
+    def fork(self, src, dst):
+        return fork_sequences(self.k, self.v, self.tables, self.lengths, self.refs, src, dst)
+
+    def free(self, seqs):
+        return free_sequences(self.tables, self.lengths, self.refs, seqs)
+
+    def compact(self):
+        return compact_pages(self.k, self.v, self.tables, self.refs)[2]
+
+    def append(self, layer, q, k, v, positions, *, cos=None, sin=None, seqs=None, out=None):
+        return paged_append(q, k, v, positions, self.tables, self.k[layer], self.v[layer], cos=cos, sin=sin, seqs=seqs, out=out)
+
+    def attention(self, layer, q, lengths, *, seqs=None, scale=None, out=None):
+        return paged_attention(q, self.k[layer], self.v[layer], self.tables, lengths, seqs=seqs, scale=scale, out=out)
