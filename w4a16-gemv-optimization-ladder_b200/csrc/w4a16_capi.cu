@@ -811,8 +811,9 @@ int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* leng
   int rc = check_pool(pool, &pl);
   if (rc == W4A16_OK) rc = check_tables(tables, &tb);
   if (rc != W4A16_OK) return rc;
-  if (rows < 0 || heads <= 0 || heads % pl.kv_heads) {
-    set_error("bad shape: %d rows, %d heads over %d kv heads", rows, heads, pl.kv_heads);
+  if (rows < 0 || heads <= 0 || heads % pl.kv_heads || ((long long)tb.width << pl.page_shift) > (1 << 30)) {
+    set_error("bad shape: %d rows, %d heads over %d kv heads, tables of %d pages (at most 2^30 positions)", rows, heads,
+              pl.kv_heads, tb.width);
     return W4A16_ERR_SHAPE;
   }
   if (rows == 0) return W4A16_OK;
