@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "w4a16_device.cuh"
@@ -98,18 +99,22 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppend a, const
 // ------------------------------------------------------------------------- attention
 //
 // Bound by the bytes of the keys and values: each is used for the few query heads of its kv
-// head only.  One pass over them with a running maximum and sum; the pages go straight from
-// global memory into the operand registers of m16n8k16 tensor-core products (no shared memory
-// in between), which the freedom to number the contracted index allows:
-//   S^T[position][head] = K Q^T    A = K: lane (g = lane / 4, j = lane % 4) loads 16 bytes of
+// head only.  One pass over them with a running maximum and sum.  Every warp copies its own
+// tiles of 16 (head_dim 64: 32) positions into its own ring of shared memory stages with
+// 16-byte asynchronous copies, so no barrier and no register holds bytes in flight, and reads
+// the operands of m16n8k16 tensor-core products with 16-byte shared loads, which the freedom
+// to number the contracted index allows:
+//   S^T[position][head] = K Q^T    A = K: lane (g = lane / 4, j = lane % 4) reads 16 bytes of
 //                                  positions g and g + 8 at dimensions 8j of each block of 32;
 //                                  these four words are the k = 2j, 2j+1, 2j+8, 2j+9 operands
 //                                  of two products, and Q is loaded by the same numbering
-//   O^T[dimension][head] = V^T P   A = V^T: the lane loads 16 bytes (dimensions 8g) of positions
+//   O^T[dimension][head] = V^T P   A = V^T: the lane reads 16 bytes (dimensions 8g) of positions
 //                                  2j, 2j+1, 2j+8, 2j+9 and pairs two positions with one byte
-//                                  permutation per word; P^T comes from S^T by two 8 x 8 matrix
-//                                  transpositions
-// The 8 (NH = 1) or 16 (NH = 2) query heads of a CTA are the n of the products.
+//                                  permutation per word; P^T comes from S^T by 8 x 8 matrix
+//                                  transpositions, in two 16-bit parts (value and remainder), so
+//                                  that the probabilities lose nothing to the type
+// The 16-byte chunks of a row are permuted by swizzle(row), which keeps both reads free of
+// bank conflicts.  The 8 (NH = 1) or 16 (NH = 2) query heads of a CTA are the n of the products.
 //
 // Work is shared out by a count of units of kUnit positions over all (row, kv head, block of
 // query heads) items, in that order: worker w (a CTA) takes units [w T / W, (w + 1) T / W) of
@@ -122,11 +127,17 @@ constexpr int kAttnMaxWorkers = 592;  // bounds the workspace: 148 SMs with 4 wo
 
 template <int D, int NH>
 struct AttnCfg {
-  static constexpr int kTiles = D == 64 ? 2 : 1;  // 16-position tiles a warp holds at once
+  static constexpr int kTiles = D == 64 ? 2 : 1;  // 16-position tiles of a stage
   static constexpr int kUnit = 16 * kTiles * kAttnWarps;
   static constexpr int kHeads = 8 * NH;
-  static constexpr int kPerSm = D == 64 ? (NH == 1 ? 4 : 3) : D == 128 ? (NH == 1 ? 3 : 2) : 2;
+  static constexpr int kStages = 3;
+  static constexpr int kPerSm = D == 256 ? 1 : 2;
   static constexpr int kSlot = kHeads * (D + 2);  // floats of a part: m, l, o per head
+  static constexpr int kHalf = 16 * kTiles * D * 2;  // bytes of a stage's keys, and of its values
+  static constexpr int kRing = kStages * 2 * kHalf;  // bytes of a warp's ring
+  // the rings; between two items the same memory holds the warps' parts
+  static constexpr int kSmem = kAttnWarps * kRing;
+  static_assert(kAttnWarps * kHeads * D * 4 <= kSmem, "the parts fit the rings");
 };
 
 struct AttnDesc {  // the item that worker w began and did not finish
@@ -159,12 +170,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
-// Keys and values are read once: past L1.
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// 16 bytes to shared memory, past L1 (they are read once); zeros where `any` is false.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool any) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(any ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Permutation of a row's 16-byte chunks within 128 bytes.  Rows 2i differ in bits 1 and 2 (the
+// reads of V take rows 0, 2, 4, 6 or 1, 3, 5, 7 at two neighbouring chunks), rows 2i and 2i + 1
+// in bit 2 (the reads of K take two neighbouring rows at four neighbouring chunks).
+__device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ ((row & 1) << 2); }
 
 template <typename T, int D, int NH>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
@@ -178,7 +195,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   __shared__ long long sh_total, sh_base, sh_warp[kAttnWarps];
   __shared__ int sh_row;
   __shared__ float sh_m[kAttnWarps][kHeads], sh_l[kAttnWarps][kHeads];
-  extern __shared__ float sh_o[];  // [warp][head][D]
+  extern __shared__ __align__(128) float sh_o[];  // the rings, then [warp][head][D]
+  const uint32_t ring = smem_addr(sh_o) + warp * C::kRing;
 
   grid_launch_dependents();  // the join waits for this kernel's end before it reads anything
   AttnDesc* desc = static_cast<AttnDesc*>(a.workspace);
@@ -272,65 +290,78 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       for (int i = 0; i < kVB * 4; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
 
-    // the page of position p + lane (p: the first position of this warp's tiles), -1 for none
+    // the page of position p + lane (p: the first position of a stage's tiles), -1 for none;
+    // a position that should have one and has not makes the item NaN
+    constexpr int kPos = 16 * kU;
+    bool bad = false;
+    const int end = min(len, t1 * C::kUnit);
     auto look_up = [&](int p) {
-      const int at = p + (lane & (16 * kU - 1));
-      if (at >= len || !seq_ok || (at >> pool.page_shift) >= tab.width) return -1;
-      const int page = __ldg(ids + (at >> pool.page_shift));
-      return page < 0 || page >= pool.pages ? -1 : page;
+      const int at = p + (lane & (kPos - 1));
+      int page = -1;
+      if (at < end) {
+        if (seq_ok && (at >> pool.page_shift) < tab.width) page = __ldg(ids + (at >> pool.page_shift));
+        if (page < 0 || page >= pool.pages) {
+          page = -1;
+          bad = true;
+        }
+      }
+      return page;
     };
     const int tmask = (1 << pool.page_shift) - 1;
-    auto place = [&](int page, int at) {  // element offset of position `at` of this kv head
-      return (size_t)page * pool.page_stride + (size_t)(at & tmask) * pool.token_stride;
-    };
-    uint4 k[kU][kB][2], v[kU][kVB][4];
-    auto load_k = [&](int p, int pages) {
+    constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows of one copy instruction
+    const int crow = lane / kChunks, chunk = lane % kChunks;
+    auto load = [&](int p, int pages, int stage) {
+      const uint32_t dst = ring + stage * 2 * C::kHalf;
 #pragma unroll
-      for (int t = 0; t < kU; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int i = 16 * t + 8 * h + g;
-          const int page = __shfl_sync(0xffffffffu, pages, i);
-          const T* src = kp + place(page, p + i) + 8 * j;
-          const uint32_t none = p + i < len ? 0x7fff7fffu : 0u;  // a bad page: NaN
-#pragma unroll
-          for (int b = 0; b < kB; ++b) k[t][b][h] = page >= 0 ? ld_stream(src + 32 * b) : make_uint4(none, none, none, none);
-        }
-    };
-    auto load_v = [&](int p, int pages) {
-#pragma unroll
-      for (int t = 0; t < kU; ++t)
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int i = 16 * t + 2 * j + (h & 1) + 8 * (h >> 1);
-          const int page = __shfl_sync(0xffffffffu, pages, i);
-          const T* src = vp + place(page, p + i) + 8 * g;
-#pragma unroll
-          for (int b = 0; b < kVB; ++b) v[t][b][h] = page >= 0 ? ld_stream(src + 64 * b) : make_uint4(0u, 0u, 0u, 0u);
-        }
+      for (int i = 0; i < kPos / kRows; ++i) {
+        const int r = i * kRows + crow;
+        const int page = __shfl_sync(0xffffffffu, pages, r);
+        const size_t at = (size_t)(page < 0 ? 0 : page) * pool.page_stride + (size_t)((p + r) & tmask) * pool.token_stride + 8 * chunk;
+        const uint32_t to = dst + r * (D * 2) + ((chunk & ~7) | ((chunk & 7) ^ swizzle(r))) * 16;
+        copy_async16(to, kp + at, page >= 0);
+        copy_async16(to + C::kHalf, vp + at, page >= 0);
+      }
     };
 
-    const int first = t0 * C::kUnit + warp * 16 * kU, end = min(len, t1 * C::kUnit);
+    const int first = t0 * C::kUnit + warp * kPos;
     int pages = look_up(first);
-    int pages_next = look_up(first + C::kUnit);
-    load_k(first, pages);
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) {  // a tile past the end is copied as zeros
+      load(first + i * C::kUnit, pages, i);
+      copies_commit();
+      pages = look_up(first + (i + 1) * C::kUnit);
+    }
+    int stage = 0;
     for (int p = first; p < end; p += C::kUnit) {
-      load_v(p, pages);
+      copies_wait<C::kStages - 2>();
+      __syncwarp();  // every lane's copies of this stage are in, its reads of the one before done
+      {
+        const int ahead = p + (C::kStages - 1) * C::kUnit, to = stage == 0 ? C::kStages - 1 : stage - 1;
+        if (ahead < end) {
+          load(ahead, pages, to);
+          pages = look_up(ahead + C::kUnit);
+        }
+        copies_commit();
+      }
+      const uint32_t kt = ring + stage * 2 * C::kHalf, vt = kt + C::kHalf;
+      stage = stage == C::kStages - 1 ? 0 : stage + 1;
       float s[NH][kU][4];
 #pragma unroll
-      for (int n = 0; n < NH; ++n)
+      for (int t = 0; t < kU; ++t) {
 #pragma unroll
-        for (int t = 0; t < kU; ++t) {
-          s[n][t][0] = s[n][t][1] = s[n][t][2] = s[n][t][3] = 0.f;
+        for (int n = 0; n < NH; ++n) s[n][t][0] = s[n][t][1] = s[n][t][2] = s[n][t][3] = 0.f;
 #pragma unroll
-          for (int b = 0; b < kB; ++b) {
-            mma16816<T>(s[n][t], k[t][b][0].x, k[t][b][1].x, k[t][b][0].y, k[t][b][1].y, q[n][b].x, q[n][b].y);
-            mma16816<T>(s[n][t], k[t][b][0].z, k[t][b][1].z, k[t][b][0].w, k[t][b][1].w, q[n][b].z, q[n][b].w);
+        for (int b = 0; b < kB; ++b) {
+          const uint32_t from = kt + (16 * t + g) * (D * 2) + (b >> 1) * 128 + (((b & 1) * 4 + j) ^ swizzle(g)) * 16;
+          const uint4 k0 = lds128(from), k1 = lds128(from + 8 * D * 2);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) {
+            mma16816<T>(s[n][t], k0.x, k1.x, k0.y, k1.y, q[n][b].x, q[n][b].y);
+            mma16816<T>(s[n][t], k0.z, k1.z, k0.w, k1.w, q[n][b].z, q[n][b].w);
           }
         }
-      pages = pages_next;
-      if (p + C::kUnit < end) load_k(p + C::kUnit, pages);
-      pages_next = look_up(p + 2 * C::kUnit);
+      }
+      uint32_t ph[NH][kU][2], pl[NH][kU][2];  // P^T: 16-bit values and remainders
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
         float mx[2] = {-INFINITY, -INFINITY};
@@ -338,7 +369,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
         for (int t = 0; t < kU; ++t)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {  // c: head 2j + (c & 1), position g + 8 (c >> 1)
-            s[n][t][c] = p + 16 * t + g + 8 * (c >> 1) < len ? s[n][t][c] * scale : -INFINITY;
+            s[n][t][c] = p + 16 * t + g + 8 * (c >> 1) < end ? s[n][t][c] * scale : -INFINITY;
             mx[c & 1] = fmaxf(mx[c & 1], s[n][t][c]);
           }
         float corr[2], low[2];
@@ -366,23 +397,47 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
             s[n][t][c] = exp2_fast(s[n][t][c] - low[c & 1]);
             l[n][c & 1] += s[n][t][c];
           }
-          // rounded to 16 bits for the product with V; the sum l keeps fp32
-          const uint32_t b0 = transpose_8x8(pack2<T>(s[n][t][0], s[n][t][1]));
-          const uint32_t b1 = transpose_8x8(pack2<T>(s[n][t][2], s[n][t][3]));
 #pragma unroll
-          for (int b = 0; b < kVB; ++b) {
-            const uint32_t w[4][4] = {{v[t][b][0].x, v[t][b][0].y, v[t][b][0].z, v[t][b][0].w},
-                                      {v[t][b][1].x, v[t][b][1].y, v[t][b][1].z, v[t][b][1].w},
-                                      {v[t][b][2].x, v[t][b][2].y, v[t][b][2].z, v[t][b][2].w},
-                                      {v[t][b][3].x, v[t][b][3].y, v[t][b][3].z, v[t][b][3].w}};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma16816<T>(o[n][b * 4 + i], prmt(w[0][i], w[1][i], 0x5410u), prmt(w[0][i], w[1][i], 0x7632u),
-                          prmt(w[2][i], w[3][i], 0x5410u), prmt(w[2][i], w[3][i], 0x7632u), b0, b1);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t hi = pack2<T>(s[n][t][2 * h], s[n][t][2 * h + 1]);
+            const float2 f = unpack2<T>(hi);
+            ph[n][t][h] = transpose_8x8(hi);
+            pl[n][t][h] = transpose_8x8(pack2<T>(s[n][t][2 * h] - f.x, s[n][t][2 * h + 1] - f.y));
           }
         }
       }
+#pragma unroll
+      for (int t = 0; t < kU; ++t)
+#pragma unroll
+        for (int b = 0; b < kVB; ++b) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int r = 2 * j + (h & 1);  // and + 8 for h >= 2: the same chunk permutation
+            const uint4 x = lds128(vt + (16 * t + r + 8 * (h >> 1)) * (D * 2) + b * 128 + (g ^ swizzle(r)) * 16);
+            w[h][0] = x.x;
+            w[h][1] = x.y;
+            w[h][2] = x.z;
+            w[h][3] = x.w;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a0 = prmt(w[0][i], w[1][i], 0x5410u), a1 = prmt(w[0][i], w[1][i], 0x7632u);
+            const uint32_t a2 = prmt(w[2][i], w[3][i], 0x5410u), a3 = prmt(w[2][i], w[3][i], 0x7632u);
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+              mma16816<T>(o[n][b * 4 + i], a0, a1, a2, a3, ph[n][t][0], ph[n][t][1]);
+              mma16816<T>(o[n][b * 4 + i], a0, a1, a2, a3, pl[n][t][0], pl[n][t][1]);
+            }
+          }
+        }
     }
+    copies_wait<0>();
+    if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll
+      for (int n = 0; n < NH; ++n) l[n][0] = l[n][1] = nan;
+    }
+    __syncthreads();  // no warp reads or fills its ring any more: the parts go there
 
     // the warps' parts, joined in shared memory
 #pragma unroll
@@ -531,9 +586,15 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   if (rc != W4A16_OK) return rc;
   const int group = a.heads / pool.kv_heads, blocks = (group + C::kHeads - 1) / C::kHeads;
   const int workers = sms * C::kPerSm < kAttnMaxWorkers ? sms * C::kPerSm : kAttnMaxWorkers;
-  constexpr size_t smem = (size_t)kAttnWarps * C::kHeads * D * 4;
-  static_assert(smem <= 40960, "with the static arrays under the 48 KB that need no opt-in");
-  k_paged_attention<T, D, NH><<<workers, kAttnWarps * 32, smem, stream>>>(a, pool, tab, group, blocks);
+  static std::atomic<uint64_t> configured{0};  // one bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(configured.load(std::memory_order_acquire) >> (dev & 63) & 1ull)) {
+    e = cudaFuncSetAttribute(k_paged_attention<T, D, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev, std::memory_order_acq_rel);
+  }
+  if (e != cudaSuccess) return launched("configuring k_paged_attention,", e);
+  k_paged_attention<T, D, NH><<<workers, kAttnWarps * 32, C::kSmem, stream>>>(a, pool, tab, group, blocks);
   const int rc2 = launched("k_paged_attention", cudaGetLastError());
   if (rc2 != W4A16_OK) return rc2;
   return launched("k_paged_join", launch_maybe_pdl(k_paged_join<T, D, NH>, dim3(workers), dim3(C::kHeads * D / 4), 0, stream, true, a,
