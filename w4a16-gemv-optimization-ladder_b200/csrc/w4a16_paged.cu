@@ -135,9 +135,7 @@ struct AttnCfg {
   static constexpr int kSlot = kHeads * (D + 2);  // floats of a part: m, l, o per head
   static constexpr int kHalf = 16 * kTiles * D * 2;  // bytes of a stage's keys, and of its values
   static constexpr int kRing = kStages * 2 * kHalf;  // bytes of a warp's ring
-  // the rings; between two items the same memory holds the warps' parts
-  static constexpr int kSmem = kAttnWarps * kRing;
-  static_assert(kAttnWarps * kHeads * D * 4 <= kSmem, "the parts fit the rings");
+  static constexpr int kSmem = kAttnWarps * (kRing + 8 * D * 4);  // the rings, then the warps' parts of 8 heads
 };
 
 struct AttnDesc {  // the item that worker w began and did not finish
@@ -192,11 +190,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   const int worker = blockIdx.x, workers = gridDim.x;
   const int items = pool.kv_heads * blocks;
   const float nan = __int_as_float(0x7fc00000);
-  __shared__ long long sh_total, sh_base, sh_warp[kAttnWarps];
+  __shared__ long long sh_base, sh_warp[kAttnWarps];
   __shared__ int sh_row;
-  __shared__ float sh_m[kAttnWarps][kHeads], sh_l[kAttnWarps][kHeads];
-  extern __shared__ __align__(128) float sh_o[];  // the rings, then [warp][head][D]
-  const uint32_t ring = smem_addr(sh_o) + warp * C::kRing;
+  __shared__ float sh_m[kAttnWarps][8], sh_l[kAttnWarps][8];
+  extern __shared__ __align__(128) uint8_t sh_raw[];
+  const uint32_t ring = smem_addr(sh_raw) + warp * C::kRing;
+  float* sh_o = reinterpret_cast<float*>(sh_raw + kAttnWarps * C::kRing);  // [warp][8][D]
 
   grid_launch_dependents();  // the join waits for this kernel's end before it reads anything
   AttnDesc* desc = static_cast<AttnDesc*>(a.workspace);
@@ -251,26 +250,93 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
         reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)r * a.out_stride)[e] = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
 
-  int row = sh_row;
-  long long base = sh_base;
+  if (u0 >= u1) return;
   const float scale = a.scale * 1.4426950408889634f;  // probabilities as powers of two
-  for (long long u = u0; u < u1;) {
-    int len = length(row), nt = tiles(len);
-    while (u >= base + (long long)nt * items) {  // on to the next row that has units
-      base += (long long)nt * items;
-      ++row;
-      len = length(row);
-      nt = tiles(len);
+  constexpr int kPos = 16 * kU;                       // positions of a stage
+
+  // A span: the tiles [t0, t1) of one item that the worker takes in a row.
+  struct Span {
+    long long base;  // units before the row
+    int row, len, nt, item, t0, t1;
+  };
+  auto open = [&](Span& sp, long long u) {  // the span that begins at unit u; sp holds an earlier one
+    while (u >= sp.base + (long long)sp.nt * items) {
+      sp.base += (long long)sp.nt * items;
+      ++sp.row;
+      sp.len = length(sp.row);
+      sp.nt = tiles(sp.len);
     }
-    const int item = (int)((u - base) / nt), t0 = (int)((u - base) % nt);
-    const int t1 = (int)min((long long)nt, t0 + (u1 - u));
+    sp.item = (int)((u - sp.base) / sp.nt);
+    sp.t0 = (int)((u - sp.base) % sp.nt);
+    sp.t1 = (int)min((long long)sp.nt, sp.t0 + (u1 - u));
+  };
+  Span cur;
+  cur.base = sh_base;
+  cur.row = sh_row;
+  cur.len = length(cur.row);
+  cur.nt = tiles(cur.len);
+  cur.t0 = cur.t1 = cur.item = 0;
+
+  // Copies run kStages - 1 units ahead of the products, across items, and the page numbers one
+  // unit ahead of the copies.
+  Span ahead = cur;
+  long long ahead_u = u0;
+  int ahead_t = 0, pos = 0, page = -1;  // pos, page, head_off: of the unit to be copied next
+  size_t head_off = 0;
+  const int* ids = tab.ids;
+  bool seq_ok = false;
+  // page of position pos + lane: -1 for none, -2 where a position has none and should
+  auto look_up = [&]() {
+    page = -1;
+    if (ahead_u >= u1) return;
+    if (ahead_t == ahead.t1) {
+      open(ahead, ahead_u);
+      ahead_t = ahead.t0;
+      const int seq = a.seqs ? __ldg(a.seqs + ahead.row) : ahead.row;
+      seq_ok = seq >= 0 && seq < tab.rows;
+      ids = tab.ids + (seq_ok ? (size_t)seq * tab.stride : 0);
+      head_off = (size_t)(ahead.item / blocks) * pool.head_stride;
+    }
+    pos = ahead_t * C::kUnit + warp * kPos;
+    const int at = pos + (lane & (kPos - 1));
+    if (at < ahead.len) {
+      if (seq_ok && (at >> pool.page_shift) < tab.width) page = __ldg(ids + (at >> pool.page_shift));
+      if (page < 0 || page >= pool.pages) page = -2;
+    }
+    ++ahead_t;
+    ++ahead_u;
+  };
+  const int tmask = (1 << pool.page_shift) - 1;
+  constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows of one copy instruction
+  const int crow = lane / kChunks, chunk = lane % kChunks;
+  unsigned bad = 0;  // bit: the stage holds a position without a page
+  auto load = [&](int stage) {
+    const uint32_t dst = ring + stage * 2 * C::kHalf;
+    bad = (bad & ~(1u << stage)) | (page == -2 ? 1u << stage : 0u);
+#pragma unroll
+    for (int i = 0; i < kPos / kRows; ++i) {
+      const int r = i * kRows + crow;
+      const int pg = __shfl_sync(0xffffffffu, page, r);
+      const size_t at = (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)((pos + r) & tmask) * pool.token_stride + head_off + 8 * chunk;
+      const uint32_t to = dst + r * (D * 2) + ((chunk & ~7) | ((chunk & 7) ^ swizzle(r))) * 16;
+      copy_async16(to, static_cast<const T*>(pool.k) + at, pg >= 0);
+      copy_async16(to + C::kHalf, static_cast<const T*>(pool.v) + at, pg >= 0);
+    }
+    copies_commit();
+  };
+  ahead_t = ahead.t1;  // open a span at the first call
+  look_up();
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) {  // units past the last are copied as zeros
+    load(i);
+    look_up();
+  }
+  int stage = 0;
+  for (long long u = u0; u < u1;) {
+    open(cur, u);
+    const int row = cur.row, item = cur.item, t0 = cur.t0, t1 = cur.t1, len = cur.len, nt = cur.nt;
     const int kvh = item / blocks, h0 = kvh * group + (item % blocks) * kHeads;
     const int nheads = min(kHeads, group - (item % blocks) * kHeads);
-    const int seq = a.seqs ? __ldg(a.seqs + row) : row;
-    const bool seq_ok = seq >= 0 && seq < tab.rows;
-    const int* ids = tab.ids + (seq_ok ? (size_t)seq * tab.stride : 0);
-    const T* kp = static_cast<const T*>(pool.k) + (size_t)kvh * pool.head_stride;
-    const T* vp = static_cast<const T*>(pool.v) + (size_t)kvh * pool.head_stride;
 
     uint4 q[NH][kB];
 #pragma unroll
@@ -290,61 +356,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       for (int i = 0; i < kVB * 4; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
 
-    // the page of position p + lane (p: the first position of a stage's tiles), -1 for none;
-    // a position that should have one and has not makes the item NaN
-    constexpr int kPos = 16 * kU;
-    bool bad = false;
-    const int end = min(len, t1 * C::kUnit);
-    auto look_up = [&](int p) {
-      const int at = p + (lane & (kPos - 1));
-      int page = -1;
-      if (at < end) {
-        if (seq_ok && (at >> pool.page_shift) < tab.width) page = __ldg(ids + (at >> pool.page_shift));
-        if (page < 0 || page >= pool.pages) {
-          page = -1;
-          bad = true;
-        }
-      }
-      return page;
-    };
-    const int tmask = (1 << pool.page_shift) - 1;
-    constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows of one copy instruction
-    const int crow = lane / kChunks, chunk = lane % kChunks;
-    auto load = [&](int p, int pages, int stage) {
-      const uint32_t dst = ring + stage * 2 * C::kHalf;
-#pragma unroll
-      for (int i = 0; i < kPos / kRows; ++i) {
-        const int r = i * kRows + crow;
-        const int page = __shfl_sync(0xffffffffu, pages, r);
-        const size_t at = (size_t)(page < 0 ? 0 : page) * pool.page_stride + (size_t)((p + r) & tmask) * pool.token_stride + 8 * chunk;
-        const uint32_t to = dst + r * (D * 2) + ((chunk & ~7) | ((chunk & 7) ^ swizzle(r))) * 16;
-        copy_async16(to, kp + at, page >= 0);
-        copy_async16(to + C::kHalf, vp + at, page >= 0);
-      }
-    };
-
-    const int first = t0 * C::kUnit + warp * kPos;
-    int pages = look_up(first);
-#pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) {  // a tile past the end is copied as zeros
-      load(first + i * C::kUnit, pages, i);
-      copies_commit();
-      pages = look_up(first + (i + 1) * C::kUnit);
-    }
-    int stage = 0;
-    for (int p = first; p < end; p += C::kUnit) {
+    bool no_page = false;
+    for (int tile = t0; tile < t1; ++tile) {
       copies_wait<C::kStages - 2>();
       __syncwarp();  // every lane's copies of this stage are in, its reads of the one before done
-      {
-        const int ahead = p + (C::kStages - 1) * C::kUnit, to = stage == 0 ? C::kStages - 1 : stage - 1;
-        if (ahead < end) {
-          load(ahead, pages, to);
-          pages = look_up(ahead + C::kUnit);
-        }
-        copies_commit();
-      }
+      load(stage == 0 ? C::kStages - 1 : stage - 1);
+      look_up();
+      no_page |= (bad >> stage & 1u) != 0;
       const uint32_t kt = ring + stage * 2 * C::kHalf, vt = kt + C::kHalf;
       stage = stage == C::kStages - 1 ? 0 : stage + 1;
+      const int p = tile * C::kUnit + warp * kPos;
+      if (p >= len) continue;  // the item's last unit may leave this warp none
       float s[NH][kU][4];
 #pragma unroll
       for (int t = 0; t < kU; ++t) {
@@ -369,7 +391,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
         for (int t = 0; t < kU; ++t)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {  // c: head 2j + (c & 1), position g + 8 (c >> 1)
-            s[n][t][c] = p + 16 * t + g + 8 * (c >> 1) < end ? s[n][t][c] * scale : -INFINITY;
+            s[n][t][c] = p + 16 * t + g + 8 * (c >> 1) < len ? s[n][t][c] * scale : -INFINITY;
             mx[c & 1] = fmaxf(mx[c & 1], s[n][t][c]);
           }
         float corr[2], low[2];
@@ -432,74 +454,74 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
           }
         }
     }
-    copies_wait<0>();
-    if (__any_sync(0xffffffffu, bad)) {
+    if (__any_sync(0xffffffffu, no_page)) {
 #pragma unroll
       for (int n = 0; n < NH; ++n) l[n][0] = l[n][1] = nan;
     }
-    __syncthreads();  // no warp reads or fills its ring any more: the parts go there
 
-    // the warps' parts, joined in shared memory
+    // the warps' parts, joined in shared memory, 8 heads at a time
+    const bool whole = t0 == 0 && t1 == nt;
+    float* slot = slots + (size_t)(2 * worker + (t0 == 0 ? 1 : 0)) * C::kSlot;
 #pragma unroll
-    for (int n = 0; n < NH; ++n)
+    for (int n = 0; n < NH; ++n) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
-        const int head = 8 * n + 2 * j + c;
+        const int head = 2 * j + c;
         if (g == 0) {
           sh_m[warp][head] = m[n][c];
           sh_l[warp][head] = l[n][c];
         }
 #pragma unroll
         for (int b = 0; b < kVB; ++b) {
-          float4* dst = reinterpret_cast<float4*>(sh_o + ((size_t)warp * kHeads + head) * D + 64 * b + 8 * g);
+          float4* dst = reinterpret_cast<float4*>(sh_o + (warp * 8 + head) * D + 64 * b + 8 * g);
           dst[0] = make_float4(o[n][4 * b][c], o[n][4 * b][2 + c], o[n][4 * b + 1][c], o[n][4 * b + 1][2 + c]);
           dst[1] = make_float4(o[n][4 * b + 2][c], o[n][4 * b + 2][2 + c], o[n][4 * b + 3][c], o[n][4 * b + 3][2 + c]);
         }
       }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == nt;
-    float* slot = slots + (size_t)(2 * worker + (t0 == 0 ? 1 : 0)) * C::kSlot;
-    for (int e = threadIdx.x; e < nheads * (D / 4); e += kThreads) {
-      const int head = e / (D / 4), d = (e % (D / 4)) * 4;
-      float mm = sh_m[0][head], ll = 0.f;
+      __syncthreads();
+      for (int e = threadIdx.x; e < min(8, nheads - 8 * n) * (D / 4); e += kThreads) {
+        const int h = e / (D / 4), d = (e % (D / 4)) * 4, head = 8 * n + h;
+        float mm = sh_m[0][h], ll = 0.f;
 #pragma unroll
-      for (int w = 1; w < kAttnWarps; ++w) mm = fmaxf(mm, sh_m[w][head]);
-      const float low = mm == -INFINITY ? 0.f : mm;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 1; w < kAttnWarps; ++w) mm = fmaxf(mm, sh_m[w][h]);
+        const float low = mm == -INFINITY ? 0.f : mm;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        const float f = exp2_fast(sh_m[w][head] - low);
-        const float4 x = *reinterpret_cast<const float4*>(sh_o + ((size_t)w * kHeads + head) * D + d);
-        ll = fmaf(sh_l[w][head], f, ll);
-        acc.x = fmaf(x.x, f, acc.x);
-        acc.y = fmaf(x.y, f, acc.y);
-        acc.z = fmaf(x.z, f, acc.z);
-        acc.w = fmaf(x.w, f, acc.w);
-      }
-      if (whole) {
-        uint2 r;
-        r.x = pack2<T>(acc.x / ll, acc.y / ll);
-        r.y = pack2<T>(acc.z / ll, acc.w / ll);
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (size_t)row * a.out_stride + (size_t)(h0 + head) * D + d) = r;
-      } else {
-        *reinterpret_cast<float4*>(slot + 2 * kHeads + head * D + d) = acc;
-        if (d == 0) {
-          slot[head] = mm;
-          slot[kHeads + head] = ll;
+        for (int w = 0; w < kAttnWarps; ++w) {
+          const float f = exp2_fast(sh_m[w][h] - low);
+          const float4 x = *reinterpret_cast<const float4*>(sh_o + (w * 8 + h) * D + d);
+          ll = fmaf(sh_l[w][h], f, ll);
+          acc.x = fmaf(x.x, f, acc.x);
+          acc.y = fmaf(x.y, f, acc.y);
+          acc.z = fmaf(x.z, f, acc.z);
+          acc.w = fmaf(x.w, f, acc.w);
+        }
+        if (whole) {
+          uint2 r;
+          r.x = pack2<T>(acc.x / ll, acc.y / ll);
+          r.y = pack2<T>(acc.z / ll, acc.w / ll);
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (size_t)row * a.out_stride + (size_t)(h0 + head) * D + d) = r;
+        } else {
+          *reinterpret_cast<float4*>(slot + 2 * kHeads + head * D + d) = acc;
+          if (d == 0) {
+            slot[head] = mm;
+            slot[kHeads + head] = ll;
+          }
         }
       }
+      __syncthreads();  // the parts' memory is free again
     }
     if (!whole && t0 == 0 && threadIdx.x == 0) {
-      const long long last = base + (long long)(item + 1) * nt - 1;  // the item's last unit
+      const long long last = cur.base + (long long)(item + 1) * nt - 1;  // the item's last unit
       desc[worker].row = row;
       desc[worker].item = item;
       desc[worker].parts = (int)(((last + 1) * used - 1) / total) - worker + 1;
     }
-    __syncthreads();  // shared memory is free for the next item
     u += t1 - t0;
   }
+  copies_wait<0>();
 }
 
 // Joins the parts of the item that worker blockIdx.x began, in the workers' order.
