@@ -116,29 +116,31 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppend a, const
 // The 16-byte chunks of a row are permuted by swizzle(row), which keeps both reads free of
 // bank conflicts.  The 8 (NH = 1) or 16 (NH = 2) query heads of a CTA are the n of the products.
 //
-// Work is shared out by a count of units of kUnit positions over all (row, kv head, block of
-// query heads) items, in that order: worker w (a CTA) takes units [w T / W, (w + 1) T / W) of
-// the T there are (W workers, no more than T), wherever that cuts an item.  The lengths are read on the device, so every
-// worker first sums them up.  An item that lies within one worker is finished there; the parts
-// of one that was cut go to the workspace (slot 2w + 1 if the part begins the item, else 2w)
-// and are joined by k_paged_join.
+// Work is shared out by a count of units over all (row, kv head, block of query heads) items, in
+// that order: each worker takes an equal run of them, wherever that cuts an item.  With an item for every
+// warp of the grid a worker is a warp and a unit one stage of positions, so the warps run
+// without a barrier; with fewer, which warps would cut into many parts, a worker is a CTA, a
+// unit one stage of each warp, and the CTA joins its warps' parts itself (256 rows of up to 200
+// positions, 2048 items: 34 us by warps, 42 by CTAs; 32 rows of up to 4096, 256 items: 55 and 53).  The lengths are read on the device, so every CTA first sums them up.  An item
+// that lies within one worker is finished there; the parts of one that was cut go to the
+// workspace (slot 2w + 1 if the part begins the item, else 2w) and are joined by k_paged_join.
 constexpr int kAttnWarps = 4;
-constexpr int kAttnMaxWorkers = 592;  // bounds the workspace: 148 SMs with 4 workers
+constexpr int kAttnMaxCtas = 296;  // bounds the workspace: 148 SMs with 2 CTAs
 
 template <int D, int NH>
 struct AttnCfg {
   static constexpr int kTiles = D == 64 ? 2 : 1;  // 16-position tiles of a stage
-  static constexpr int kUnit = 16 * kTiles * kAttnWarps;
+  static constexpr int kPos = 16 * kTiles;        // positions of a stage
   static constexpr int kHeads = 8 * NH;
   static constexpr int kStages = 3;
   static constexpr int kPerSm = D == 256 ? 1 : 2;
   static constexpr int kSlot = kHeads * (D + 2);  // floats of a part: m, l, o per head
-  static constexpr int kHalf = 16 * kTiles * D * 2;  // bytes of a stage's keys, and of its values
+  static constexpr int kHalf = kPos * D * 2;      // bytes of a stage's keys, and of its values
   static constexpr int kRing = kStages * 2 * kHalf;  // bytes of a warp's ring
   static constexpr int kSmem = kAttnWarps * (kRing + 8 * D * 4);  // the rings, then the warps' parts of 8 heads
 };
 
-struct AttnDesc {  // the item that worker w began and did not finish
+struct __align__(16) AttnDesc {  // the item that worker w began and did not finish
   int row, item, parts, pad;
 };
 
@@ -181,17 +183,25 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 // in bit 2 (the reads of K take two neighbouring rows at four neighbouring chunks).
 __device__ __forceinline__ int swizzle(int row) { return (row & 7) ^ ((row & 1) << 2); }
 
+// a / b for 0 <= a, 0 < b: 64-bit divisions are several times slower than 32-bit ones.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
 template <typename T, int D, int NH>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
-    k_paged_attention(const PagedAttention a, const PagedPool pool, const PagedTables tab, const int group, const int blocks) {
+    k_paged_attention(const PagedAttention a, const PagedPool pool, const PagedTables tab, const int group, const int blocks,
+                      const bool coop) {
   using C = AttnCfg<D, NH>;
-  constexpr int kB = D / 32, kVB = D / 64, kU = C::kTiles, kHeads = C::kHeads, kThreads = kAttnWarps * 32;
+  constexpr int kB = D / 32, kVB = D / 64, kU = C::kTiles, kHeads = C::kHeads, kThreads = kAttnWarps * 32, kPos = C::kPos;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-  const int worker = blockIdx.x, workers = gridDim.x;
+  const int workers = coop ? gridDim.x : gridDim.x * kAttnWarps;
+  const int worker = coop ? blockIdx.x : blockIdx.x * kAttnWarps + warp;
+  const int unit = coop ? kPos * kAttnWarps : kPos, shift = coop ? warp * kPos : 0;  // this warp's stage of a unit
   const int items = pool.kv_heads * blocks;
   const float nan = __int_as_float(0x7fc00000);
-  __shared__ long long sh_base, sh_warp[kAttnWarps];
-  __shared__ int sh_row;
+  __shared__ long long sh_base[kAttnWarps], sh_warp[kAttnWarps];
+  __shared__ int sh_row[kAttnWarps];
   __shared__ float sh_m[kAttnWarps][8], sh_l[kAttnWarps][8];
   extern __shared__ __align__(128) uint8_t sh_raw[];
   const uint32_t ring = smem_addr(sh_raw) + warp * C::kRing;
@@ -199,16 +209,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
 
   grid_launch_dependents();  // the join waits for this kernel's end before it reads anything
   AttnDesc* desc = static_cast<AttnDesc*>(a.workspace);
-  float* slots = reinterpret_cast<float*>(desc + kAttnMaxWorkers);
+  float* slots = reinterpret_cast<float*>(desc + kAttnMaxCtas * kAttnWarps);
   const long long cap = (long long)tab.width << pool.page_shift;
   // a length past the tables keeps one position there, which has no page: NaN
   auto length = [&](int row) {
     const int n = __ldg(a.lengths + row);
     return n <= 0 ? 0 : n > cap ? (int)(cap + 1) : n;
   };
-  auto tiles = [](int len) { return (len + C::kUnit - 1) / C::kUnit; };
+  auto tiles = [&](int len) { return (len + unit - 1) / unit; };
 
-  // the units of all rows, and the row that holds this worker's first one
+  // the units of all rows, and the row that holds each worker's first one
   const int per = (a.rows + kThreads - 1) / kThreads;
   const int r0 = min(a.rows, (int)threadIdx.x * per), r1 = min(a.rows, r0 + per);
   long long sum = 0;
@@ -221,83 +231,90 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     if (lane >= o) inc += n;
   }
   if (lane == 31) sh_warp[warp] = inc;
-  if (threadIdx.x == 0) sh_row = a.rows;
   __syncthreads();
   long long before = inc - sum, total = 0;
   for (int w = 0; w < kAttnWarps; ++w) {
     if (w < warp) before += sh_warp[w];
     total += sh_warp[w];
   }
-  // every worker in use has a unit, so the parts of an item lie with consecutive workers
-  const long long used = total < workers ? total : workers;
-  const long long u0 = worker < used ? worker * total / used : 0, u1 = worker < used ? (worker + 1LL) * total / used : 0;
-  if (u0 < u1 && before <= u0 && u0 < before + sum) {  // one thread
-    long long base = before;
-    int r = r0;
-    for (;; ++r) {
-      const long long n = (long long)tiles(length(r)) * items;
-      if (u0 < base + n) break;
-      base += n;
+  // every worker in use has a unit, so the parts of an item lie with consecutive workers: the
+  // first `more` of them take each + 1 units, the others each
+  const int used = total < workers ? (int)total : workers;
+  const long long each = used ? divide(total, used) : 0;
+  const int more = (int)(total - each * used);
+  auto first_unit = [&](int w) { return w < used ? w * each + min(w, more) : total; };
+  for (int w = 0; w < (coop ? 1 : kAttnWarps); ++w) {
+    const long long u = first_unit(coop ? blockIdx.x : blockIdx.x * kAttnWarps + w);
+    if (u < total && before <= u && u < before + sum) {  // one thread
+      long long base = before;
+      int r = r0;
+      for (;; ++r) {
+        const long long n = (long long)tiles(length(r)) * items;
+        if (u < base + n) break;
+        base += n;
+      }
+      sh_row[w] = r;
+      sh_base[w] = base;
     }
-    sh_row = r;
-    sh_base = base;
   }
-  if (threadIdx.x == 0) desc[worker].parts = 0;
+  if (coop ? threadIdx.x == 0 : lane == 0) desc[worker].parts = 0;
   // rows of no positions are zero
-  for (int r = worker; r < a.rows; r += workers)
+  for (int r = blockIdx.x; r < a.rows; r += gridDim.x)
     if (length(r) == 0)
-      for (int e = threadIdx.x; e < items / blocks * group * D / 8; e += kThreads)
+      for (int e = threadIdx.x; e < a.heads * D / 8; e += kThreads)
         reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)r * a.out_stride)[e] = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
-
-  if (u0 >= u1) return;
+  const long long u0 = first_unit(worker), u1 = worker + 1 < used ? first_unit(worker + 1) : total;
+  if (u0 >= u1) return;  // the whole CTA if it works as one
   const float scale = a.scale * 1.4426950408889634f;  // probabilities as powers of two
-  constexpr int kPos = 16 * kU;                       // positions of a stage
 
   // A span: the tiles [t0, t1) of one item that the worker takes in a row.
   struct Span {
-    long long base;  // units before the row
     int row, len, nt, item, t0, t1;
   };
-  auto open = [&](Span& sp, long long u) {  // the span that begins at unit u; sp holds an earlier one
-    while (u >= sp.base + (long long)sp.nt * items) {
-      sp.base += (long long)sp.nt * items;
-      ++sp.row;
-      sp.len = length(sp.row);
-      sp.nt = tiles(sp.len);
-    }
-    sp.item = (int)((u - sp.base) / sp.nt);
-    sp.t0 = (int)((u - sp.base) % sp.nt);
-    sp.t1 = (int)min((long long)sp.nt, sp.t0 + (u1 - u));
-  };
   Span cur;
-  cur.base = sh_base;
-  cur.row = sh_row;
+  long long base = sh_base[coop ? 0 : warp];  // units before the row of cur
+  cur.row = sh_row[coop ? 0 : warp];
   cur.len = length(cur.row);
   cur.nt = tiles(cur.len);
-  cur.t0 = cur.t1 = cur.item = 0;
+  cur.item = (int)divide(u0 - base, cur.nt);
+  cur.t0 = (int)(u0 - base - (long long)cur.item * cur.nt);
+  cur.t1 = (int)min((long long)cur.nt, cur.t0 + (u1 - u0));
+  auto next_span = [&](Span& sp, long long u) {  // the span that begins at unit u < u1, where sp ends
+    sp.t0 = 0;
+    if (++sp.item == items) {
+      sp.item = 0;
+      do sp.len = length(++sp.row);
+      while (sp.len == 0);
+      sp.nt = tiles(sp.len);
+    }
+    sp.t1 = (int)min((long long)sp.nt, u1 - u);
+  };
 
   // Copies run kStages - 1 units ahead of the products, across items, and the page numbers one
   // unit ahead of the copies.
   Span ahead = cur;
   long long ahead_u = u0;
-  int ahead_t = 0, pos = 0, page = -1;  // pos, page, head_off: of the unit to be copied next
+  int ahead_t = ahead.t0, pos = 0, page = -1;  // pos, page, head_off: of the unit to be copied next
   size_t head_off = 0;
   const int* ids = tab.ids;
   bool seq_ok = false;
+  auto enter = [&]() {
+    const int seq = a.seqs ? __ldg(a.seqs + ahead.row) : ahead.row;
+    seq_ok = seq >= 0 && seq < tab.rows;
+    ids = tab.ids + (seq_ok ? (size_t)seq * tab.stride : 0);
+    head_off = (size_t)(ahead.item / blocks) * pool.head_stride;
+  };
   // page of position pos + lane: -1 for none, -2 where a position has none and should
   auto look_up = [&]() {
     page = -1;
     if (ahead_u >= u1) return;
     if (ahead_t == ahead.t1) {
-      open(ahead, ahead_u);
-      ahead_t = ahead.t0;
-      const int seq = a.seqs ? __ldg(a.seqs + ahead.row) : ahead.row;
-      seq_ok = seq >= 0 && seq < tab.rows;
-      ids = tab.ids + (seq_ok ? (size_t)seq * tab.stride : 0);
-      head_off = (size_t)(ahead.item / blocks) * pool.head_stride;
+      next_span(ahead, ahead_u);
+      ahead_t = 0;
+      enter();
     }
-    pos = ahead_t * C::kUnit + warp * kPos;
+    pos = ahead_t * unit + shift;
     const int at = pos + (lane & (kPos - 1));
     if (at < ahead.len) {
       if (seq_ok && (at >> pool.page_shift) < tab.width) page = __ldg(ids + (at >> pool.page_shift));
@@ -324,7 +341,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     }
     copies_commit();
   };
-  ahead_t = ahead.t1;  // open a span at the first call
+  enter();
   look_up();
 #pragma unroll
   for (int i = 0; i < C::kStages - 1; ++i) {  // units past the last are copied as zeros
@@ -332,8 +349,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     look_up();
   }
   int stage = 0;
-  for (long long u = u0; u < u1;) {
-    open(cur, u);
+  for (long long u = u0;;) {
     const int row = cur.row, item = cur.item, t0 = cur.t0, t1 = cur.t1, len = cur.len, nt = cur.nt;
     const int kvh = item / blocks, h0 = kvh * group + (item % blocks) * kHeads;
     const int nheads = min(kHeads, group - (item % blocks) * kHeads);
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       no_page |= (bad >> stage & 1u) != 0;
       const uint32_t kt = ring + stage * 2 * C::kHalf, vt = kt + C::kHalf;
       stage = stage == C::kStages - 1 ? 0 : stage + 1;
-      const int p = tile * C::kUnit + warp * kPos;
+      const int p = tile * unit + shift;
       if (p >= len) continue;  // the item's last unit may leave this warp none
       float s[NH][kU][4];
 #pragma unroll
@@ -459,15 +475,50 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       for (int n = 0; n < NH; ++n) l[n][0] = l[n][1] = nan;
     }
 
-    // the warps' parts, joined in shared memory, 8 heads at a time
     const bool whole = t0 == 0 && t1 == nt;
     float* slot = slots + (size_t)(2 * worker + (t0 == 0 ? 1 : 0)) * C::kSlot;
+    T* out = static_cast<T*>(a.out) + (size_t)row * a.out_stride + (size_t)h0 * D;
 #pragma unroll
-    for (int n = 0; n < NH; ++n) {
+    for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+    if (!coop) {
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int head = 8 * n + 2 * j + c;
+          if (head >= nheads) continue;
+          const float inv = 1.f / l[n][c];
+#pragma unroll
+          for (int b = 0; b < kVB; ++b) {
+            const float x[8] = {o[n][4 * b][c],     o[n][4 * b][2 + c],     o[n][4 * b + 1][c], o[n][4 * b + 1][2 + c],
+                                o[n][4 * b + 2][c], o[n][4 * b + 2][2 + c], o[n][4 * b + 3][c], o[n][4 * b + 3][2 + c]};
+            if (whole) {
+              uint4 r;
+              r.x = pack2<T>(x[0] * inv, x[1] * inv);
+              r.y = pack2<T>(x[2] * inv, x[3] * inv);
+              r.z = pack2<T>(x[4] * inv, x[5] * inv);
+              r.w = pack2<T>(x[6] * inv, x[7] * inv);
+              *reinterpret_cast<uint4*>(out + head * D + 64 * b + 8 * g) = r;
+            } else {
+              float4* dst = reinterpret_cast<float4*>(slot + 2 * kHeads + head * D + 64 * b + 8 * g);
+              dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+              dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+            }
+          }
+          if (!whole && g == 0) {
+            slot[head] = m[n][c];
+            slot[kHeads + head] = l[n][c];
+          }
+        }
+    } else
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {  // the warps' parts, joined in shared memory, 8 heads at a time
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
         const int head = 2 * j + c;
         if (g == 0) {
           sh_m[warp][head] = m[n][c];
@@ -502,7 +553,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
           uint2 r;
           r.x = pack2<T>(acc.x / ll, acc.y / ll);
           r.y = pack2<T>(acc.z / ll, acc.w / ll);
-          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (size_t)row * a.out_stride + (size_t)(h0 + head) * D + d) = r;
+          *reinterpret_cast<uint2*>(out + head * D + d) = r;
         } else {
           *reinterpret_cast<float4*>(slot + 2 * kHeads + head * D + d) = acc;
           if (d == 0) {
@@ -513,13 +564,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       }
       __syncthreads();  // the parts' memory is free again
     }
-    if (!whole && t0 == 0 && threadIdx.x == 0) {
-      const long long last = cur.base + (long long)(item + 1) * nt - 1;  // the item's last unit
+    if (!whole && t0 == 0 && (coop ? threadIdx.x == 0 : lane == 0)) {
+      // the worker of the item's last unit, which lies nt - t1 units past this span
+      const long long last = u + nt - 1;
       desc[worker].row = row;
       desc[worker].item = item;
-      desc[worker].parts = (int)(((last + 1) * used - 1) / total) - worker + 1;
+      const long long whole_ones = more * (each + 1);
+      const int w = last < whole_ones ? (int)divide(last, each + 1) : more + (int)divide(last - whole_ones, each);
+      desc[worker].parts = w - worker + 1;
     }
     u += t1 - t0;
+    if (u >= u1) break;
+    next_span(cur, u);
   }
   copies_wait<0>();
 }
@@ -530,19 +586,19 @@ __global__ void __launch_bounds__(8 * NH * D / 4) k_paged_join(const PagedAttent
   using C = AttnCfg<D, NH>;
   grid_dependency_wait();
   const AttnDesc* desc = static_cast<const AttnDesc*>(a.workspace);
-  const float* slots = reinterpret_cast<const float*>(desc + kAttnMaxWorkers);
-  const AttnDesc it = desc[blockIdx.x];
+  const float* slots = reinterpret_cast<const float*>(desc + kAttnMaxCtas * kAttnWarps);
   const int head = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
+  const float* mine = slots + (size_t)(2 * blockIdx.x + 1) * C::kSlot;
+  // in one round trip: the description and the two parts that there are if there are any
+  const float* next = slots + (size_t)2 * min(blockIdx.x + 1, gridDim.x - 1) * C::kSlot;
+  const AttnDesc it = desc[blockIdx.x];
+  float mm = mine[head], ll = mine[C::kHeads + head], pm = next[head], pl = next[C::kHeads + head];
+  float4 acc = *reinterpret_cast<const float4*>(mine + 2 * C::kHeads + head * D + d);
+  float4 x = *reinterpret_cast<const float4*>(next + 2 * C::kHeads + head * D + d);
   const int nheads = min(C::kHeads, group - (it.item % blocks) * C::kHeads);
   if (it.parts == 0 || head >= nheads) return;
-  const float* mine = slots + (size_t)(2 * blockIdx.x + 1) * C::kSlot;
-  float mm = mine[head], ll = mine[C::kHeads + head];
-  float4 acc = *reinterpret_cast<const float4*>(mine + 2 * C::kHeads + head * D + d);
 #pragma unroll 4
   for (int i = 1; i < it.parts; ++i) {
-    const float* part = slots + (size_t)(2 * (blockIdx.x + i)) * C::kSlot;
-    const float pm = part[head], pl = part[C::kHeads + head];
-    const float4 x = *reinterpret_cast<const float4*>(part + 2 * C::kHeads + head * D + d);
     const float mx = fmaxf(mm, pm), low = mx == -INFINITY ? 0.f : mx;
     const float f = exp2_fast(mm - low), pf = exp2_fast(pm - low);
     mm = mx;
@@ -551,6 +607,10 @@ __global__ void __launch_bounds__(8 * NH * D / 4) k_paged_join(const PagedAttent
     acc.y = acc.y * f + x.y * pf;
     acc.z = acc.z * f + x.z * pf;
     acc.w = acc.w * f + x.w * pf;
+    const float* part = slots + (size_t)2 * min((int)blockIdx.x + i + 1, (int)gridDim.x - 1) * C::kSlot;
+    pm = part[head];
+    pl = part[C::kHeads + head];
+    x = *reinterpret_cast<const float4*>(part + 2 * C::kHeads + head * D + d);
   }
   uint2 r;
   r.x = pack2<T>(acc.x / ll, acc.y / ll);
@@ -607,7 +667,9 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   const int rc = current_sm_count(&sms);
   if (rc != W4A16_OK) return rc;
   const int group = a.heads / pool.kv_heads, blocks = (group + C::kHeads - 1) / C::kHeads;
-  const int workers = sms * C::kPerSm < kAttnMaxWorkers ? sms * C::kPerSm : kAttnMaxWorkers;
+  const int ctas = sms * C::kPerSm < kAttnMaxCtas ? sms * C::kPerSm : kAttnMaxCtas;
+  const bool coop = (long long)a.rows * pool.kv_heads * blocks < ctas * kAttnWarps;
+  const int workers = coop ? ctas : ctas * kAttnWarps;
   static std::atomic<uint64_t> configured{0};  // one bit per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -616,7 +678,7 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
     if (e == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev, std::memory_order_acq_rel);
   }
   if (e != cudaSuccess) return launched("configuring k_paged_attention,", e);
-  k_paged_attention<T, D, NH><<<workers, kAttnWarps * 32, C::kSmem, stream>>>(a, pool, tab, group, blocks);
+  k_paged_attention<T, D, NH><<<ctas, kAttnWarps * 32, C::kSmem, stream>>>(a, pool, tab, group, blocks, coop);
   const int rc2 = launched("k_paged_attention", cudaGetLastError());
   if (rc2 != W4A16_OK) return rc2;
   return launched("k_paged_join", launch_maybe_pdl(k_paged_join<T, D, NH>, dim3(workers), dim3(C::kHeads * D / 4), 0, stream, true, a,
@@ -627,7 +689,7 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
   const size_t h = attn_wide(heads / kv_heads, head_dim) ? 16 : 8;
-  return (size_t)kAttnMaxWorkers * (sizeof(AttnDesc) + 2 * h * (head_dim + 2) * 4);
+  return (size_t)kAttnMaxCtas * kAttnWarps * (sizeof(AttnDesc) + 2 * h * (head_dim + 2) * 4);
 }
 
 int launch_paged_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream) {
