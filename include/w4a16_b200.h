@@ -414,8 +414,7 @@ int w4a16_paged_append(const void* q, long long q_stride, const void* k, long lo
  * elements (multiples of 8) between rows, 16-byte aligned; heads a multiple of kv_heads.
  * Several rows may name one sequence (a prompt's tokens with growing lengths).  A length <= 0
  * gives zeros; a length past the tables, a sequence outside them or a page outside the pool
- * gives NaN.  Scores, softmax and sums in fp32; the probabilities are rounded to the pool's
- * dtype for the product with V.  workspace: w4a16_paged_attention_workspace_bytes bytes of
+ * gives NaN.  scale is positive.  Scores, softmax and sums in fp32, rounded once.  workspace: w4a16_paged_attention_workspace_bytes bytes of
  * scratch, 16-byte aligned, whose content does not matter before or after the call; calls that
  * may overlap on the GPU need their own.  The length of each row is read on the device and the
  * rows' positions are shared out evenly over the GPU, so neither the tables' width nor unequal

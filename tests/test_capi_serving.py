@@ -26,8 +26,8 @@ def tables(**kw):
     return ctypes.byref(_lib.PageTables(**(dict(ids=P, sequences=4, width=3, stride=3) | kw)))
 
 
-def attention(lib, q=P, qs=256, lens=P, seqs=None, rows=4, heads=4, t=None, p=None, out=P, os=256, ws=P, wsb=1 << 30):
-    return lib.w4a16_paged_attention(q, qs, lens, seqs, rows, heads, t or tables(), p or pool(), 0.125, out, os, ws, wsb, None)
+def attention(lib, q=P, qs=256, lens=P, seqs=None, rows=4, heads=4, t=None, p=None, out=P, os=256, ws=P, wsb=1 << 30, scale=0.125):
+    return lib.w4a16_paged_attention(q, qs, lens, seqs, rows, heads, t or tables(), p or pool(), scale, out, os, ws, wsb, None)
 
 
 def append(lib, q=P, qs=256, k=P, ks=128, v=P, vs=128, pos=P, tokens=4, heads=4, t=None, cos=P, sin=P, rows=64, p=None, out=P, os=256):
@@ -47,7 +47,8 @@ def test_attention(lib):
         assert attention(lib, t=tables(**change)) == status, change
     for kw, status in ((dict(q=None), -1), (dict(lens=None), -1), (dict(out=None), -1), (dict(rows=-1), -2), (dict(heads=3), -2),
                        (dict(heads=0), -2), (dict(q=P + 8), -3), (dict(out=P + 2), -3), (dict(qs=252), -3), (dict(os=128), -3),
-                       (dict(lens=P + 1), -3), (dict(seqs=P + 2), -3)):
+                       (dict(lens=P + 1), -3), (dict(seqs=P + 2), -3), (dict(scale=0.0), -2), (dict(scale=-1.0), -2),
+                       (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2)):
         assert attention(lib, **kw) == status, kw
     need = lib.w4a16_paged_attention_workspace_bytes(4, 2, 64)
     assert need > 0

@@ -816,6 +816,10 @@ int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* leng
               pl.kv_heads, tb.width);
     return W4A16_ERR_SHAPE;
   }
+  if (!(scale > 0.f) || scale > 3e38f) {
+    set_error("scale %g is not a positive number", scale);
+    return W4A16_ERR_SHAPE;
+  }
   if (rows == 0) return W4A16_OK;
   if (!q || !lengths || !out) {
     set_error("null pointer argument");

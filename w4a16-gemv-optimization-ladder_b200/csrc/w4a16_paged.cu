@@ -8,6 +8,10 @@
 // tables[s][p / page_size], row p % page_size.  Pages are looked up with bounds checks: an
 // entry outside the pool (or a position past the row's entries) is never dereferenced and
 // gives NaN.
+//
+// Every kernel here is launched with programmatic stream serialisation: its CTAs may be placed
+// while the kernel before it in the stream ends, and wait for that one before they read or
+// write anything.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -36,6 +40,8 @@ __device__ __forceinline__ int page_of(const PagedTables& t, int s, int p, int p
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_paged_append(const PagedAppend a, const PagedPool pool, const PagedTables tab) {
   constexpr int kChunks = D / 16;
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int per_token = (a.heads + 2 * pool.kv_heads) * kChunks;
   const long long total = (long long)a.tokens * per_token;
   for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
@@ -125,15 +131,22 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppend a, const
 // that lies within one worker is finished there; the parts of one that was cut go to the
 // workspace (slot 2w + 1 if the part begins the item, else 2w) and are joined by k_paged_join.
 constexpr int kAttnWarps = 4;
-constexpr int kAttnMaxCtas = 296;  // bounds the workspace: 148 SMs with 2 CTAs
+constexpr int kAttnMaxSms = 148;  // bounds the workspace
+// Workers for each item at most: more cost more to join than they save (one sequence of 30000
+// positions with one kv head: MAXPARTS).
+constexpr int kMaxParts = 64;
+// CTAs of an SM.  head_dim 64 has more to compute for a byte and wants more warps, with two
+// stages each (64 rows of up to 2048 positions: 31 us with 3 CTAs of 2 stages, 35 with 2 of 3).
+constexpr int attn_per_sm(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
 
 template <int D, int NH>
 struct AttnCfg {
   static constexpr int kTiles = D == 64 ? 2 : 1;  // 16-position tiles of a stage
   static constexpr int kPos = 16 * kTiles;        // positions of a stage
   static constexpr int kHeads = 8 * NH;
-  static constexpr int kStages = 3;
-  static constexpr int kPerSm = D == 256 ? 1 : 2;
+  static constexpr int kStages = D == 64 ? 2 : 3;
+  static constexpr int kPerSm = NH == 2 && D == 64 ? 2 : attn_per_sm(D);  // 16 heads take more registers
+  static constexpr int kMaxWorkers = kAttnMaxSms * attn_per_sm(D) * kAttnWarps;
   static constexpr int kSlot = kHeads * (D + 2);  // floats of a part: m, l, o per head
   static constexpr int kHalf = kPos * D * 2;      // bytes of a stage's keys, and of its values
   static constexpr int kRing = kStages * 2 * kHalf;  // bytes of a warp's ring
@@ -207,9 +220,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   const uint32_t ring = smem_addr(sh_raw) + warp * C::kRing;
   float* sh_o = reinterpret_cast<float*>(sh_raw + kAttnWarps * C::kRing);  // [warp][8][D]
 
-  grid_launch_dependents();  // the join waits for this kernel's end before it reads anything
+  grid_dependency_wait();    // launched early; nothing is read before this
+  grid_launch_dependents();  // the join waits for this kernel's end in turn
   AttnDesc* desc = static_cast<AttnDesc*>(a.workspace);
-  float* slots = reinterpret_cast<float*>(desc + kAttnMaxCtas * kAttnWarps);
+  float* slots = reinterpret_cast<float*>(desc + C::kMaxWorkers);
   const long long cap = (long long)tab.width << pool.page_shift;
   // a length past the tables keeps one position there, which has no page: NaN
   auto length = [&](int row) {
@@ -239,7 +253,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   }
   // every worker in use has a unit, so the parts of an item lie with consecutive workers: the
   // first `more` of them take each + 1 units, the others each
-  const int used = total < workers ? (int)total : workers;
+  const long long most = min((long long)workers, (long long)a.rows * items * kMaxParts);
+  const int used = (int)min(total, most);
   const long long each = used ? divide(total, used) : 0;
   const int more = (int)(total - each * used);
   auto first_unit = [&](int w) { return w < used ? w * each + min(w, more) : total; };
@@ -295,7 +310,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   // unit ahead of the copies.
   Span ahead = cur;
   long long ahead_u = u0;
-  int ahead_t = ahead.t0, pos = 0, page = -1;  // pos, page, head_off: of the unit to be copied next
+  int ahead_t = ahead.t0, pos = 0, page = -1, ahead_len = 0;  // pos, page, ahead_len, head_off: of the unit to be copied next
   size_t head_off = 0;
   const int* ids = tab.ids;
   bool seq_ok = false;
@@ -315,6 +330,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       enter();
     }
     pos = ahead_t * unit + shift;
+    ahead_len = ahead.len;
     const int at = pos + (lane & (kPos - 1));
     if (at < ahead.len) {
       if (seq_ok && (at >> pool.page_shift) < tab.width) page = __ldg(ids + (at >> pool.page_shift));
@@ -326,18 +342,39 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   const int tmask = (1 << pool.page_shift) - 1;
   constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows of one copy instruction
   const int crow = lane / kChunks, chunk = lane % kChunks;
+  const size_t row_step = (size_t)kRows * pool.token_stride;
+  const T* k_chunk = static_cast<const T*>(pool.k) + (size_t)crow * pool.token_stride + 8 * chunk;
+  const T* v_chunk = static_cast<const T*>(pool.v) + (size_t)crow * pool.token_stride + 8 * chunk;
   unsigned bad = 0;  // bit: the stage holds a position without a page
   auto load = [&](int stage) {
     const uint32_t dst = ring + stage * 2 * C::kHalf;
     bad = (bad & ~(1u << stage)) | (page == -2 ? 1u << stage : 0u);
-#pragma unroll
-    for (int i = 0; i < kPos / kRows; ++i) {
-      const int r = i * kRows + crow;
-      const int pg = __shfl_sync(0xffffffffu, page, r);
-      const size_t at = (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)((pos + r) & tmask) * pool.token_stride + head_off + 8 * chunk;
+    auto copy = [&](int r, size_t at, bool any) {
       const uint32_t to = dst + r * (D * 2) + ((chunk & ~7) | ((chunk & 7) ^ swizzle(r))) * 16;
-      copy_async16(to, static_cast<const T*>(pool.k) + at, pg >= 0);
-      copy_async16(to + C::kHalf, static_cast<const T*>(pool.v) + at, pg >= 0);
+      copy_async16(to, k_chunk + at, any);
+      copy_async16(to + C::kHalf, v_chunk + at, any);
+    };
+    if (pool.page_shift >= 4) {  // the 16 positions of a tile lie in one page
+#pragma unroll
+      for (int t = 0; t < kU; ++t) {
+        const int pg = __shfl_sync(0xffffffffu, page, 16 * t);
+        size_t at = (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)((pos + 16 * t) & tmask) * pool.token_stride + head_off;
+#pragma unroll
+        for (int i = 0; i < 16 / kRows; ++i) {
+          // positions past the length have no page of their own here, so ask for the position's
+          const int r = 16 * t + i * kRows + crow;
+          copy(r, at, pg >= 0 && pos + r < ahead_len);
+          at += row_step;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPos / kRows; ++i) {
+        const int r = i * kRows + crow;
+        const int pg = __shfl_sync(0xffffffffu, page, r);
+        copy(r, (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)((pos + r) & tmask) * pool.token_stride - (size_t)crow * pool.token_stride +
+                    head_off, pg >= 0);
+      }
     }
     copies_commit();
   };
@@ -402,37 +439,41 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       uint32_t ph[NH][kU][2], pl[NH][kU][2];  // P^T: 16-bit values and remainders
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
-        float mx[2] = {-INFINITY, -INFINITY};
+        if (p + kPos > len) {
+#pragma unroll
+          for (int t = 0; t < kU; ++t)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)  // c: head 2j + (c & 1), position g + 8 (c >> 1)
+              if (p + 16 * t + g + 8 * (c >> 1) >= len) s[n][t][c] = -INFINITY;
+        }
+        float mx[2] = {m[n][0], m[n][1]};
 #pragma unroll
         for (int t = 0; t < kU; ++t)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {  // c: head 2j + (c & 1), position g + 8 (c >> 1)
-            s[n][t][c] = p + 16 * t + g + 8 * (c >> 1) < len ? s[n][t][c] * scale : -INFINITY;
-            mx[c & 1] = fmaxf(mx[c & 1], s[n][t][c]);
-          }
-        float corr[2], low[2];
+          for (int c = 0; c < 4; ++c) mx[c & 1] = fmaxf(mx[c & 1], s[n][t][c]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], x));
-          mx[c] = fmaxf(mx[c], m[n][c]);
-          low[c] = mx[c] == -INFINITY ? 0.f : mx[c];
-          corr[c] = exp2_fast(m[n][c] - low[c]);
-          m[n][c] = mx[c];
-          l[n][c] *= corr[c];
-        }
+        if (__any_sync(0xffffffffu, mx[0] > m[n][0] || mx[1] > m[n][1])) {  // rarely, once the maxima have settled
 #pragma unroll
-        for (int i = 0; i < kVB * 4; ++i) {
-          o[n][i][0] *= corr[0];
-          o[n][i][1] *= corr[1];
-          o[n][i][2] *= corr[0];
-          o[n][i][3] *= corr[1];
+          for (int c = 0; c < 2; ++c) {
+            const float corr = m[n][c] == mx[c] ? 1.f : exp2_fast((m[n][c] - mx[c]) * scale);
+            m[n][c] = mx[c];
+            l[n][c] *= corr;
+#pragma unroll
+            for (int i = 0; i < kVB * 4; ++i) {
+              o[n][i][c] *= corr;
+              o[n][i][2 + c] *= corr;
+            }
+          }
         }
+        const float low[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0] * scale, m[n][1] == -INFINITY ? 0.f : m[n][1] * scale};
 #pragma unroll
         for (int t = 0; t < kU; ++t) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            s[n][t][c] = exp2_fast(s[n][t][c] - low[c & 1]);
+            s[n][t][c] = exp2_fast(fmaf(s[n][t][c], scale, -low[c & 1]));
             l[n][c & 1] += s[n][t][c];
           }
 #pragma unroll
@@ -484,6 +525,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {  // from here on maxima of the scaled scores, as powers of two
+      m[n][0] *= scale;
+      m[n][1] *= scale;
+    }
     if (!coop) {
 #pragma unroll
       for (int n = 0; n < NH; ++n)
@@ -580,42 +626,136 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   copies_wait<0>();
 }
 
-// Joins the parts of the item that worker blockIdx.x began, in the workers' order.
-template <typename T, int D, int NH>
-__global__ void __launch_bounds__(8 * NH * D / 4) k_paged_join(const PagedAttention a, const int group, const int blocks) {
+// Joins the parts of the item that worker blockIdx.x began.  A thread adds up four dimensions of
+// one head.  Few parts: kJoinFew in a round trip to memory, after the description's.  Many
+// (compiled in where workers are CTAs: up to kMaxParts parts of a long sequence): groups of threads take every G-th part, in a fixed order, and the maxima and
+// weights come first, so that the long sums are plain multiply-adds of independent loads (one
+// sequence of 8000 positions, 8 kv heads of 64: 12.7 us with the attention, 20 with one group).
+constexpr int kJoinChunk = 128, kJoinFew = 4;
+template <int D, int NH>
+constexpr int join_lanes() { return 8 * NH * D / 4; }
+
+template <typename T, int D, int NH, bool kMany>
+__global__ void __launch_bounds__(kMany ? 1024 : join_lanes<D, NH>()) k_paged_join(const PagedAttention a, const int group, const int blocks) {
   using C = AttnCfg<D, NH>;
+  constexpr int kLanes = join_lanes<D, NH>(), kHeads = C::kHeads;
   grid_dependency_wait();
+  grid_launch_dependents();
   const AttnDesc* desc = static_cast<const AttnDesc*>(a.workspace);
-  const float* slots = reinterpret_cast<const float*>(desc + kAttnMaxCtas * kAttnWarps);
-  const int head = threadIdx.x / (D / 4), d = (threadIdx.x % (D / 4)) * 4;
-  const float* mine = slots + (size_t)(2 * blockIdx.x + 1) * C::kSlot;
-  // in one round trip: the description and the two parts that there are if there are any
-  const float* next = slots + (size_t)2 * min(blockIdx.x + 1, gridDim.x - 1) * C::kSlot;
+  const float* slots = reinterpret_cast<const float*>(desc + C::kMaxWorkers);
   const AttnDesc it = desc[blockIdx.x];
-  float mm = mine[head], ll = mine[C::kHeads + head], pm = next[head], pl = next[C::kHeads + head];
-  float4 acc = *reinterpret_cast<const float4*>(mine + 2 * C::kHeads + head * D + d);
-  float4 x = *reinterpret_cast<const float4*>(next + 2 * C::kHeads + head * D + d);
-  const int nheads = min(C::kHeads, group - (it.item % blocks) * C::kHeads);
-  if (it.parts == 0 || head >= nheads) return;
-#pragma unroll 4
-  for (int i = 1; i < it.parts; ++i) {
-    const float mx = fmaxf(mm, pm), low = mx == -INFINITY ? 0.f : mx;
-    const float f = exp2_fast(mm - low), pf = exp2_fast(pm - low);
-    mm = mx;
-    ll = ll * f + pl * pf;
-    acc.x = acc.x * f + x.x * pf;
-    acc.y = acc.y * f + x.y * pf;
-    acc.z = acc.z * f + x.z * pf;
-    acc.w = acc.w * f + x.w * pf;
-    const float* part = slots + (size_t)2 * min((int)blockIdx.x + i + 1, (int)gridDim.x - 1) * C::kSlot;
-    pm = part[head];
-    pl = part[C::kHeads + head];
-    x = *reinterpret_cast<const float4*>(part + 2 * C::kHeads + head * D + d);
+  if (it.parts == 0) return;
+  const int head = threadIdx.x % kLanes / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  auto part = [&](int i) { return slots + (size_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::kSlot; };
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  if (!kMany || it.parts <= 2 * kJoinFew) {
+    if (threadIdx.x >= kLanes) return;
+    float top = -INFINITY;
+    for (int i0 = 0; i0 < it.parts; i0 += kJoinFew) {
+      float m[kJoinFew], l[kJoinFew];
+      float4 x[kJoinFew];
+      const float old = top;
+#pragma unroll
+      for (int i = 0; i < kJoinFew; ++i) {
+        m[i] = -INFINITY;
+        if (i0 + i < it.parts) {
+          const float* p = part(i0 + i);
+          m[i] = p[head];
+          l[i] = p[kHeads + head];
+          x[i] = *reinterpret_cast<const float4*>(p + 2 * kHeads + head * D + d);
+        }
+        top = fmaxf(top, m[i]);
+      }
+      const float low = top == -INFINITY ? 0.f : top, corr = exp2_fast(old - low);
+      sum *= corr;
+      acc.x *= corr;
+      acc.y *= corr;
+      acc.z *= corr;
+      acc.w *= corr;
+#pragma unroll
+      for (int i = 0; i < kJoinFew; ++i)
+        if (i0 + i < it.parts) {
+          const float f = exp2_fast(m[i] - low);
+          sum = fmaf(l[i], f, sum);
+          acc.x = fmaf(x[i].x, f, acc.x);
+          acc.y = fmaf(x[i].y, f, acc.y);
+          acc.z = fmaf(x[i].z, f, acc.z);
+          acc.w = fmaf(x[i].w, f, acc.w);
+        }
+    }
+  } else if constexpr (kMany) {
+    __shared__ float sh_w[kJoinChunk][kHeads], sh_l[kJoinChunk][kHeads], sh_max[kHeads], sh_sum[kHeads], sh_corr[kHeads];
+    __shared__ float4 sh_acc[1024];
+    const int grp = threadIdx.x / kLanes, groups = blockDim.x / kLanes;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (threadIdx.x < kHeads) {
+      sh_max[threadIdx.x] = -INFINITY;
+      sh_sum[threadIdx.x] = 0.f;
+    }
+    for (int c0 = 0; c0 < it.parts; c0 += kJoinChunk) {
+      const int n = min(kJoinChunk, it.parts - c0);
+      for (int e = threadIdx.x; e < n * kHeads; e += blockDim.x) {
+        const float* p = part(c0 + e / kHeads);
+        sh_w[e / kHeads][e % kHeads] = p[e % kHeads];
+        sh_l[e / kHeads][e % kHeads] = p[kHeads + e % kHeads];
+      }
+      __syncthreads();
+      for (int h = warp; h < kHeads; h += warps) {
+        float top = sh_max[h];
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, sh_w[i][h]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float low = top == -INFINITY ? 0.f : top;
+        float t = 0.f;
+        for (int i = lane; i < n; i += 32) {
+          const float f = exp2_fast(sh_w[i][h] - low);
+          sh_w[i][h] = f;
+          t = fmaf(sh_l[i][h], f, t);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (lane == 0) {
+          const float corr = exp2_fast(sh_max[h] - low);
+          sh_corr[h] = corr;
+          sh_sum[h] = sh_sum[h] * corr + t;
+          sh_max[h] = top;
+        }
+      }
+      __syncthreads();
+      const float corr = sh_corr[head];
+      acc.x *= corr;
+      acc.y *= corr;
+      acc.z *= corr;
+      acc.w *= corr;
+#pragma unroll 8
+      for (int i = grp; i < n; i += groups) {
+        const float4 x = *reinterpret_cast<const float4*>(part(c0 + i) + 2 * kHeads + head * D + d);
+        const float f = sh_w[i][head];
+        acc.x = fmaf(x.x, f, acc.x);
+        acc.y = fmaf(x.y, f, acc.y);
+        acc.z = fmaf(x.z, f, acc.z);
+        acc.w = fmaf(x.w, f, acc.w);
+      }
+      __syncthreads();  // the weights' memory is free again
+    }
+    sh_acc[threadIdx.x] = acc;
+    __syncthreads();
+    if (grp > 0) return;
+    for (int i = 1; i < groups; ++i) {
+      const float4 x = sh_acc[threadIdx.x + i * kLanes];
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
+    }
+    sum = sh_sum[head];
   }
+  if (head >= group - it.item % blocks * kHeads) return;  // a head block's empty places
   uint2 r;
-  r.x = pack2<T>(acc.x / ll, acc.y / ll);
-  r.y = pack2<T>(acc.z / ll, acc.w / ll);
-  const int h = it.item / blocks * group + it.item % blocks * C::kHeads + head;
+  r.x = pack2<T>(acc.x / sum, acc.y / sum);
+  r.y = pack2<T>(acc.z / sum, acc.w / sum);
+  const int h = it.item / blocks * group + it.item % blocks * kHeads + head;
   *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (size_t)it.row * a.out_stride + (size_t)h * D + d) = r;
 }
 
@@ -649,8 +789,8 @@ int launch_paged_append(const PagedAppend& a, const PagedPool& pool, const Paged
     constexpr int D = decltype(d)::value;
     const long long total = (long long)a.tokens * (a.heads + 2 * pool.kv_heads) * (D / 16);
     const long long blocks = (total + 255) / 256, most = (long long)sms * 8;
-    k_paged_append<T, D><<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(a, pool, tab);
-    return launched("k_paged_append", cudaGetLastError());
+    return launched("k_paged_append", launch_maybe_pdl(k_paged_append<T, D>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0,
+                                                       stream, true, a, pool, tab));
   });
 }
 
@@ -667,7 +807,7 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   const int rc = current_sm_count(&sms);
   if (rc != W4A16_OK) return rc;
   const int group = a.heads / pool.kv_heads, blocks = (group + C::kHeads - 1) / C::kHeads;
-  const int ctas = sms * C::kPerSm < kAttnMaxCtas ? sms * C::kPerSm : kAttnMaxCtas;
+  const int ctas = (sms < kAttnMaxSms ? sms : kAttnMaxSms) * C::kPerSm;
   const bool coop = (long long)a.rows * pool.kv_heads * blocks < ctas * kAttnWarps;
   const int workers = coop ? ctas : ctas * kAttnWarps;
   static std::atomic<uint64_t> configured{0};  // one bit per device
@@ -678,18 +818,20 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
     if (e == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev, std::memory_order_acq_rel);
   }
   if (e != cudaSuccess) return launched("configuring k_paged_attention,", e);
-  k_paged_attention<T, D, NH><<<ctas, kAttnWarps * 32, C::kSmem, stream>>>(a, pool, tab, group, blocks, coop);
-  const int rc2 = launched("k_paged_attention", cudaGetLastError());
+  const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
+                                                                 stream, true, a, pool, tab, group, blocks, coop));
   if (rc2 != W4A16_OK) return rc2;
-  return launched("k_paged_join", launch_maybe_pdl(k_paged_join<T, D, NH>, dim3(workers), dim3(C::kHeads * D / 4), 0, stream, true, a,
-                                                   group, blocks));
+  constexpr int lanes = join_lanes<D, NH>();
+  return launched("k_paged_join",
+                  launch_maybe_pdl(coop ? k_paged_join<T, D, NH, true> : k_paged_join<T, D, NH, false>, dim3(workers),
+                                   dim3(!coop ? lanes : 4 * lanes < 1024 ? 4 * lanes : 1024), 0, stream, true, a, group, blocks));
 }
 
 }  // namespace
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
   const size_t h = attn_wide(heads / kv_heads, head_dim) ? 16 : 8;
-  return (size_t)kAttnMaxCtas * kAttnWarps * (sizeof(AttnDesc) + 2 * h * (head_dim + 2) * 4);
+  return (size_t)kAttnMaxSms * attn_per_sm(head_dim) * kAttnWarps * (sizeof(AttnDesc) + 2 * h * (head_dim + 2) * 4);
 }
 
 int launch_paged_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream) {
