@@ -935,7 +935,7 @@ int w4a16_process_logits(const w4a16_logits_desc* d, w4a16_stream_t stream) {
     set_error("tokens of %d bytes (4 or 8)", d->token_bytes);
     return W4A16_ERR_DTYPE;
   }
-  if (d->rows < 0 || d->vocab < 0 || d->history < 0 || d->pairs < 0 || d->stride < 0 || d->bias_stride < 0 ||
+  if (d->rows < 0 || d->vocab < 0 || d->vocab > (1 << 30) || d->history < 0 || d->history > (1 << 30) || d->pairs < 0 || d->stride < 0 || d->bias_stride < 0 ||
       d->mask_stride < 0 || d->token_stride < 0 || (d->rows > 1 && d->out_stride < d->vocab)) {
     set_error("bad shape: rows %d vocab %d history %d pairs %d or a negative or overlapping stride", d->rows, d->vocab,
               d->history, d->pairs);
