@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedAppend a, const
 constexpr int kAttnWarps = 4;
 constexpr int kAttnMaxSms = 148;  // bounds the workspace
 // Workers for each item at most: more cost more to join than they save (one sequence of 30000
-// positions with one kv head: MAXPARTS).
+// positions with one kv head: 16.5 us with 64, 20.9 with 32, 17.9 with 128, 28.6 without a bound).
 constexpr int kMaxParts = 64;
 // CTAs of an SM.  head_dim 64 has more to compute for a byte and wants more warps, with two
 // stages each (64 rows of up to 2048 positions: 31 us with 3 CTAs of 2 stages, 35 with 2 of 3).

@@ -27,51 +27,72 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernels import _need, _ptr, _stream
 
 _POOL_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+_byref = ctypes.byref
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(device).cuda_stream, without the object
 
 
-def _is_cuda(t):
-    return isinstance(t, torch.Tensor) and t.is_cuda
+def _refuse(msg):
+    raise RuntimeError(msg)
+
+
+def _call(name, dev, *args):
+    """Run a C entry on dev's current stream, its last argument.  The checks before it build their
+    messages only when they fail: a decode step is short of host time."""
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == dev.index:
+        status = fn(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _raw_stream(dev.index))
+    if status:
+        _lib.check(status, name)
 
 
 def _pool(k_pages, v_pages):
     """The C description of one layer's pool, checked."""
-    _need(_is_cuda(k_pages) and k_pages.dim() == 4 and k_pages.dtype in _POOL_DTYPES,
-          "k_pages must be an fp16 or bf16 CUDA tensor [pages, kv_heads, page_size, head_dim]")
-    _need(isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype == k_pages.dtype
-          and v_pages.shape == k_pages.shape and v_pages.stride() == k_pages.stride(),
-          "v_pages must have the device, dtype, shape and strides of k_pages")
+    if not (isinstance(k_pages, torch.Tensor) and k_pages.is_cuda and k_pages.dim() == 4 and k_pages.dtype in _POOL_DTYPES):
+        _refuse("k_pages must be an fp16 or bf16 CUDA tensor [pages, kv_heads, page_size, head_dim]")
+    stride = k_pages.stride()
+    if not (isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype == k_pages.dtype
+            and v_pages.shape == k_pages.shape and v_pages.stride() == stride):
+        _refuse("v_pages must have the device, dtype, shape and strides of k_pages")
     pages, kv_heads, page_size, head_dim = k_pages.shape
-    sp, sh, st, sd = k_pages.stride()
-    _need(sd == 1, "the last dimension of the pages must be contiguous")
+    sp, sh, st, sd = stride
+    if sd != 1:
+        _refuse("the last dimension of the pages must be contiguous")
     # a dimension of one entry may carry any stride
     return _lib.PagePool(k_pages.data_ptr(), v_pages.data_ptr(), _POOL_DTYPES[k_pages.dtype], pages, kv_heads, page_size,
                          head_dim, sp if pages > 1 else 8, sh if kv_heads > 1 else 8, st if page_size > 1 else 8)
 
 
 def _tables(tables, dev):
-    _need(isinstance(tables, torch.Tensor) and tables.device == dev and tables.dtype == torch.int32 and tables.dim() == 2
-          and (tables.stride(1) == 1 or tables.shape[1] <= 1),
-          f"tables must be an int32 [sequences, width] tensor on {dev} with contiguous rows")
-    return _lib.PageTables(tables.data_ptr(), tables.shape[0], tables.shape[1], tables.stride(0))
+    if not (isinstance(tables, torch.Tensor) and tables.device == dev and tables.dtype == torch.int32 and tables.dim() == 2):
+        _refuse(f"tables must be an int32 [sequences, width] tensor on {dev}")
+    sequences, width = tables.shape
+    stride, one = tables.stride()
+    if one != 1 and width > 1:
+        _refuse("the rows of tables must be contiguous")
+    return _lib.PageTables(tables.data_ptr(), sequences, width, stride)
 
 
 def _index(t, n, name, dev):
-    _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == torch.int32 and t.dim() == 1
-          and t.is_contiguous() and (n is None or t.shape[0] == n),
-          f"{name} must be a contiguous int32 [{'n' if n is None else n}] tensor on {dev}")
+    if not (isinstance(t, torch.Tensor) and t.device == dev and t.dtype == torch.int32 and t.dim() == 1
+            and t.is_contiguous() and (n is None or t.shape[0] == n)):
+        _refuse(f"{name} must be a contiguous int32 [{'n' if n is None else n}] tensor on {dev}")
     return t.data_ptr()
 
 
 def _tokens(t, n, heads, head_dim, dtype, name, dev):
     """(address, elements between tokens) of a [tokens, heads, head_dim] tensor whose tokens are
     contiguous blocks (rows of a wider projection output will do)."""
-    _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == dtype and t.dim() == 3
-          and t.shape == (n, heads, head_dim) and t.stride(2) == 1 and (heads == 1 or t.stride(1) == head_dim),
-          f"{name} must be a {dtype} [{n}, {heads}, {head_dim}] tensor on {dev}, contiguous within a token")
-    return t.data_ptr(), t.stride(0) if n > 1 else heads * head_dim
+    if not (isinstance(t, torch.Tensor) and t.device == dev and t.dtype == dtype and t.shape == (n, heads, head_dim)):
+        _refuse(f"{name} must be a {dtype} [{n}, {heads}, {head_dim}] tensor on {dev}")
+    sn, sh, sd = t.stride()
+    if sd != 1 or (heads > 1 and sh != head_dim):
+        _refuse(f"{name} must be contiguous within a token")
+    return t.data_ptr(), sn if n > 1 else heads * head_dim
 
 
 def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=None, seqs=None, out=None):
@@ -90,35 +111,37 @@ def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=
     page outside the pool writes nothing to the cache and gives NaN.  A (sequence, position) may
     occur once per call."""
     pool = _pool(k_pages, v_pages)
-    dev, dtype, d = k_pages.device, k_pages.dtype, k_pages.shape[3]
-    _need(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
-    n, kvh = k.shape[0], k_pages.shape[1]
+    dev, dtype = k_pages.device, k_pages.dtype
+    if not (isinstance(k, torch.Tensor) and k.dim() == 3):
+        _refuse("k must be [tokens, kv_heads, head_dim]")
+    n, kvh, d = k.shape[0], pool.kv_heads, pool.head_dim
     kp, ks = _tokens(k, n, kvh, d, dtype, "k", dev)
     vp, vs = _tokens(v, n, kvh, d, dtype, "v", dev)
     pos = _index(positions, n, "positions", dev)
     sq = _index(seqs, n, "seqs", dev) if seqs is not None else None
     tab = _tables(tables, dev)
-    _need((cos is None) == (sin is None), "cos and sin go together")
-    if cos is not None:
+    cp = sp = None
+    angles = 0
+    if cos is not None or sin is not None:
         for name, t in (("cos", cos), ("sin", sin)):
-            _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == torch.float32 and t.dim() == 2
-                  and t.shape == cos.shape and t.shape[1] == d and t.is_contiguous(),
-                  f"{name} must be a contiguous fp32 [positions, {d}] tensor on {dev}")
+            if not (isinstance(t, torch.Tensor) and t.device == dev and t.dtype == torch.float32 and t.dim() == 2
+                    and t.shape[1] == d and t.is_contiguous()):
+                _refuse(f"{name} must be a contiguous fp32 [positions, {d}] tensor on {dev} (cos and sin go together)")
+        angles = cos.shape[0]
+        if sin.shape[0] != angles:
+            _refuse("cos and sin must have the same shape")
+        cp, sp = cos.data_ptr(), sin.data_ptr()
     heads, qp, qs, op, os_ = 0, None, 0, None, 0
     if q is not None:
-        _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [tokens, heads, head_dim]")
+        if not (isinstance(q, torch.Tensor) and q.dim() == 3):
+            _refuse("q must be [tokens, heads, head_dim]")
         heads = q.shape[1]
         qp, qs = _tokens(q, n, heads, d, dtype, "q", dev)
         if out is None:
-            out = torch.empty((n, heads, d), dtype=dtype, device=dev)
+            out = q.new_empty((n, heads, d))
         op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
-    if n == 0:
-        return out
-    with torch.cuda.device(dev):
-        status = _lib.lib().w4a16_paged_append(
-            qp, qs, kp, ks, vp, vs, pos, sq, n, heads, ctypes.byref(tab), _ptr(cos), _ptr(sin),
-            cos.shape[0] if cos is not None else 0, ctypes.byref(pool), op, os_, _stream(dev))
-    _lib.check(status, "w4a16_paged_append")
+    if n:
+        _call("w4a16_paged_append", dev, qp, qs, kp, ks, vp, vs, pos, sq, n, heads, _byref(tab), cp, sp, angles, _byref(pool), op, os_)
     return out
 
 
@@ -138,59 +161,62 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     width, a sequence outside `tables` or a page outside the pool gives NaN."""
     pool = _pool(k_pages, v_pages)
     dev, dtype = k_pages.device, k_pages.dtype
-    kvh, d = k_pages.shape[1], k_pages.shape[3]
-    _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [rows, heads, head_dim]")
+    kvh, d = pool.kv_heads, pool.head_dim
+    if not (isinstance(q, torch.Tensor) and q.dim() == 3):
+        _refuse("q must be [rows, heads, head_dim]")
     n, heads = q.shape[0], q.shape[1]
     qp, qs = _tokens(q, n, heads, d, dtype, "q", dev)
-    _need(heads > 0 and heads % kvh == 0, f"{heads} query heads are not a multiple of {kvh} kv heads")
+    if heads == 0 or kvh == 0 or heads % kvh:
+        _refuse(f"{heads} query heads are not a multiple of {kvh} kv heads")
     lens = _index(lengths, n, "lengths", dev)
     sq = _index(seqs, n, "seqs", dev) if seqs is not None else None
     tab = _tables(tables, dev)
     if out is None:
-        out = torch.empty((n, heads, d), dtype=dtype, device=dev)
+        out = q.new_empty((n, heads, d))
     op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
     if n == 0:
         return out
-    L = _lib.lib()
-    with torch.cuda.device(dev):
-        if workspace is None:
-            workspace = torch.empty(L.w4a16_paged_attention_workspace_bytes(heads, kvh, d), dtype=torch.uint8, device=dev)
-        else:
-            _need(isinstance(workspace, torch.Tensor) and workspace.device == dev and workspace.dtype == torch.uint8
-                  and workspace.is_contiguous(), f"workspace must be a contiguous uint8 tensor on {dev}")
-        status = L.w4a16_paged_attention(qp, qs, lens, sq, n, heads, ctypes.byref(tab), ctypes.byref(pool),
-                                         float(d ** -0.5 if scale is None else scale), op, os_, workspace.data_ptr(),
-                                         workspace.numel(), _stream(dev))
-    _lib.check(status, "w4a16_paged_attention")
+    if workspace is None:
+        size = _lib.lib().w4a16_paged_attention_workspace_bytes(heads, kvh, d)
+        workspace = q.new_empty((size + 1) // 2)
+    else:
+        if not (isinstance(workspace, torch.Tensor) and workspace.device == dev and workspace.dtype == torch.uint8
+                and workspace.is_contiguous()):
+            _refuse(f"workspace must be a contiguous uint8 tensor on {dev}")
+        size = workspace.numel()
+    _call("w4a16_paged_attention", dev, qp, qs, lens, sq, n, heads, _byref(tab), _byref(pool), float(d ** -0.5 if scale is None else scale),
+          op, os_, workspace.data_ptr(), size)
     return out
 
 
 # ------------------------------------------------------------------------------ page bookkeeping
 
 def _state(tables, lengths, refs, page_size):
-    _need(_is_cuda(tables) and tables.dtype == torch.int32 and tables.dim() == 2 and tables.is_contiguous(),
-          "tables must be a contiguous int32 [sequences, width] CUDA tensor")
+    if not (isinstance(tables, torch.Tensor) and tables.is_cuda and tables.dtype == torch.int32 and tables.dim() == 2
+            and tables.is_contiguous()):
+        _refuse("tables must be a contiguous int32 [sequences, width] CUDA tensor")
     dev = tables.device
-    _index(lengths, tables.shape[0], "lengths", dev)
-    _index(refs, None, "refs", dev)
-    return _lib.PageState(tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), tables.shape[0], tables.shape[1],
-                          refs.shape[0], page_size, tables.shape[1])
+    sequences, width = tables.shape
+    return _lib.PageState(tables.data_ptr(), _index(lengths, sequences, "lengths", dev), _index(refs, None, "refs", dev), sequences,
+                          width, refs.shape[0], page_size, width)
 
 
 def _blocks(k_pages, v_pages):
     """The C description of the pages' bytes in all layers, checked: [layers, pages, ...] or one
     layer's [pages, kv_heads, page_size, head_dim], every page one dense block."""
-    _need(_is_cuda(k_pages) and k_pages.dim() in (4, 5), "k_pages must be a CUDA tensor [layers, pages, kv_heads, page_size, "
-          "head_dim] or [pages, kv_heads, page_size, head_dim]")
-    _need(isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype == k_pages.dtype
-          and v_pages.shape == k_pages.shape and v_pages.stride() == k_pages.stride(),
-          "v_pages must have the device, dtype, shape and strides of k_pages")
-    size, shape, stride = k_pages.element_size(), k_pages.shape, k_pages.stride()
+    if not (isinstance(k_pages, torch.Tensor) and k_pages.is_cuda and k_pages.dim() in (4, 5)):
+        _refuse("k_pages must be a CUDA tensor [layers, pages, kv_heads, page_size, head_dim] or [pages, kv_heads, page_size, head_dim]")
+    shape, stride = k_pages.shape, k_pages.stride()
+    if not (isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype == k_pages.dtype
+            and v_pages.shape == shape and v_pages.stride() == stride):
+        _refuse("v_pages must have the device, dtype, shape and strides of k_pages")
+    size = k_pages.element_size()
     layers, ls = (shape[0], stride[0]) if len(shape) == 5 else (1, 0)
     pages, ps = shape[-4], stride[-4]
     elements = 1
     for st, n in sorted(zip(stride[-3:], shape[-3:])):  # dense in some order of its dimensions
-        _need(n == 1 or st == elements, "a page must be one dense block")
+        if n != 1 and st != elements:
+            _refuse("a page must be one dense block")
         elements *= n
     return _lib.PageBlocks(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, ls * size if layers > 1 else 0,
                            (ps if pages > 1 else elements) * size, elements * size)
@@ -209,10 +235,8 @@ def extend_sequences(tables, lengths, refs, seqs, counts, *, page_size):
     s = _index(seqs, None, "seqs", dev)
     n = seqs.shape[0]
     c = _index(counts, n, "counts", dev)
-    ok = torch.empty(n, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        status = _lib.lib().w4a16_pages_extend(ctypes.byref(st), s, c, n, ok.data_ptr(), _stream(dev))
-    _lib.check(status, "w4a16_pages_extend")
+    ok = torch.empty_like(seqs)
+    _call("w4a16_pages_extend", dev, _byref(st), s, c, n, ok.data_ptr())
     return ok
 
 
@@ -226,18 +250,15 @@ def fork_sequences(k_pages, v_pages, tables, lengths, refs, src, dst):
     b = _blocks(k_pages, v_pages)
     st = _state(tables, lengths, refs, k_pages.shape[-2])
     dev = tables.device
-    _need(k_pages.device == dev and refs.shape[0] == k_pages.shape[-4], f"refs must have one entry per page and k_pages be on {dev}")
+    if k_pages.device != dev or st.pages != b.pages:
+        _refuse(f"refs must have one entry for each of the {b.pages} pages, and k_pages be on {dev}")
     s = _index(src, None, "src", dev)
     n = src.shape[0]
     t = _index(dst, n, "dst", dev)
-    ok = torch.empty(n, dtype=torch.int32, device=dev)
-    L = _lib.lib()
-    need = L.w4a16_pages_fork_scratch_bytes(n)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        status = L.w4a16_pages_fork(ctypes.byref(st), ctypes.byref(b), s, t, n, ok.data_ptr(), scratch.data_ptr(), need,
-                                    _stream(dev))
-    _lib.check(status, "w4a16_pages_fork")
+    ok = torch.empty_like(src)
+    need = _lib.lib().w4a16_pages_fork_scratch_bytes(n)
+    scratch = src.new_empty((need + 3) // 4)
+    _call("w4a16_pages_fork", dev, _byref(st), _byref(b), s, t, n, ok.data_ptr(), scratch.data_ptr(), need)
     return ok
 
 
@@ -247,11 +268,8 @@ def free_sequences(tables, lengths, refs, seqs):
     st = _state(tables, lengths, refs, 1)
     dev = tables.device
     s = _index(seqs, None, "seqs", dev)
-    n = seqs.shape[0]
-    ok = torch.empty(n, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        status = _lib.lib().w4a16_pages_free(ctypes.byref(st), s, n, ok.data_ptr(), _stream(dev))
-    _lib.check(status, "w4a16_pages_free")
+    ok = torch.empty_like(seqs)
+    _call("w4a16_pages_free", dev, _byref(st), s, seqs.shape[0], ok.data_ptr())
     return ok
 
 
@@ -262,10 +280,7 @@ def copy_pages(k_pages, v_pages, src, dst):
     dev = k_pages.device
     s = _index(src, None, "src", dev)
     n = src.shape[0]
-    t = _index(dst, n, "dst", dev)
-    with torch.cuda.device(dev):
-        status = _lib.lib().w4a16_pages_copy(ctypes.byref(b), s, t, n, _stream(dev))
-    _lib.check(status, "w4a16_pages_copy")
+    _call("w4a16_pages_copy", dev, _byref(b), s, _index(dst, n, "dst", dev), n)
 
 
 def compact_pages(k_pages, v_pages, tables, refs, *, inplace=True):
@@ -276,18 +291,15 @@ def compact_pages(k_pages, v_pages, tables, refs, *, inplace=True):
     new tensors with inplace=False), and the number of pages moved, int32 [1] on the device."""
     b = _blocks(k_pages, v_pages)
     dev = k_pages.device
-    _need(isinstance(tables, torch.Tensor) and tables.device == dev and tables.dtype == torch.int32 and tables.is_contiguous(),
-          f"tables must be a contiguous int32 tensor on {dev}")
-    r = _index(refs, k_pages.shape[-4], "refs", dev)
+    if not (isinstance(tables, torch.Tensor) and tables.device == dev and tables.dtype == torch.int32 and tables.is_contiguous()):
+        _refuse(f"tables must be a contiguous int32 tensor on {dev}")
+    r = _index(refs, b.pages, "refs", dev)
     new_tables, new_refs = (tables, refs) if inplace else (torch.empty_like(tables), torch.empty_like(refs))
-    moved = torch.empty(1, dtype=torch.int32, device=dev)
-    L = _lib.lib()
-    need = L.w4a16_pages_compact_scratch_bytes(refs.shape[0])
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        status = L.w4a16_pages_compact(ctypes.byref(b), tables.data_ptr(), new_tables.data_ptr(), tables.numel(), r,
-                                       new_refs.data_ptr(), moved.data_ptr(), scratch.data_ptr(), need, _stream(dev))
-    _lib.check(status, "w4a16_pages_compact")
+    moved = refs.new_empty(1)
+    need = _lib.lib().w4a16_pages_compact_scratch_bytes(b.pages)
+    scratch = refs.new_empty((need + 3) // 4)
+    _call("w4a16_pages_compact", dev, _byref(b), tables.data_ptr(), new_tables.data_ptr(), tables.numel(), r, new_refs.data_ptr(),
+          moved.data_ptr(), scratch.data_ptr(), need)
     return new_tables, new_refs, moved
 
 
