@@ -213,7 +213,7 @@ int check_blocks(const w4a16_page_blocks* b, w4a16::PageBlocks* out) {
     set_error("null page blocks");
     return W4A16_ERR_NULL;
   }
-  if (b->layers <= 0 || b->pages <= 0 || b->page_bytes <= 0 || b->page_stride < b->page_bytes || b->layer_stride < 0) {
+  if (b->layers <= 0 || b->pages <= 0 || b->page_bytes <= 0 || b->page_bytes > (1 << 30) || b->page_stride < b->page_bytes || b->layer_stride < 0) {
     set_error("bad page blocks: %d layers of %d pages, layer stride %lld, page stride %lld, %lld bytes a page", b->layers,
               b->pages, b->layer_stride, b->page_stride, b->page_bytes);
     return W4A16_ERR_SHAPE;

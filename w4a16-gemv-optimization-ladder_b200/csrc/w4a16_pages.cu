@@ -5,11 +5,13 @@
 //   refs    int32 [pages]             number of table entries that hold the page (0: free)
 // Whole pages may be shared by several sequences; a partly filled page belongs to one.
 //
-// extend and fork first run one CTA that serves the requests in order with the lowest free
-// pages (k_pages_plan); what is proportional to table widths or page contents is done by
-// grid-wide kernels (k_pages_apply, k_page_moves).
+// extend, fork and compact first run one CTA that decides which page goes where (k_pages_plan,
+// k_compact_plan); what is proportional to table widths or page contents is done by one
+// grid-wide kernel after it (k_pages_apply).  Every kernel is launched with programmatic stream
+// serialisation and waits for the one before it before it reads or writes anything.
 #include <cuda_runtime.h>
 
+#include "w4a16_device.cuh"
 #include "w4a16_internal.h"
 
 namespace w4a16 {
@@ -55,6 +57,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
                                                              const int* __restrict__ src, const int* __restrict__ counts,
                                                              int n, int* __restrict__ ok, int2* __restrict__ moves) {
   __shared__ int sh[33], named[kPlanThreads], cum[kPlanThreads], first[kPlanThreads];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int i = threadIdx.x;
   const int seq = i < n ? seqs[i] : -1;
   named[i] = seq;
@@ -62,7 +66,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
   const int mask = (1 << st.page_shift) - 1;
   const long long cap = (long long)st.width << st.page_shift;
   bool valid = i < n && seq >= 0 && seq < st.sequences;
-  for (int j = 0; valid && j < i; ++j) valid = named[j] != seq;
+  if (i < n) {
+#pragma unroll 8
+    for (int j = 0; j < i; ++j) valid &= named[j] != seq;
+  }
   int need = 0, length = 0, from = 0, grown = 0;
   if (valid) {
     length = st.lengths[seq];
@@ -90,36 +97,42 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
   cum[i] = before + need;
   first[i] = (int)(((long long)length + mask) >> st.page_shift);  // table column of the request's first new page
   __syncthreads();
-  // the lowest free pages, as many as are wanted: rank -> request -> table entry.  Which
-  // requests are served is known once the free pages are counted, so count, then hand out.
-  int found = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    int have = 0;
-    for (int p0 = 0; p0 < st.pages && have < wanted; p0 += kPlanThreads) {
-      const int p = p0 + i;
-      const bool free = p < st.pages && st.refs[p] == 0;
-      int got;
-      const int rank = have + block_prefix(free ? 1 : 0, sh, &got);
-      __syncthreads();
-      if (pass == 1 && free && rank < wanted) {
-        int lo = 0, hi = kPlanThreads - 1;  // the first request whose running sum exceeds rank
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (cum[mid] > rank) hi = mid; else lo = mid + 1;
-        }
-        if (cum[lo] <= found) {
-          const int k = rank - (lo ? cum[lo - 1] : 0);
-          st.refs[p] = 1;
-          if (moves) {
-            const int f = src[lo];
-            moves[lo] = make_int2(st.tables[(size_t)f * st.table_stride + first[lo]], p);
-          }
-          st.tables[(size_t)named[lo] * st.table_stride + first[lo] + k] = p;
-        }
+  // the lowest free pages, as many as are wanted, 4 for a thread at a time: rank -> request ->
+  // table entry.  Which requests are served is known once the free pages are counted, so count,
+  // then hand out (from the same registers where the first round has enough pages).
+  constexpr int kRound = 4 * kPlanThreads;
+  int found = 0, rounds = 0, rank = 0;
+  unsigned bits = 0;
+  auto look = [&](int p0, int have) {  // free pages of this thread's 4, and their first's rank
+    bits = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (p0 + 4 * i + k < st.pages && st.refs[p0 + 4 * i + k] == 0) bits |= 1u << k;
+    int got;
+    __syncthreads();
+    rank = have + block_prefix(__popc(bits), sh, &got);
+    return got;
+  };
+  for (int p0 = 0; p0 < st.pages && found < wanted; p0 += kRound, ++rounds) found += look(p0, found);
+  int have = 0;
+  for (int r = 0; r < rounds; ++r) {
+    if (rounds > 1) have += look(r * kRound, have);
+    for (int k = 0; k < 4; ++k) {
+      if (!(bits >> k & 1u)) continue;
+      if (rank >= wanted) break;
+      int lo = 0, hi = n - 1;  // the first request whose running sum exceeds rank
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cum[mid] > rank) hi = mid; else lo = mid + 1;
       }
-      have += got;
+      if (cum[lo] <= found) {
+        const int p = r * kRound + 4 * i + k, nth = rank - (lo ? cum[lo - 1] : 0);
+        st.refs[p] = 1;
+        if (moves) moves[lo] = make_int2(st.tables[(size_t)src[lo] * st.table_stride + first[lo]], p);
+        st.tables[(size_t)named[lo] * st.table_stride + first[lo] + nth] = p;
+      }
+      ++rank;
     }
-    if (pass == 0) found = have;
   }
   if (i < n) {
     const bool served = valid && (need == 0 || cum[i] <= found);
@@ -129,23 +142,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
   }
 }
 
-// Shares the whole pages of fork's sources: one CTA row per request.
-__global__ void __launch_bounds__(256) k_pages_share(const PagesState st, const int* __restrict__ src, const int* __restrict__ dst,
-                                                     const int* __restrict__ ok) {
-  const int i = blockIdx.y;
-  if (!ok[i]) return;
-  const int whole = st.lengths[dst[i]] >> st.page_shift;  // set by the plan; a source may be another request's dst
-  const int* from = st.tables + (size_t)src[i] * st.table_stride;
-  int* to = st.tables + (size_t)dst[i] * st.table_stride;
-  for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < whole; c += gridDim.x * blockDim.x) {
-    const int p = from[c];
-    to[c] = p;
-    if (p >= 0 && p < st.pages) atomicAdd(st.refs + p, 1);
-  }
-}
-
 // Frees sequences: one CTA per request; the first request that names a sequence counts.
 __global__ void __launch_bounds__(256) k_pages_free(const PagesState st, const int* __restrict__ seqs, int n, int* __restrict__ ok) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int i = blockIdx.x;
   const int seq = seqs[i];
   int again = 0;
@@ -169,6 +169,8 @@ __global__ void __launch_bounds__(256) k_pages_free(const PagesState st, const i
 __global__ void __launch_bounds__(1024) k_compact_plan(const int* refs, int pages, int* refs_out, int* __restrict__ where,
                                                        int2* __restrict__ moves, int* __restrict__ moved) {
   __shared__ int sh[33];
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int per = (pages + 1023) / 1024, p0 = min(pages, (int)threadIdx.x * per), p1 = min(pages, p0 + per);
   int live = 0;
   for (int p = p0; p < p1; ++p) live += refs[p] > 0;
@@ -204,73 +206,117 @@ __global__ void __launch_bounds__(1024) k_compact_plan(const int* refs, int page
   if (threadIdx.x == 0) *moved = count;
 }
 
-__global__ void __launch_bounds__(256) k_tables_remap(const int* tables, int* out, long long n, const int* __restrict__ where, int pages) {
-  for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (long long)gridDim.x * blockDim.x) {
-    const int p = tables[e];
-    out[e] = p >= 0 && p < pages ? where[p] : p;
-  }
-}
+// The table work that goes with a set of page moves, in the first `ctas` CTAs of k_pages_apply.
+struct TableWork {
+  int ctas = 0;
+  // fork: dst[i] shares the whole pages of src[i] if ok[i]
+  PagesState st;
+  const int* src = nullptr;
+  const int* dst = nullptr;
+  const int* ok = nullptr;
+  int n = 0;
+  // compact: out[e] = where[tables[e]]
+  const int* tables = nullptr;
+  int* out = nullptr;
+  const int* where = nullptr;
+  long long entries = 0;
+};
 
 // Copies whole pages of every layer, k and v: moves are pairs (src, dst), or two lists.  A pair
-// with an index outside [0, pages) is skipped.  Item = (pair, layer, pool); 16 bytes a thread.
-__global__ void __launch_bounds__(256) k_page_moves(const PageBlocks b, const int2* __restrict__ pairs, const int* __restrict__ src,
-                                                    const int* __restrict__ dst, int n, const int* __restrict__ count) {
+// with an index outside [0, pages) is skipped.  Bound by the bytes, read once and written once:
+// a CTA takes one pair of one pool at a time, a thread kFlight 16-byte words in flight.
+__global__ void __launch_bounds__(256) k_pages_apply(const PageBlocks b, const int2* pairs, const int* src, const int* dst, int n,
+                                                     const int* count, const TableWork t) {
+  constexpr int kFlight = 8;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < t.ctas) {
+    for (long long e = (long long)blockIdx.x * 256 + tid; e < t.entries; e += (long long)t.ctas * 256) {
+      const int p = t.tables[e];
+      t.out[e] = p >= 0 && p < b.pages ? t.where[p] : p;
+    }
+    for (int i = blockIdx.x; i < t.n; i += t.ctas) {
+      if (!t.ok[i]) continue;
+      const int whole = t.st.lengths[t.dst[i]] >> t.st.page_shift;  // set by the plan; a source may be another request's dst
+      const int* from = t.st.tables + (size_t)t.src[i] * t.st.table_stride;
+      int* to = t.st.tables + (size_t)t.dst[i] * t.st.table_stride;
+      for (int c = tid; c < whole; c += 256) {
+        const int p = from[c];
+        to[c] = p;
+        if (p >= 0 && p < t.st.pages) atomicAdd(t.st.refs + p, 1);
+      }
+    }
+    return;
+  }
   if (count) n = min(n, *count);
   const long long items = 2LL * n * b.layers;
-  for (long long e = blockIdx.x; e < items; e += gridDim.x) {
+  const int words = (int)(b.page_bytes / 16);
+  for (long long e = blockIdx.x - t.ctas; e < items; e += gridDim.x - t.ctas) {
     const int which = (int)(e & 1), layer = (int)((e >> 1) % b.layers), i = (int)((e >> 1) / b.layers);
-    const int f = pairs ? pairs[i].x : src[i], t = pairs ? pairs[i].y : dst[i];
-    if (f < 0 || f >= b.pages || t < 0 || t >= b.pages || f == t) continue;
+    const int f = pairs ? pairs[i].x : src[i], d = pairs ? pairs[i].y : dst[i];
+    if (f < 0 || f >= b.pages || d < 0 || d >= b.pages || f == d) continue;
     uint8_t* base = static_cast<uint8_t*>(which ? b.v : b.k) + (size_t)layer * b.layer_stride;
     const uint4* from = reinterpret_cast<const uint4*>(base + (size_t)f * b.page_stride);
-    uint4* to = reinterpret_cast<uint4*>(base + (size_t)t * b.page_stride);
-    const long long words = b.page_bytes / 16;
-    for (long long w = threadIdx.x; w < words; w += 256) to[w] = from[w];
+    uint4* to = reinterpret_cast<uint4*>(base + (size_t)d * b.page_stride);
+    for (int w0 = tid; w0 < words; w0 += 256 * kFlight) {
+      uint4 x[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k)
+        if (w0 + 256 * k < words) x[k] = __ldcs(from + w0 + 256 * k);
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k)
+        if (w0 + 256 * k < words) __stcs(to + w0 + 256 * k, x[k]);
+    }
   }
 }
 
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
+int launched(const char* what, cudaError_t e) {
+  (void)cudaGetLastError();
   if (e == cudaSuccess) return W4A16_OK;
   set_error("%s launch failed: %s", what, cudaGetErrorString(e));
   return W4A16_ERR_CUDA;
 }
 
-int launch_moves(const PageBlocks& b, const int2* pairs, const int* src, const int* dst, int n, const int* count, cudaStream_t stream) {
+int launch_apply(const PageBlocks& b, const int2* pairs, const int* src, const int* dst, int n, const int* count, const TableWork& t,
+                 cudaStream_t stream) {
   int sms = 0;
   const int rc = current_sm_count(&sms);
   if (rc != W4A16_OK) return rc;
-  const long long items = 2LL * n * b.layers, most = (long long)sms * 8;
-  k_page_moves<<<(unsigned)(items < most ? items : most), 256, 0, stream>>>(b, pairs, src, dst, n, count);
-  return launched("k_page_moves");
+  const long long items = 2LL * n * b.layers, most = (long long)sms * 4;
+  return launched("k_pages_apply", launch_maybe_pdl(k_pages_apply, dim3((unsigned)(t.ctas + (items < most ? items : most))), dim3(256), 0,
+                                                    stream, true, b, pairs, src, dst, n, count, t));
 }
 
 }  // namespace
 
 int launch_pages_extend(const PagesState& st, const int* seqs, const int* counts, int n, int* ok, cudaStream_t stream) {
-  k_pages_plan<<<1, kPlanThreads, 0, stream>>>(st, seqs, nullptr, counts, n, ok, nullptr);
-  return launched("k_pages_plan");
+  return launched("k_pages_plan", launch_maybe_pdl(k_pages_plan, dim3(1), dim3(kPlanThreads), 0, stream, true, st, seqs,
+                                                   (const int*)nullptr, counts, n, ok, (int2*)nullptr));
 }
 
 int launch_pages_fork(const PagesState& st, const PageBlocks& b, const int* src, const int* dst, int n, int* ok, void* scratch,
                       cudaStream_t stream) {
   int2* moves = static_cast<int2*>(scratch);
-  k_pages_plan<<<1, kPlanThreads, 0, stream>>>(st, dst, src, nullptr, n, ok, moves);
-  int rc = launched("k_pages_plan");
+  const int rc = launched("k_pages_plan", launch_maybe_pdl(k_pages_plan, dim3(1), dim3(kPlanThreads), 0, stream, true, st, dst, src,
+                                                           (const int*)nullptr, n, ok, moves));
   if (rc != W4A16_OK) return rc;
-  const int blocks = (st.width + 1023) / 1024;
-  k_pages_share<<<dim3(blocks, n), 256, 0, stream>>>(st, src, dst, ok);
-  rc = launched("k_pages_share");
-  return rc == W4A16_OK ? launch_moves(b, moves, nullptr, nullptr, n, nullptr, stream) : rc;
+  TableWork t;
+  t.ctas = n < 128 ? n : 128;
+  t.st = st;
+  t.src = src;
+  t.dst = dst;
+  t.ok = ok;
+  t.n = n;
+  return launch_apply(b, moves, nullptr, nullptr, n, nullptr, t, stream);
 }
 
 int launch_pages_free(const PagesState& st, const int* seqs, int n, int* ok, cudaStream_t stream) {
-  k_pages_free<<<n, 256, 0, stream>>>(st, seqs, n, ok);
-  return launched("k_pages_free");
+  return launched("k_pages_free", launch_maybe_pdl(k_pages_free, dim3(n), dim3(256), 0, stream, true, st, seqs, n, ok));
 }
 
 int launch_pages_copy(const PageBlocks& b, const int* src, const int* dst, int n, cudaStream_t stream) {
-  return launch_moves(b, nullptr, src, dst, n, nullptr, stream);
+  return launch_apply(b, nullptr, src, dst, n, nullptr, TableWork(), stream);
 }
 
 size_t pages_compact_scratch_bytes(int pages) { return (size_t)pages * 12; }
@@ -279,15 +325,16 @@ int launch_pages_compact(const PageBlocks& b, const int* tables, int* tables_out
                          int* moved, void* scratch, cudaStream_t stream) {
   int2* moves = static_cast<int2*>(scratch);
   int* where = reinterpret_cast<int*>(moves + b.pages);
-  k_compact_plan<<<1, 1024, 0, stream>>>(refs, b.pages, refs_out, where, moves, moved);
-  int rc = launched("k_compact_plan");
+  const int rc = launched("k_compact_plan", launch_maybe_pdl(k_compact_plan, dim3(1), dim3(1024), 0, stream, true, refs, b.pages, refs_out,
+                                                             where, moves, moved));
   if (rc != W4A16_OK) return rc;
-  if (entries > 0) {
-    const long long blocks = (entries + 255) / 256;
-    k_tables_remap<<<(unsigned)(blocks < 1024 ? blocks : 1024), 256, 0, stream>>>(tables, tables_out, entries, where, b.pages);
-    rc = launched("k_tables_remap");
-  }
-  return rc == W4A16_OK ? launch_moves(b, moves, nullptr, nullptr, b.pages, moved, stream) : rc;
+  TableWork t;
+  t.tables = tables;
+  t.out = tables_out;
+  t.where = where;
+  t.entries = entries;
+  t.ctas = (int)((entries + 1023) / 1024 < 128 ? (entries + 1023) / 1024 : 128);
+  return launch_apply(b, moves, nullptr, nullptr, b.pages, moved, t, stream);
 }
 
 }  // namespace w4a16
