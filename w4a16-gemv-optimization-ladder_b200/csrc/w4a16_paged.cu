@@ -35,70 +35,82 @@ __device__ __forceinline__ int page_of(const PagedTables& t, int s, int p, int p
 
 // ---------------------------------------------------------------------------- append
 //
-// One thread turns 8 pairs (i, i + D/2) of one head of one token: two 16-byte loads, two
-// 16-byte stores, angles read as float4 (they stay in L1 across a token's heads).
+// Bound by the bytes of q, k and v, read once and written once.  A CTA takes a token at a time;
+// a thread turns 8 pairs (i, i + D/2) of every 16th head with the angles of its pairs in
+// registers, kBatch heads' loads in flight before the token's position and page are known.
+template <int D>
+constexpr int append_threads() { return 16 * (D / 16); }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_paged_append(const PagedAppend a, const PagedPool pool, const PagedTables tab) {
-  constexpr int kChunks = D / 16;
+__global__ void __launch_bounds__(append_threads<D>(), 768 / append_threads<D>())
+    k_paged_append(const PagedAppend a, const PagedPool pool, const PagedTables tab) {
+  constexpr int kChunks = D / 16, kBatch = 3;
   grid_dependency_wait();
   grid_launch_dependents();
-  const int per_token = (a.heads + 2 * pool.kv_heads) * kChunks;
-  const long long total = (long long)a.tokens * per_token;
-  for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
-    const int t = (int)(e / per_token), r = (int)(e % per_token);
-    const int head = r / kChunks, i = (r % kChunks) * 8;
+  const int slot = threadIdx.x / kChunks, i = threadIdx.x % kChunks * 8;
+  const int keys = a.heads, values = a.heads + pool.kv_heads, all = values + pool.kv_heads;  // heads in the order q, k, v
+  for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
     const int pos = __ldg(a.positions + t);
     const int seq = a.seqs ? __ldg(a.seqs + t) : t;
-    int page = pos < 0 ? -1 : page_of(tab, seq, pos, pool.page_shift, pool.pages);
-    if (a.cos_t && pos >= a.angle_rows) page = -1;
-    const bool is_q = head < a.heads;
-    if (!is_q && page < 0) continue;
-    uint4 lo, hi;
-    T* dst;
-    if (is_q) {
-      dst = static_cast<T*>(a.q_out) + (size_t)t * a.q_out_stride + head * D;
-      if (page < 0) {  // padding: zeros; a bad position, sequence or page: NaN
-        const uint32_t w = pos < 0 ? 0u : pack2<T>(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
-        lo = hi = make_uint4(w, w, w, w);
-        *reinterpret_cast<uint4*>(dst + i) = lo;
-        *reinterpret_cast<uint4*>(dst + i + D / 2) = hi;
-        continue;
-      }
-      const T* src = static_cast<const T*>(a.q) + (size_t)t * a.q_stride + head * D;
-      lo = *reinterpret_cast<const uint4*>(src + i);
-      hi = *reinterpret_cast<const uint4*>(src + i + D / 2);
-    } else {
-      const int kvh = (head - a.heads) % pool.kv_heads;
-      const bool is_v = head - a.heads >= pool.kv_heads;
-      const T* src = is_v ? static_cast<const T*>(a.v) + (size_t)t * a.v_stride + kvh * D
-                          : static_cast<const T*>(a.k) + (size_t)t * a.k_stride + kvh * D;
-      dst = static_cast<T*>(is_v ? pool.v : pool.k) + (size_t)page * pool.page_stride + (size_t)kvh * pool.head_stride +
-            (size_t)(pos & ((1 << pool.page_shift) - 1)) * pool.token_stride;
-      lo = *reinterpret_cast<const uint4*>(src + i);
-      hi = *reinterpret_cast<const uint4*>(src + i + D / 2);
-      if (is_v) {
-        *reinterpret_cast<uint4*>(dst + i) = lo;
-        *reinterpret_cast<uint4*>(dst + i + D / 2) = hi;
-        continue;
-      }
-    }
-    if (a.cos_t) {
-      uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
-      uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
-      const float* cr = a.cos_t + (size_t)pos * D + i;
-      const float* sr = a.sin_t + (size_t)pos * D + i;
+    const T* q = static_cast<const T*>(a.q) + (size_t)t * a.q_stride + i;
+    const T* k = static_cast<const T*>(a.k) + (size_t)t * a.k_stride + i;
+    const T* v = static_cast<const T*>(a.v) + (size_t)t * a.v_stride + i;
+    int page = -1;
+    float4 cs[8];  // cos, sin of the pairs' first halves, then of their second
+    size_t place = 0;
+    for (int h0 = 0; h0 < all; h0 += 16 * kBatch) {
+      uint4 lo[kBatch], hi[kBatch];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = unpack2<T>(l[j]), y = unpack2<T>(h[j]);
-        const float2 c0 = __ldg(reinterpret_cast<const float2*>(cr) + j), s0 = __ldg(reinterpret_cast<const float2*>(sr) + j);
-        const float2 c1 = __ldg(reinterpret_cast<const float2*>(cr + D / 2) + j);
-        const float2 s1 = __ldg(reinterpret_cast<const float2*>(sr + D / 2) + j);
-        l[j] = pack2<T>(x.x * c0.x - y.x * s0.x, x.y * c0.y - y.y * s0.y);
-        h[j] = pack2<T>(y.x * c1.x + x.x * s1.x, y.y * c1.y + x.y * s1.y);
+      for (int b = 0; b < kBatch; ++b) {
+        const int h = h0 + 16 * b + slot;
+        if (h >= all) continue;
+        const T* src = h < keys ? q + (size_t)h * D : h < values ? k + (size_t)(h - keys) * D : v + (size_t)(h - values) * D;
+        lo[b] = *reinterpret_cast<const uint4*>(src);
+        hi[b] = *reinterpret_cast<const uint4*>(src + D / 2);
+      }
+      if (h0 == 0) {
+        page = pos < 0 || (a.cos_t && pos >= a.angle_rows) ? -1 : page_of(tab, seq, pos, pool.page_shift, pool.pages);
+        if (page >= 0) {
+          place = (size_t)page * pool.page_stride + (size_t)(pos & ((1 << pool.page_shift) - 1)) * pool.token_stride + i;
+          if (a.cos_t) {
+            const float4* c = reinterpret_cast<const float4*>(a.cos_t + (size_t)pos * D + i);
+            const float4* s = reinterpret_cast<const float4*>(a.sin_t + (size_t)pos * D + i);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              cs[e] = __ldg(c + e);
+              cs[2 + e] = __ldg(s + e);
+              cs[4 + e] = __ldg(c + D / 8 + e);
+              cs[6 + e] = __ldg(s + D / 8 + e);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int h = h0 + 16 * b + slot;
+        if (h >= all || (page < 0 && h >= keys)) continue;
+        if (page < 0) {  // padding: zeros; a bad position, sequence or page: NaN
+          const uint32_t w = pos < 0 ? 0u : pack2<T>(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+          lo[b] = hi[b] = make_uint4(w, w, w, w);
+        } else if (a.cos_t && h < values) {
+          uint32_t* l = reinterpret_cast<uint32_t*>(&lo[b]);
+          uint32_t* u = reinterpret_cast<uint32_t*>(&hi[b]);
+          const float2* c = reinterpret_cast<const float2*>(cs);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = unpack2<T>(l[e]), y = unpack2<T>(u[e]);
+            const float2 c0 = c[e], s0 = c[4 + e], c1 = c[8 + e], s1 = c[12 + e];
+            l[e] = pack2<T>(x.x * c0.x - y.x * s0.x, x.y * c0.y - y.y * s0.y);
+            u[e] = pack2<T>(y.x * c1.x + x.x * s1.x, y.y * c1.y + x.y * s1.y);
+          }
+        }
+        T* dst = h < keys     ? static_cast<T*>(a.q_out) + (size_t)t * a.q_out_stride + (size_t)h * D + i
+                 : h < values ? static_cast<T*>(pool.k) + place + (size_t)(h - keys) * pool.head_stride
+                              : static_cast<T*>(pool.v) + place + (size_t)(h - values) * pool.head_stride;
+        *reinterpret_cast<uint4*>(dst) = lo[b];
+        *reinterpret_cast<uint4*>(dst + D / 2) = hi[b];
       }
     }
-    *reinterpret_cast<uint4*>(dst + i) = lo;
-    *reinterpret_cast<uint4*>(dst + i + D / 2) = hi;
   }
 }
 
@@ -787,9 +799,9 @@ int launch_paged_append(const PagedAppend& a, const PagedPool& pool, const Paged
   return by_type(pool.dtype, pool.head_dim, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    const long long total = (long long)a.tokens * (a.heads + 2 * pool.kv_heads) * (D / 16);
-    const long long blocks = (total + 255) / 256, most = (long long)sms * 8;
-    return launched("k_paged_append", launch_maybe_pdl(k_paged_append<T, D>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0,
+    constexpr int threads = append_threads<D>();
+    const int most = sms * (2048 / threads);
+    return launched("k_paged_append", launch_maybe_pdl(k_paged_append<T, D>, dim3(a.tokens < most ? a.tokens : most), dim3(threads), 0,
                                                        stream, true, a, pool, tab));
   });
 }
