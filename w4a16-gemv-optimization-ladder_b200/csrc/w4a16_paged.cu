@@ -42,9 +42,9 @@ template <int D>
 constexpr int append_threads() { return 16 * (D / 16); }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(append_threads<D>(), 768 / append_threads<D>())
+__global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>())
     k_paged_append(const PagedAppend a, const PagedPool pool, const PagedTables tab) {
-  constexpr int kChunks = D / 16, kBatch = 3;
+  constexpr int kChunks = D / 16, kBatch = 2;
   grid_dependency_wait();
   grid_launch_dependents();
   const int slot = threadIdx.x / kChunks, i = threadIdx.x % kChunks * 8;
@@ -800,7 +800,7 @@ int launch_paged_append(const PagedAppend& a, const PagedPool& pool, const Paged
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     constexpr int threads = append_threads<D>();
-    const int most = sms * (2048 / threads);
+    const int most = sms * (2048 / threads);  // more than fit at once: the faster SMs take more
     return launched("k_paged_append", launch_maybe_pdl(k_paged_append<T, D>, dim3(a.tokens < most ? a.tokens : most), dim3(threads), 0,
                                                        stream, true, a, pool, tab));
   });
