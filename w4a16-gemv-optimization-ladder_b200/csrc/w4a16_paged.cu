@@ -397,20 +397,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     load(i);
     look_up();
   }
+  uint4 q[NH][kB];
+  auto load_q = [&](const Span& sp) {
+    const int h0 = sp.item / blocks * group + sp.item % blocks * kHeads, nheads = min(kHeads, group - sp.item % blocks * kHeads);
+    const T* src = static_cast<const T*>(a.q) + (size_t)sp.row * a.q_stride + (size_t)(h0 + g) * D + 8 * j;
+#pragma unroll
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+      for (int b = 0; b < kB; ++b)
+        q[n][b] = n * 8 + g < nheads ? *reinterpret_cast<const uint4*>(src + n * 8 * D + 32 * b) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  load_q(cur);
   int stage = 0;
   for (long long u = u0;;) {
     const int row = cur.row, item = cur.item, t0 = cur.t0, t1 = cur.t1, len = cur.len, nt = cur.nt;
     const int kvh = item / blocks, h0 = kvh * group + (item % blocks) * kHeads;
     const int nheads = min(kHeads, group - (item % blocks) * kHeads);
 
-    uint4 q[NH][kB];
-#pragma unroll
-    for (int n = 0; n < NH; ++n)
-#pragma unroll
-      for (int b = 0; b < kB; ++b)
-        q[n][b] = n * 8 + g < nheads ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (size_t)row * a.q_stride +
-                                                                       (size_t)(h0 + n * 8 + g) * D + 32 * b + 8 * j)
-                                     : make_uint4(0u, 0u, 0u, 0u);
     float o[NH][kVB * 4][4];
     float m[NH][2], l[NH][2];
 #pragma unroll
@@ -523,6 +526,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
           }
         }
     }
+    const long long begun = u;
+    u += t1 - t0;
+    if (u < u1) {  // the next span's queries are on their way while this one's parts are joined
+      next_span(cur, u);
+      load_q(cur);
+    }
     if (__any_sync(0xffffffffu, no_page)) {
 #pragma unroll
       for (int n = 0; n < NH; ++n) l[n][0] = l[n][1] = nan;
@@ -624,16 +633,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     }
     if (!whole && t0 == 0 && (coop ? threadIdx.x == 0 : lane == 0)) {
       // the worker of the item's last unit, which lies nt - t1 units past this span
-      const long long last = u + nt - 1;
+      const long long last = begun + nt - 1;
       desc[worker].row = row;
       desc[worker].item = item;
       const long long whole_ones = more * (each + 1);
       const int w = last < whole_ones ? (int)divide(last, each + 1) : more + (int)divide(last - whole_ones, each);
       desc[worker].parts = w - worker + 1;
     }
-    u += t1 - t0;
     if (u >= u1) break;
-    next_span(cur, u);
   }
   copies_wait<0>();
 }
