@@ -144,6 +144,9 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
 // workspace (slot 2w + 1 if the part begins the item, else 2w) and are joined by k_paged_join.
 constexpr int kAttnWarps = 4;
 constexpr int kAttnMaxSms = 148;  // bounds the workspace
+// What it costs to begin and end an item, in units of a warp's and of a CTA's work (256 rows of
+// up to 200 positions: 30 us with it, 34 without; 32 rows of up to 4096: 52 and 53).
+constexpr int kItemCost = 2, kItemCostCta = 1;
 // Workers for each item at most: more cost more to join than they save (one sequence of 30000
 // positions with one kv head: 16.5 us with 64, 20.9 with 32, 17.9 with 128, 28.6 without a bound).
 constexpr int kMaxParts = 64;
@@ -216,7 +219,7 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
 template <typename T, int D, int NH>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     k_paged_attention(const PagedAttention a, const PagedPool pool, const PagedTables tab, const int group, const int blocks,
-                      const bool coop) {
+                      const bool coop, const int cost) {
   using C = AttnCfg<D, NH>;
   constexpr int kB = D / 32, kVB = D / 64, kU = C::kTiles, kHeads = C::kHeads, kThreads = kAttnWarps * 32, kPos = C::kPos;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
@@ -242,7 +245,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     const int n = __ldg(a.lengths + row);
     return n <= 0 ? 0 : n > cap ? (int)(cap + 1) : n;
   };
-  auto tiles = [&](int len) { return (len + unit - 1) / unit; };
+  // An item's units: those of its positions, then cost more that stand for what it takes to begin
+  // and end one
+  auto tiles = [&](int len) { return len == 0 ? 0 : (len + unit - 1) / unit + cost; };
 
   // the units of all rows, and the row that holds each worker's first one
   const int per = (a.rows + kThreads - 1) / kThreads;
@@ -335,8 +340,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   // page of position pos + lane: -1 for none, -2 where a position has none and should
   auto look_up = [&]() {
     page = -1;
-    if (ahead_u >= u1) return;
-    if (ahead_t == ahead.t1) {
+    while (ahead_t >= min(ahead.t1, ahead.nt - cost)) {  // the span's positions are done
+      ahead_u += ahead.t1 - ahead.t0;
+      if (ahead_u >= u1) {
+        ahead.t0 = ahead.t1;  // stay here
+        pos = ahead_len;      // a stage without positions
+        return;
+      }
       next_span(ahead, ahead_u);
       ahead_t = 0;
       enter();
@@ -349,7 +359,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       if (page < 0 || page >= pool.pages) page = -2;
     }
     ++ahead_t;
-    ++ahead_u;
   };
   const int tmask = (1 << pool.page_shift) - 1;
   constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows of one copy instruction
@@ -360,6 +369,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   unsigned bad = 0;  // bit: the stage holds a position without a page
   auto load = [&](int stage) {
     const uint32_t dst = ring + stage * 2 * C::kHalf;
+    if (pos >= ahead_len) {  // a unit without positions for this warp
+      copies_commit();
+      return;
+    }
     bad = (bad & ~(1u << stage)) | (page == -2 ? 1u << stage : 0u);
     auto copy = [&](int r, size_t at, bool any) {
       const uint32_t to = dst + r * (D * 2) + ((chunk & ~7) | ((chunk & 7) ^ swizzle(r))) * 16;
@@ -425,7 +438,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     }
 
     bool no_page = false;
-    for (int tile = t0; tile < t1; ++tile) {
+    for (int tile = t0; tile < min(t1, nt - cost); ++tile) {
       copies_wait<C::kStages - 2>();
       __syncwarp();  // every lane's copies of this stage are in, its reads of the one before done
       load(stage == 0 ? C::kStages - 1 : stage - 1);
@@ -829,6 +842,8 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   const int ctas = (sms < kAttnMaxSms ? sms : kAttnMaxSms) * C::kPerSm;
   const bool coop = (long long)a.rows * pool.kv_heads * blocks < ctas * kAttnWarps;
   const int workers = coop ? ctas : ctas * kAttnWarps;
+  // with far fewer items than CTAs a CTA has one at most, and the cost of beginning it is no matter of balance
+  const int cost = !coop ? kItemCost : (long long)a.rows * pool.kv_heads * blocks * 4 >= ctas ? kItemCostCta : 0;
   static std::atomic<uint64_t> configured{0};  // one bit per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -838,7 +853,7 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   }
   if (e != cudaSuccess) return launched("configuring k_paged_attention,", e);
   const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
-                                                                 stream, true, a, pool, tab, group, blocks, coop));
+                                                                 stream, true, a, pool, tab, group, blocks, coop, cost));
   if (rc2 != W4A16_OK) return rc2;
   constexpr int lanes = join_lanes<D, NH>();
   return launched("k_paged_join",
