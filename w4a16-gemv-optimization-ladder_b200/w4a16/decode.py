@@ -27,6 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from . import kernels as K
+from .logits import process_logits
 
 GROUP = 128
 
@@ -286,6 +287,8 @@ class W4A16LlamaDecoder:
         self.gen_tokens = torch.zeros(cfg.max_len, dtype=torch.long, device=dev)
         self.gen_idx = torch.zeros(1, dtype=torch.long, device=dev)
         self.gen_graph = None
+        self.gen_rules = None       # process_logits' inputs for generate(), static for its graph
+        self.gen_rules_graph = None
 
     # ------------------------------------------------------------------ pieces
 
@@ -393,7 +396,39 @@ class W4A16LlamaDecoder:
         self.lm_head(x, out=self.logits)
         return self.logits
 
+    def _project(self, p, x, out_dtype=torch.float16):
+        """[T, rows] = x [T, cols] times a projection, T of any size."""
+        if p.dense:
+            return F.linear(x, p.w).to(out_dtype)
+        if x.shape[0] <= 64:
+            return K.gemv(p.packed, p.scale, x, group=GROUP, out_dtype=out_dtype)
+        return K.gemm(p.packed, p.scale, x, group=GROUP, out_dtype=out_dtype)
+
     # ------------------------------------------------------------------- public
+
+    def step_paged(self, tokens, seqs, positions, cache):
+        """Logits (fp32 [T, vocab]) of T tokens of any sequences of a paged cache, prompts' tokens and
+        single new ones mixed: token t (tokens int64 [T]) is position positions[t] (int32) of sequence
+        seqs[t] (int32), for which cache.extend has made room, and attends to the positions up to
+        its own.  A negative position is padding.  cache: a PagedKVCache of this model's layers,
+        kv heads and head_dim, in fp16."""
+        cfg, D = self.cfg, self.cfg.head_dim
+        if cache.k.dtype != torch.float16 or tuple(cache.k.shape[i] for i in (0, 2, 4)) != (cfg.layers, cfg.kv_heads, D):
+            raise ValueError(f"the cache must be fp16 with {cfg.layers} layers, {cfg.kv_heads} kv heads and head_dim {D}")
+        lengths = positions + 1
+        h = self.embed.index_select(0, tokens).float()
+
+        def norm(w):
+            return (h * torch.rsqrt(h.pow(2).mean(1, keepdim=True) + cfg.eps) * w).half()
+
+        for li, L in enumerate(self.layers):
+            qkv = self._project(L["qkv"], norm(L["norm_attn"])).unflatten(1, (-1, D))
+            q, k, v = qkv.split([cfg.heads, cfg.kv_heads, cfg.kv_heads], dim=1)
+            cache.append(li, q, k, v, positions, cos=self.cos, sin=self.sin, seqs=seqs, out=q)
+            h = h + self._project(L["o"], cache.attention(li, q, lengths, seqs=seqs).flatten(1), torch.float32)
+            gate, up = split_gate_up(self._project(L["gu"], norm(L["norm_mlp"])).t(), cfg.intermediate, self.gu_interleaved)
+            h = h + self._project(L["down"], (F.silu(gate.float()) * up.float()).half().t().contiguous(), torch.float32)
+        return self._project(self.lm_head, norm(self.norm_final), torch.float32)
 
     def step(self, token, pos):
         """Eager step: logits (fp32 [vocab]) for `token` at position `pos`."""
@@ -415,17 +450,35 @@ class W4A16LlamaDecoder:
             self._step()
         return self.graph
 
-    def _greedy_step(self):
+    def _greedy_step(self, rules=False):
         logits = self._step()
+        if rules:
+            r = self.gen_rules
+            logits = process_logits(logits.view(1, -1), **r)
         nxt = torch.argmax(logits).view(1)
+        if rules:
+            r["tokens"].view(-1).index_copy_(0, r["total_lens"].long(), nxt)
+            r["total_lens"].add_(1)
         self.gen_tokens.index_copy_(0, self.gen_idx, nxt)
         self.token.copy_(nxt)
         self.pos.add_(1)
         self.gen_idx.add_(1)
 
-    def capture_generate(self):
+    def capture_generate(self, rules=False):
         """Record one greedy step in a CUDA graph: the step, the argmax of the logits fed
-        back as the next token, the position advanced; replays need no host round trip."""
+        back as the next token, the position advanced; replays need no host round trip.
+        rules: the logits go through process_logits with self.gen_rules first."""
+        if rules:
+            cfg, dev = self.cfg, self.device
+
+            def one(x, dtype=torch.float32):
+                return torch.full((1,), x, dtype=dtype, device=dev)
+
+            self.gen_rules = dict(
+                tokens=torch.zeros(1, 2 * cfg.max_len, dtype=torch.long, device=dev), prompt_lens=one(0, torch.int32),
+                total_lens=one(0, torch.int32), repetition=one(1.0), frequency=one(0.0), presence=one(0.0),
+                bias=torch.zeros(cfg.vocab, device=dev),
+                mask=torch.full((-(-cfg.vocab // 32),), -1, dtype=torch.int32, device=dev))
         K.reserve_workspace(self.device, 1, self.cfg.vocab, self.cfg.hidden)
         saved = (self.token.clone(), self.pos.clone(), self.gen_idx.clone(), self.k_cache.clone(),
                  self.v_cache.clone())
@@ -435,27 +488,51 @@ class W4A16LlamaDecoder:
             for _ in range(2):  # warm-up outside capture (restored below)
                 self.pos.zero_()
                 self.gen_idx.zero_()
-                self._greedy_step()
+                self._greedy_step(rules)
         torch.cuda.current_stream(self.device).wait_stream(s)
-        self.gen_graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.gen_graph):
-            self._greedy_step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self._greedy_step(rules)
+        if rules:
+            self.gen_rules_graph = graph
+        else:
+            self.gen_graph = graph
         for t, v in zip((self.token, self.pos, self.gen_idx, self.k_cache, self.v_cache), saved):
             t.copy_(v)
-        return self.gen_graph
+        return graph
 
-    def generate(self, token, pos, n):
+    def generate(self, token, pos, n, *, prompt=None, repetition=None, frequency=None, presence=None, bias=None, mask=None):
         """Greedy continuation of `token` at position `pos` for n tokens (graph replays);
-        returns the n generated token ids on the host."""
+        returns the n generated token ids on the host.  With any of the keywords each step's
+        logits go through process_logits: repetition, frequency and presence are its penalties
+        (numbers), prompt the ids before the first generated one (default [token]), bias fp32
+        [vocab] and mask int32 [ceil(vocab / 32)] tensors."""
         if pos + n > self.cfg.max_len:
             raise ValueError(f"pos + n = {pos + n} exceeds the cache length {self.cfg.max_len}")
-        if self.gen_graph is None:
+        rules = any(x is not None for x in (prompt, repetition, frequency, presence, bias, mask))
+        if rules:
+            prompt = [int(token)] if prompt is None else [int(x) for x in prompt]
+            if len(prompt) > self.cfg.max_len:
+                raise ValueError(f"a prompt of {len(prompt)} ids exceeds the cache length {self.cfg.max_len}")
+            if self.gen_rules_graph is None:
+                self.capture_generate(rules=True)
+            r = self.gen_rules
+            r["tokens"][0, :len(prompt)] = torch.tensor(prompt, dtype=torch.long)
+            for name, value in (("prompt_lens", len(prompt)), ("total_lens", len(prompt)), ("repetition", 1.0 if repetition is None else repetition),
+                                ("frequency", frequency or 0.0), ("presence", presence or 0.0), ("bias", 0.0 if bias is None else bias),
+                                ("mask", -1 if mask is None else mask)):
+                if isinstance(value, torch.Tensor):
+                    r[name].copy_(value)
+                else:
+                    r[name].fill_(value)
+        elif self.gen_graph is None:
             self.capture_generate()
+        graph = self.gen_rules_graph if rules else self.gen_graph
         self.token.fill_(int(token))
         self.pos.fill_(int(pos))
         self.gen_idx.zero_()
         for _ in range(n):
-            self.gen_graph.replay()
+            graph.replay()
         return self.gen_tokens[:n].cpu()
 
     def replay(self, token, pos):
