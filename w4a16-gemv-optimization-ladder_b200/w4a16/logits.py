@@ -12,7 +12,8 @@ _LOGIT_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, t
 def _per_row(t, rows, dtype, name, dev):
     if t is None:
         return None
-    if not (isinstance(t, torch.Tensor) and t.device == dev and t.dtype == dtype and t.shape == (rows,) and t.is_contiguous()):
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev and t.dim() == 1 and t.shape[0] == rows
+            and t.is_contiguous()):
         _refuse(f"{name} must be a contiguous {dtype} [{rows}] tensor on {dev}")
     return t.data_ptr()
 
@@ -54,37 +55,40 @@ def process_logits(logits, *, tokens=None, prompt_lens=None, total_lens=None, re
     rows, vocab = (1, shape[0]) if len(shape) == 1 else shape
     if out is None:
         out = logits.new_empty(shape)
-    d = _lib.LogitsDesc()
-    d.logits, d.out, d.dtype = logits.data_ptr(), _rows(out, (logits.dtype,), (shape,), "out", dev), _LOGIT_DTYPES[logits.dtype]
-    d.rows, d.vocab = rows, vocab
-    d.stride, d.out_stride = (vocab, vocab) if rows <= 1 else (logits.stride(0), out.stride(0))
+    else:
+        _rows(out, (logits.dtype,), (shape,), "out", dev)
+    tp = pl = tl = rp = fp = pp = bp = ip = vp = mp = None
+    token_bytes = history = token_stride = bias_stride = pairs = mask_stride = 0
     if tokens is not None:
         if not (isinstance(tokens, torch.Tensor) and tokens.dim() == 2):
             _refuse(f"tokens must be an int32 or int64 [{rows}, history] tensor")
-        d.tokens = _rows(tokens, (torch.int32, torch.int64), ((rows, tokens.shape[1]),), "tokens", dev)
-        d.token_bytes, d.history, d.token_stride = tokens.element_size(), tokens.shape[1], tokens.stride(0)
-        d.prompt_lens = _per_row(prompt_lens, rows, torch.int32, "prompt_lens", dev)
-        d.total_lens = _per_row(total_lens, rows, torch.int32, "total_lens", dev)
-        d.repetition = _per_row(repetition, rows, torch.float32, "repetition", dev)
-        d.frequency = _per_row(frequency, rows, torch.float32, "frequency", dev)
-        d.presence = _per_row(presence, rows, torch.float32, "presence", dev)
+        history = tokens.shape[1]
+        tp = _rows(tokens, (torch.int32, torch.int64), ((rows, history),), "tokens", dev)
+        token_bytes, token_stride = tokens.element_size(), tokens.stride(0)
+        pl = _per_row(prompt_lens, rows, torch.int32, "prompt_lens", dev)
+        tl = _per_row(total_lens, rows, torch.int32, "total_lens", dev)
+        rp = _per_row(repetition, rows, torch.float32, "repetition", dev)
+        fp = _per_row(frequency, rows, torch.float32, "frequency", dev)
+        pp = _per_row(presence, rows, torch.float32, "presence", dev)
     elif not (prompt_lens is total_lens is repetition is frequency is presence is None):
         _refuse("penalties and lengths need tokens")
     if bias is not None:
-        d.bias = _rows(bias, (torch.float32,), ((vocab,), (rows, vocab)), "bias", dev)
-        d.bias_stride = bias.stride(0) if bias.dim() == 2 and rows > 1 else 0
+        bp = _rows(bias, (torch.float32,), ((vocab,), (rows, vocab)), "bias", dev)
+        bias_stride = bias.stride(0) if bias.dim() == 2 and rows > 1 else 0
     if bias_ids is not None or bias_values is not None:
         if not (isinstance(bias_ids, torch.Tensor) and bias_ids.dim() == 2 and isinstance(bias_values, torch.Tensor)
                 and bias_ids.is_contiguous() and bias_values.is_contiguous()):
             _refuse(f"bias_ids and bias_values must be contiguous [{rows}, pairs] tensors, and go together")
-        shape = (rows, bias_ids.shape[1])
-        d.bias_ids = _rows(bias_ids, (torch.int32,), (shape,), "bias_ids", dev)
-        d.bias_values = _rows(bias_values, (torch.float32,), (shape,), "bias_values", dev)
-        d.pairs = shape[1]
+        pairs = bias_ids.shape[1]
+        ip = _rows(bias_ids, (torch.int32,), ((rows, pairs),), "bias_ids", dev)
+        vp = _rows(bias_values, (torch.float32,), ((rows, pairs),), "bias_values", dev)
     if mask is not None:
         words = -(-vocab // 32)
-        d.mask = _rows(mask, (torch.int32,), ((words,), (rows, words)), "mask", dev)
-        d.mask_stride = mask.stride(0) if mask.dim() == 2 and rows > 1 else 0
+        mp = _rows(mask, (torch.int32,), ((words,), (rows, words)), "mask", dev)
+        mask_stride = mask.stride(0) if mask.dim() == 2 and rows > 1 else 0
     if rows and vocab:
+        stride, out_stride = (vocab, vocab) if rows == 1 else (logits.stride(0), out.stride(0))
+        d = _lib.LogitsDesc(logits.data_ptr(), out.data_ptr(), _LOGIT_DTYPES[logits.dtype], rows, vocab, stride, out_stride, tp, token_bytes,
+                            history, token_stride, pl, tl, rp, fp, pp, bp, bias_stride, ip, vp, pairs, mp, mask_stride)
         _call("w4a16_process_logits", dev, _byref(d))
     return out

@@ -23,6 +23,7 @@ RuntimeError before anything is launched; indices are checked in the kernels (a 
 or sequence gives NaN, is skipped, or is refused, as each function says).
 """
 import ctypes
+import functools
 
 import torch
 
@@ -30,7 +31,9 @@ from . import _lib
 
 _POOL_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _byref = ctypes.byref
-_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(device).cuda_stream, without the object
+# torch.cuda.current_stream(device).cuda_stream and torch.cuda.current_device(), without the objects
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _refuse(msg):
@@ -40,31 +43,37 @@ def _refuse(msg):
 def _call(name, dev, *args):
     """Run a C entry on dev's current stream, its last argument.  The checks before it build their
     messages only when they fail: a decode step is short of host time."""
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == dev.index:
-        status = fn(*args, _raw_stream(dev.index))
+    fn, index = getattr(_lib.lib(), name), dev.index
+    if _current_device() == index:
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev.index))
+            status = fn(*args, _raw_stream(index))
     if status:
         _lib.check(status, name)
 
 
 def _pool(k_pages, v_pages):
     """The C description of one layer's pool, checked."""
-    if not (isinstance(k_pages, torch.Tensor) and k_pages.is_cuda and k_pages.dim() == 4 and k_pages.dtype in _POOL_DTYPES):
+    dtype = _POOL_DTYPES.get(getattr(k_pages, "dtype", None))
+    if dtype is None or k_pages.dim() != 4 or not k_pages.is_cuda:
         _refuse("k_pages must be an fp16 or bf16 CUDA tensor [pages, kv_heads, page_size, head_dim]")
-    stride = k_pages.stride()
-    if not (isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype == k_pages.dtype
-            and v_pages.shape == k_pages.shape and v_pages.stride() == stride):
+    shape, stride = k_pages.shape, k_pages.stride()
+    if not (isinstance(v_pages, torch.Tensor) and v_pages.device == k_pages.device and v_pages.dtype is k_pages.dtype
+            and v_pages.shape == shape and v_pages.stride() == stride):
         _refuse("v_pages must have the device, dtype, shape and strides of k_pages")
-    pages, kv_heads, page_size, head_dim = k_pages.shape
+    pages, kv_heads, page_size, head_dim = shape
     sp, sh, st, sd = stride
     if sd != 1:
         _refuse("the last dimension of the pages must be contiguous")
     # a dimension of one entry may carry any stride
-    return _lib.PagePool(k_pages.data_ptr(), v_pages.data_ptr(), _POOL_DTYPES[k_pages.dtype], pages, kv_heads, page_size,
-                         head_dim, sp if pages > 1 else 8, sh if kv_heads > 1 else 8, st if page_size > 1 else 8)
+    return _lib.PagePool(k_pages.data_ptr(), v_pages.data_ptr(), dtype, pages, kv_heads, page_size, head_dim,
+                         sp if pages > 1 else 8, sh if kv_heads > 1 else 8, st if page_size > 1 else 8)
+
+
+@functools.lru_cache(maxsize=64)
+def _attention_workspace(heads, kv_heads, head_dim):
+    return _lib.lib().w4a16_paged_attention_workspace_bytes(heads, kv_heads, head_dim)
 
 
 def _tables(tables, dev):
@@ -139,7 +148,9 @@ def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=
         qp, qs = _tokens(q, n, heads, d, dtype, "q", dev)
         if out is None:
             out = q.new_empty((n, heads, d))
-        op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
+            op, os_ = out.data_ptr(), heads * d
+        else:
+            op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
     if n:
         _call("w4a16_paged_append", dev, qp, qs, kp, ks, vp, vs, pos, sq, n, heads, _byref(tab), cp, sp, angles, _byref(pool), op, os_)
     return out
@@ -173,11 +184,13 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     tab = _tables(tables, dev)
     if out is None:
         out = q.new_empty((n, heads, d))
-    op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
+        op, os_ = out.data_ptr(), heads * d
+    else:
+        op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
     if n == 0:
         return out
     if workspace is None:
-        size = _lib.lib().w4a16_paged_attention_workspace_bytes(heads, kvh, d)
+        size = _attention_workspace(heads, kvh, d)
         workspace = q.new_empty((size + 1) // 2)
     else:
         if not (isinstance(workspace, torch.Tensor) and workspace.device == dev and workspace.dtype == torch.uint8
@@ -213,11 +226,13 @@ def _blocks(k_pages, v_pages):
     size = k_pages.element_size()
     layers, ls = (shape[0], stride[0]) if len(shape) == 5 else (1, 0)
     pages, ps = shape[-4], stride[-4]
-    elements = 1
-    for st, n in sorted(zip(stride[-3:], shape[-3:])):  # dense in some order of its dimensions
-        if n != 1 and st != elements:
-            _refuse("a page must be one dense block")
-        elements *= n
+    elements = shape[-1] * shape[-2] * shape[-3]
+    if stride[-3:] != (shape[-2] * shape[-1], shape[-1], 1):
+        block = 1
+        for st, n in sorted(zip(stride[-3:], shape[-3:])):  # dense in some order of its dimensions
+            if n != 1 and st != block:
+                _refuse("a page must be one dense block")
+            block *= n
     return _lib.PageBlocks(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, ls * size if layers > 1 else 0,
                            (ps if pages > 1 else elements) * size, elements * size)
 
