@@ -42,6 +42,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
   extern __shared__ __align__(16) uint32_t word[];
   uint2* paired = reinterpret_cast<uint2*>(word + kSlice);
   __shared__ uint32_t allowed[C::kWords], pairs_here;
+  __shared__ int first_ids[kThreads];  // the row's first pairs
+  __shared__ float first_values[kThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dependency_wait();
   grid_launch_dependents();
@@ -88,7 +90,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
     }
   }
   const int* ids = p.bias_ids + (size_t)row * p.pairs;
-  const int pair_id = tid < p.pairs ? __ldg(ids + tid) : -1;
+  const float* values = p.bias_values + (size_t)row * p.pairs;
+  if (p.pairs) {
+    first_ids[tid] = tid < p.pairs ? __ldg(ids + tid) : -1;
+    first_values[tid] = tid < p.pairs ? __ldg(values + tid) : 0.f;
+  }
   const int first_word = lo >> 5;
   if (p.mask)
     for (int i = tid; i <= ((v1 - 1) >> 5) - first_word; i += kThreads)
@@ -126,10 +132,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
     for (int j = done + tid; j < total; j += kThreads) count(token_at(j), j);
     // the first pair of an id adds up all of the id's values, in the pairs' order: a warp looks
     // at 32 pairs at a time, and for each that falls into the slice at all of the row's
-    const float* values = p.bias_values + (size_t)row * p.pairs;
     if (p.pairs) __syncthreads();  // the counts are final
+    auto id_at = [&](int k) { return k < kThreads ? first_ids[k] : k < p.pairs ? __ldg(ids + k) : -1; };
     for (int j0 = warp * 32; j0 < p.pairs; j0 += kThreads) {
-      const int id = j0 == warp * 32 ? pair_id : j0 + lane < p.pairs ? __ldg(ids + j0 + lane) : -1;
+      const int id = id_at(j0 + lane);
       unsigned here = __ballot_sync(0xffffffffu, id >= lo && id < v1);
       while (here) {
         const int src = __ffs(here) - 1, wanted = __shfl_sync(0xffffffffu, id, src);
@@ -137,8 +143,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
         float sum = 0.f;
         bool first = true;
         for (int k0 = 0; k0 < p.pairs && first; k0 += 32) {
-          const bool same = k0 + lane < p.pairs && __ldg(ids + k0 + lane) == wanted;
-          const float value = same ? __ldg(values + k0 + lane) : 0.f;
+          const bool same = id_at(k0 + lane) == wanted;  // an id in the slice is not -1
+          const float value = !same ? 0.f : k0 + lane < kThreads ? first_values[k0 + lane] : __ldg(values + k0 + lane);
           unsigned m = __ballot_sync(0xffffffffu, same);
           if (m && k0 + __ffs(m) - 1 < j0 + src) first = false;
           for (; m && first; m &= m - 1) sum += __shfl_sync(0xffffffffu, value, __ffs(m) - 1);
