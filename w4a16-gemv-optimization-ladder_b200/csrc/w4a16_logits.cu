@@ -130,30 +130,27 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
     }
 #pragma unroll 4
     for (int j = done + tid; j < total; j += kThreads) count(token_at(j), j);
-    // the first pair of an id adds up all of the id's values, in the pairs' order: a warp looks
-    // at 32 pairs at a time, and for each that falls into the slice at all of the row's
+    // the first pair of an id adds up all of the id's values, in the pairs' order: a warp for
+    // each pair that falls into the slice
     if (p.pairs) __syncthreads();  // the counts are final
     auto id_at = [&](int k) { return k < kThreads ? first_ids[k] : k < p.pairs ? __ldg(ids + k) : -1; };
-    for (int j0 = warp * 32; j0 < p.pairs; j0 += kThreads) {
-      const int id = id_at(j0 + lane);
-      unsigned here = __ballot_sync(0xffffffffu, id >= lo && id < v1);
-      while (here) {
-        const int src = __ffs(here) - 1, wanted = __shfl_sync(0xffffffffu, id, src);
-        here &= here - 1;
-        float sum = 0.f;
-        bool first = true;
-        for (int k0 = 0; k0 < p.pairs && first; k0 += 32) {
-          const bool same = id_at(k0 + lane) == wanted;  // an id in the slice is not -1
-          const float value = !same ? 0.f : k0 + lane < kThreads ? first_values[k0 + lane] : __ldg(values + k0 + lane);
-          unsigned m = __ballot_sync(0xffffffffu, same);
-          if (m && k0 + __ffs(m) - 1 < j0 + src) first = false;
-          for (; m && first; m &= m - 1) sum += __shfl_sync(0xffffffffu, value, __ffs(m) - 1);
-        }
-        if (first && lane == 0) {
-          const uint32_t i = atomicAdd(&pairs_here, 1u);
-          paired[i] = make_uint2(word[wanted - v0], __float_as_uint(sum));
-          word[wanted - v0] = kPair | i;
-        }
+#pragma unroll 1
+    for (int j = warp; j < p.pairs; j += kThreads / 32) {
+      const int wanted = id_at(j);
+      if (wanted < lo || wanted >= v1) continue;
+      float sum = 0.f;
+      bool first = true;
+      for (int k0 = 0; k0 < p.pairs && first; k0 += 32) {
+        const bool same = id_at(k0 + lane) == wanted;  // an id in the slice is not -1
+        const float value = !same ? 0.f : k0 + lane < kThreads ? first_values[k0 + lane] : __ldg(values + k0 + lane);
+        unsigned m = __ballot_sync(0xffffffffu, same);
+        if (m && k0 + __ffs(m) - 1 < j) first = false;
+        for (; m && first; m &= m - 1) sum += __shfl_sync(0xffffffffu, value, __ffs(m) - 1);
+      }
+      if (first && lane == 0) {
+        const uint32_t i = atomicAdd(&pairs_here, 1u);
+        paired[i] = make_uint2(word[wanted - v0], __float_as_uint(sum));
+        word[wanted - v0] = kPair | i;
       }
     }
   }
