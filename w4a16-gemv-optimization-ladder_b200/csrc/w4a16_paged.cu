@@ -855,10 +855,12 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
                                                                  stream, true, a, pool, tab, group, blocks, coop, cost));
   if (rc2 != W4A16_OK) return rc2;
-  constexpr int lanes = join_lanes<D, NH>();
+  // groups of threads that share an item's parts, for items few enough to be cut into many
+  constexpr int lanes = join_lanes<D, NH>(), most = 1024 / lanes < 4 ? 1024 / lanes : 4;
+  const int groups = coop && (long long)a.rows * pool.kv_heads * blocks * 2 * kJoinFew < ctas ? most : 1;
   return launched("k_paged_join",
                   launch_maybe_pdl(coop ? k_paged_join<T, D, NH, true> : k_paged_join<T, D, NH, false>, dim3(workers),
-                                   dim3(!coop ? lanes : 4 * lanes < 1024 ? 4 * lanes : 1024), 0, stream, true, a, group, blocks));
+                                   dim3(lanes * groups), 0, stream, true, a, group, blocks));
 }
 
 }  // namespace
