@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
 
 // Joins the parts of the item that worker blockIdx.x began.  A thread adds up four dimensions of
 // one head.  Few parts: kJoinFew in a round trip to memory, after the description's.  Many
-// (compiled in where workers are CTAs: up to kMaxParts parts of a long sequence): groups of threads take every G-th part, in a fixed order, and the maxima and
+// (compiled in for calls of few items: up to kMaxParts parts of a long sequence): groups of threads take every G-th part, in a fixed order, and the maxima and
 // weights come first, so that the long sums are plain multiply-adds of independent loads (one
 // sequence of 8000 positions, 8 kv heads of 64: 12.7 us with the attention, 20 with one group).
 constexpr int kJoinChunk = 128, kJoinFew = 4;
@@ -855,12 +855,13 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
                                                                  stream, true, a, pool, tab, group, blocks, coop, cost));
   if (rc2 != W4A16_OK) return rc2;
-  // groups of threads that share an item's parts, for items few enough to be cut into many
-  constexpr int lanes = join_lanes<D, NH>(), most = 1024 / lanes < 4 ? 1024 / lanes : 4;
-  const int groups = coop && (long long)a.rows * pool.kv_heads * blocks * 2 * kJoinFew < ctas ? most : 1;
+  // Items few enough to be cut into many parts get groups of threads that share them; the rest the
+  // kernel without shared memory, whose CTAs do not keep the next attention's off the SMs.
+  const bool many = coop && (long long)a.rows * pool.kv_heads * blocks * 2 * kJoinFew < ctas;
+  constexpr int lanes = join_lanes<D, NH>(), groups = 1024 / lanes < 4 ? 1024 / lanes : 4;
   return launched("k_paged_join",
-                  launch_maybe_pdl(coop ? k_paged_join<T, D, NH, true> : k_paged_join<T, D, NH, false>, dim3(workers),
-                                   dim3(lanes * groups), 0, stream, true, a, group, blocks));
+                  launch_maybe_pdl(many ? k_paged_join<T, D, NH, true> : k_paged_join<T, D, NH, false>, dim3(workers),
+                                   dim3(many ? lanes * groups : lanes), 0, stream, true, a, group, blocks));
 }
 
 }  // namespace
