@@ -671,8 +671,7 @@ template <typename T, int D, int NH, bool kMany>
 __global__ void __launch_bounds__(kMany ? 1024 : join_lanes<D, NH>()) k_paged_join(const PagedAttention a, const int group, const int blocks) {
   using C = AttnCfg<D, NH>;
   constexpr int kLanes = join_lanes<D, NH>(), kHeads = C::kHeads;
-  grid_dependency_wait();
-  grid_launch_dependents();
+  grid_dependency_wait();  // and no early launch after this: the next attention fills the GPU, and is the slower for odd places
   const AttnDesc* desc = static_cast<const AttnDesc*>(a.workspace);
   const float* slots = reinterpret_cast<const float*>(desc + C::kMaxWorkers);
   const AttnDesc it = desc[blockIdx.x];
