@@ -451,7 +451,7 @@ typedef struct {
  * that it needs for them.  fork: sequence dst[i], which must be empty, becomes a copy of
  * src[i]: whole pages are shared, a partly filled last page is copied (in every layer) to the
  * lowest free page.  free: sequence seqs[i] gives up every page in its row and becomes empty
- * (pages whose refs reach 0 are free).  n requests (1..1024; free: any number), served in
+ * (pages whose refs reach 0 are free).  n requests (0..1024; free: 0..65536), served in
  * order; all of them see the state from before the call.  ok[i] (int32) is 1, or 0 for a
  * request that was refused and changed nothing: an index out of range, a negative count, more
  * positions than the table row holds, the same seqs / dst index as an earlier request, a dst
@@ -490,7 +490,8 @@ int w4a16_pages_compact(const w4a16_page_blocks* blocks, const int32_t* tables, 
  *   x = x + bias[v] + the values of the row's pairs (bias_ids, bias_values) with id v
  *   bit v % 32 of mask[b][v / 32] is 0:       x = -inf
  * NULL leaves a part out (total_lens NULL: all `history` tokens; prompt_lens NULL: no prompt).
- * Tokens and ids outside [0, vocab) are skipped; lengths are clamped to [0, history]. */
+ * Tokens and ids outside [0, vocab) are skipped; lengths are clamped to [0, history].  The
+ * division is a product with 1 / repetition. */
 typedef struct {
   const void* logits;       /* [rows][vocab], row stride `stride` elements */
   void* out;                /* the same layout by out_stride; may be logits itself */

@@ -880,7 +880,7 @@ int w4a16_pages_free(const w4a16_page_state* state, const int32_t* seqs, int n, 
                      w4a16_stream_t stream) {
   w4a16::PagesState st;
   int rc = check_state(state, &st);
-  if (rc == W4A16_OK) rc = check_requests(n, 1 << 20, seqs, seqs, ok);
+  if (rc == W4A16_OK) rc = check_requests(n, 1 << 16, seqs, seqs, ok);
   if (rc != W4A16_OK || n == 0) return rc;
   return w4a16::launch_pages_free(st, seqs, n, ok, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -191,6 +191,14 @@ __device__ __forceinline__ uint4 ldcg128(const void* p) {
   return v;
 }
 
+// A load by the coherent path, whatever the compiler could prove about the pointer's reads here:
+// for kernels whose CTAs may be placed while the kernel before them still writes (programmatic
+// dependent launch), after their wait for it.
+template <typename T>
+__device__ __forceinline__ T fetch(const T* p) {
+  return *p;
+}
+
 __device__ __forceinline__ uint64_t globaltimer_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));

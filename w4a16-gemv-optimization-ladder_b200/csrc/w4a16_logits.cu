@@ -74,34 +74,34 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
   int total = 0, prompt = 0;
   auto token_at = [&](int j) {  // -1 for one outside the vocabulary
     const size_t at = (size_t)row * p.token_stride + j;
-    if (p.token_bytes == 4) return __ldg(static_cast<const int*>(p.tokens) + at);
-    const long long t = __ldg(static_cast<const long long*>(p.tokens) + at);
+    if (p.token_bytes == 4) return fetch(static_cast<const int*>(p.tokens) + at);
+    const long long t = fetch(static_cast<const long long*>(p.tokens) + at);
     return t < 0 || t >= p.vocab ? -1 : (int)t;
   };
   const int4* tokens4 = nullptr;  // where int32 tokens are aligned for 16-byte loads
   int4 next = make_int4(-1, -1, -1, -1);
   if (p.tokens) {
-    total = p.total_lens ? min(max(__ldg(p.total_lens + row), 0), p.history) : p.history;
-    prompt = p.prompt_lens ? __ldg(p.prompt_lens + row) : 0;
+    total = p.total_lens ? min(max(fetch(p.total_lens + row), 0), p.history) : p.history;
+    prompt = p.prompt_lens ? fetch(p.prompt_lens + row) : 0;
     const int* t = static_cast<const int*>(p.tokens) + (size_t)row * p.token_stride;
     if (p.token_bytes == 4 && reinterpret_cast<uintptr_t>(t) % 16 == 0) {
       tokens4 = reinterpret_cast<const int4*>(t);
-      if (4 * tid + 4 <= p.history) next = __ldg(tokens4 + tid);
+      if (4 * tid + 4 <= p.history) next = fetch(tokens4 + tid);
     }
   }
   const int* ids = p.bias_ids + (size_t)row * p.pairs;
   const float* values = p.bias_values + (size_t)row * p.pairs;
   if (p.pairs) {
-    first_ids[tid] = tid < p.pairs ? __ldg(ids + tid) : -1;
-    first_values[tid] = tid < p.pairs ? __ldg(values + tid) : 0.f;
+    first_ids[tid] = tid < p.pairs ? fetch(ids + tid) : -1;
+    first_values[tid] = tid < p.pairs ? fetch(values + tid) : 0.f;
   }
   const int first_word = lo >> 5;
   if (p.mask)
     for (int i = tid; i <= ((v1 - 1) >> 5) - first_word; i += kThreads)
-      allowed[i] = (uint32_t)__ldg(p.mask + (size_t)row * p.mask_stride + first_word + i);
-  const float rep = p.repetition ? __ldg(p.repetition + row) : 1.f, inv_rep = 1.f / rep;
-  const float freq = p.frequency ? __ldg(p.frequency + row) : 0.f;
-  const float pres = p.presence ? __ldg(p.presence + row) : 0.f;
+      allowed[i] = (uint32_t)fetch(p.mask + (size_t)row * p.mask_stride + first_word + i);
+  const float rep = p.repetition ? fetch(p.repetition + row) : 1.f, inv_rep = 1.f / rep;
+  const float freq = p.frequency ? fetch(p.frequency + row) : 0.f;
+  const float pres = p.presence ? fetch(p.presence + row) : 0.f;
 
   const bool marks = p.tokens || p.pairs;
   if (marks) {
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
 #pragma unroll 1
       for (int q = tid; q < total / 4; q += kThreads) {
         const int4 t = next;
-        if (q + kThreads < total / 4) next = __ldg(tokens4 + q + kThreads);
+        if (q + kThreads < total / 4) next = fetch(tokens4 + q + kThreads);
         count(t.x, 4 * q);
         count(t.y, 4 * q + 1);
         count(t.z, 4 * q + 2);
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
     // the first pair of an id adds up all of the id's values, in the pairs' order: a warp for
     // each pair that falls into the slice
     if (p.pairs) __syncthreads();  // the counts are final
-    auto id_at = [&](int k) { return k < kThreads ? first_ids[k] : k < p.pairs ? __ldg(ids + k) : -1; };
+    auto id_at = [&](int k) { return k < kThreads ? first_ids[k] : k < p.pairs ? fetch(ids + k) : -1; };
 #pragma unroll 1
     for (int j = warp; j < p.pairs; j += kThreads / 32) {
       const int wanted = id_at(j);
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
       bool first = true;
       for (int k0 = 0; k0 < p.pairs && first; k0 += 32) {
         const bool same = id_at(k0 + lane) == wanted;  // an id in the slice is not -1
-        const float value = !same ? 0.f : k0 + lane < kThreads ? first_values[k0 + lane] : __ldg(values + k0 + lane);
+        const float value = !same ? 0.f : k0 + lane < kThreads ? first_values[k0 + lane] : fetch(values + k0 + lane);
         unsigned m = __ballot_sync(0xffffffffu, same);
         if (m && k0 + __ffs(m) - 1 < j) first = false;
         for (; m && first; m &= m - 1) sum += __shfl_sync(0xffffffffu, value, __ffs(m) - 1);
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
       if (wide_bias) {
 #pragma unroll
         for (int e = 0; e < kVec; e += 4) {
-          const float4 b = __ldg(reinterpret_cast<const float4*>(bias + v + e));
+          const float4 b = fetch(reinterpret_cast<const float4*>(bias + v + e));
           x[e] += b.x;
           x[e + 1] += b.y;
           x[e + 2] += b.z;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) x[e] += __ldg(bias + v + e);
+        for (int e = 0; e < kVec; ++e) x[e] += fetch(bias + v + e);
       }
     }
     if (any & kPair) {
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
     float add;
     resolve(w, add);
     x = penalised(x, w);
-    if (bias) x += __ldg(bias + v);
+    if (bias) x += fetch(bias + v);
     if (w & kPair) x += add;
     if (p.mask && !(allowed[(v >> 5) - first_word] >> (v & 31) & 1u)) x = -INFINITY;
     out[v] = from_f32<T>(x);

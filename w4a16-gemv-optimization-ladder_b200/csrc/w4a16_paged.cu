@@ -11,7 +11,7 @@
 //
 // Every kernel here is launched with programmatic stream serialisation: its CTAs may be placed
 // while the kernel before it in the stream ends, and wait for that one before they read or
-// write anything.
+// write anything.  What that kernel may have written is read by the coherent path only.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -29,7 +29,7 @@ namespace {
 // The page that holds position p of sequence s, or -1 (bad sequence, position or entry).
 __device__ __forceinline__ int page_of(const PagedTables& t, int s, int p, int page_shift, int pages) {
   if (s < 0 || s >= t.rows || p < 0 || (p >> page_shift) >= t.width) return -1;
-  const int page = __ldg(t.ids + (size_t)s * t.stride + (p >> page_shift));
+  const int page = fetch(t.ids + (size_t)s * t.stride + (p >> page_shift));
   return page < 0 || page >= pages ? -1 : page;
 }
 
@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
   const int slot = threadIdx.x / kChunks, i = threadIdx.x % kChunks * 8;
   const int keys = a.heads, values = a.heads + pool.kv_heads, all = values + pool.kv_heads;  // heads in the order q, k, v
   for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    const int pos = __ldg(a.positions + t);
-    const int seq = a.seqs ? __ldg(a.seqs + t) : t;
+    const int pos = fetch(a.positions + t);
+    const int seq = a.seqs ? fetch(a.seqs + t) : t;
     const T* q = static_cast<const T*>(a.q) + (size_t)t * a.q_stride + i;
     const T* k = static_cast<const T*>(a.k) + (size_t)t * a.k_stride + i;
     const T* v = static_cast<const T*>(a.v) + (size_t)t * a.v_stride + i;
@@ -77,10 +77,10 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
             const float4* s = reinterpret_cast<const float4*>(a.sin_t + (size_t)pos * D + i);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              cs[e] = __ldg(c + e);
-              cs[2 + e] = __ldg(s + e);
-              cs[4 + e] = __ldg(c + D / 8 + e);
-              cs[6 + e] = __ldg(s + D / 8 + e);
+              cs[e] = fetch(c + e);
+              cs[2 + e] = fetch(s + e);
+              cs[4 + e] = fetch(c + D / 8 + e);
+              cs[6 + e] = fetch(s + D / 8 + e);
             }
           }
         }
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   const long long cap = (long long)tab.width << pool.page_shift;
   // a length past the tables keeps one position there, which has no page: NaN
   auto length = [&](int row) {
-    const int n = __ldg(a.lengths + row);
+    const int n = fetch(a.lengths + row);
     return n <= 0 ? 0 : n > cap ? (int)(cap + 1) : n;
   };
   // An item's units: those of its positions, then cost more that stand for what it takes to begin
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   const int* ids = tab.ids;
   bool seq_ok = false;
   auto enter = [&]() {
-    const int seq = a.seqs ? __ldg(a.seqs + ahead.row) : ahead.row;
+    const int seq = a.seqs ? fetch(a.seqs + ahead.row) : ahead.row;
     seq_ok = seq >= 0 && seq < tab.rows;
     ids = tab.ids + (seq_ok ? (size_t)seq * tab.stride : 0);
     head_off = (size_t)(ahead.item / blocks) * pool.head_stride;
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     ahead_len = ahead.len;
     const int at = pos + (lane & (kPos - 1));
     if (at < ahead.len) {
-      if (seq_ok && (at >> pool.page_shift) < tab.width) page = __ldg(ids + (at >> pool.page_shift));
+      if (seq_ok && (at >> pool.page_shift) < tab.width) page = fetch(ids + (at >> pool.page_shift));
       if (page < 0 || page >= pool.pages) page = -2;
     }
     ++ahead_t;

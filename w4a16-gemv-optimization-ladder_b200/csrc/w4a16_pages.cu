@@ -53,9 +53,9 @@ __device__ __forceinline__ int block_prefix(int v, int* sh, int* total) {
 // own for src's partly filled one.  Request i is refused (ok 0, nothing changed) when its
 // arguments are out of range, when an earlier request names the same seqs[i], or when the
 // free pages do not suffice for all requests up to it.
-__global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st, const int* __restrict__ seqs,
-                                                             const int* __restrict__ src, const int* __restrict__ counts,
-                                                             int n, int* __restrict__ ok, int2* __restrict__ moves) {
+__global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st, const int* seqs,
+                                                             const int* src, const int* counts,
+                                                             int n, int* ok, int2* moves) {
   __shared__ int sh[33], named[kPlanThreads], cum[kPlanThreads], first[kPlanThreads];
   grid_dependency_wait();
   grid_launch_dependents();
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
 }
 
 // Frees sequences: one CTA per request; the first request that names a sequence counts.
-__global__ void __launch_bounds__(256) k_pages_free(const PagesState st, const int* __restrict__ seqs, int n, int* __restrict__ ok) {
+__global__ void __launch_bounds__(256) k_pages_free(const PagesState st, const int* seqs, int n, int* ok) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int i = blockIdx.x;
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(256) k_pages_free(const PagesState st, const i
 // Compaction plan, one CTA: with L live pages, the k-th live page at or above L moves to the
 // k-th free page below it.  Sources and destinations are disjoint, and no page moves that
 // does not have to.
-__global__ void __launch_bounds__(1024) k_compact_plan(const int* refs, int pages, int* refs_out, int* __restrict__ where,
-                                                       int2* __restrict__ moves, int* __restrict__ moved) {
+__global__ void __launch_bounds__(1024) k_compact_plan(const int* refs, int pages, int* refs_out, int* where,
+                                                       int2* moves, int* moved) {
   __shared__ int sh[33];
   grid_dependency_wait();
   grid_launch_dependents();
