@@ -92,6 +92,36 @@ def test_attention_batches(rows, top):
         assert torch.equal(out, K.paged_attention(q, k, v, tables, lengths))
 
 
+@pytest.mark.parametrize("head_dim,rows,top", [(64, 8, 200000), (128, 1500, 60000), (256, 3, 30000)])
+def test_attention_one_long_row_among_short_ones(head_dim, rows, top):
+    # nearly all work in one item, cut into hundreds of parts (by CTAs, by warps; 12 query heads of one
+    # kv head: two blocks of heads with head_dim 256)
+    lens = [top] + [1 + i % 3 for i in range(rows - 1)]
+    k, v, tables, _ = _cache(lens, 1, 64, head_dim, torch.float16, seed=rows)
+    q = torch.randn(rows, 12, head_dim, device=DEV).half()
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = K.paged_attention(q, k, v, tables, lengths)
+    some = [0, 1, 2, rows - 1]
+    _check(out[some], q[some], k, v, tables[some], [lens[i] for i in some])
+    assert torch.equal(out, K.paged_attention(q, k, v, tables, lengths))
+
+
+@pytest.mark.parametrize("rows", [1, 5, 127, 128, 129, 300, 2000])
+def test_attention_padded_batches(rows):
+    # rows of no positions before, between and behind the others, and nothing else
+    g = torch.Generator().manual_seed(rows)
+    lens = [0 if torch.rand((), generator=g) < 0.6 else int(torch.randint(1, 90, (), generator=g)) for _ in range(rows)]
+    lens[-1] = 0
+    k, v, tables, _ = _cache(lens, 2, 8, 64, torch.bfloat16, seed=rows)
+    q = torch.randn(rows, 6, 64, device=DEV).bfloat16()
+    out = K.paged_attention(q, k, v, tables, torch.tensor(lens, dtype=torch.int32, device=DEV))
+    some = torch.randperm(rows, generator=g)[:60].tolist()
+    _check(out[some], q[some], k, v, tables[some], [lens[i] for i in some])
+    empty = torch.tensor([n == 0 for n in lens], device=DEV)
+    assert not out[empty].any()
+    assert not K.paged_attention(q, k, v, tables, torch.zeros(rows, dtype=torch.int32, device=DEV)).any()
+
+
 def test_attention_strides_and_scale():
     lens = [130, 77, 5]
     k, v, tables, _ = _cache(lens, 8, 16, 64, torch.float16, nhd=True)  # [pages, page_size, kv_heads, head_dim] storage
@@ -214,6 +244,19 @@ def test_attention_streams_and_graphs():
         torch.cuda.synchronize()
         for q, out in zip(qs, outs):
             _check(out, q, k, v, tables, change)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+def test_calls_on_another_device_than_the_current_one():
+    dev = torch.device("cuda", 1)
+    k, v, tables, _ = _cache([70, 9], 2, 16, 64, torch.float16)
+    q = torch.randn(2, 4, 64, device=DEV).half()
+    n = torch.tensor([70, 9], dtype=torch.int32, device=DEV)
+    want = K.paged_attention(q, k, v, tables, n)
+    out = K.paged_attention(*(t.to(dev) for t in (q, k, v, tables, n)))
+    assert out.device == dev and torch.equal(out.to(DEV), want)
+    with pytest.raises(RuntimeError):
+        K.paged_attention(q, k.to(dev), v.to(dev), tables, n)
 
 
 # ------------------------------------------------------------------------------------- append
