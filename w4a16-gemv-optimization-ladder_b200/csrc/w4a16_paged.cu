@@ -202,6 +202,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool any) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(any ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -364,6 +367,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows of one copy instruction
   const int crow = lane / kChunks, chunk = lane % kChunks;
   const size_t row_step = (size_t)kRows * pool.token_stride;
+  const bool tight = pool.token_stride == D;  // a page's rows of one head one after the other: constant steps
   const T* k_chunk = static_cast<const T*>(pool.k) + (size_t)crow * pool.token_stride + 8 * chunk;
   const T* v_chunk = static_cast<const T*>(pool.v) + (size_t)crow * pool.token_stride + 8 * chunk;
   unsigned bad = 0;  // bit: the stage holds a position without a page
@@ -374,31 +378,53 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       return;
     }
     bad = (bad & ~(1u << stage)) | (page == -2 ? 1u << stage : 0u);
-    auto copy = [&](int r, size_t at, bool any) {
-      const uint32_t to = dst + r * (D * 2) + ((chunk & ~7) | ((chunk & 7) ^ swizzle(r))) * 16;
-      copy_async16(to, k_chunk + at, any);
-      copy_async16(to + C::kHalf, v_chunk + at, any);
+    const uint32_t here = dst + crow * (D * 2) + (chunk & ~7) * 16;
+    auto to = [&](int r0) {  // where this lane's chunk of row r0 + crow goes (r0 a multiple of kRows)
+      return here + r0 * (D * 2) + (((chunk & 7) ^ swizzle(r0 + crow)) * 16);
     };
     if (pool.page_shift >= 4) {  // the 16 positions of a tile lie in one page
 #pragma unroll
       for (int t = 0; t < kU; ++t) {
-        const int pg = __shfl_sync(0xffffffffu, page, 16 * t);
-        size_t at = (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)((pos + 16 * t) & tmask) * pool.token_stride + head_off;
+        const int pg = __shfl_sync(0xffffffffu, page, 16 * t), p0 = pos + 16 * t;
+        const size_t at = (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)(p0 & tmask) * pool.token_stride + head_off;
+        const T* ks = k_chunk + at;
+        const T* vs = v_chunk + at;
+        if (pg >= 0 && p0 + 16 <= ahead_len) {  // all tiles but a sequence's last
+          if (tight) {
 #pragma unroll
-        for (int i = 0; i < 16 / kRows; ++i) {
-          // positions past the length have no page of their own here, so ask for the position's
-          const int r = 16 * t + i * kRows + crow;
-          copy(r, at, pg >= 0 && pos + r < ahead_len);
-          at += row_step;
+            for (int i = 0; i < 16; i += kRows) {
+              copy_async16(to(16 * t + i), ks + i * D);
+              copy_async16(to(16 * t + i) + C::kHalf, vs + i * D);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += kRows) {
+              copy_async16(to(16 * t + i), ks);
+              copy_async16(to(16 * t + i) + C::kHalf, vs);
+              ks += row_step;
+              vs += row_step;
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 16; i += kRows) {
+            const bool any = pg >= 0 && p0 + i + crow < ahead_len;
+            copy_async16(to(16 * t + i), ks, any);
+            copy_async16(to(16 * t + i) + C::kHalf, vs, any);
+            ks += row_step;
+            vs += row_step;
+          }
         }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kPos / kRows; ++i) {
-        const int r = i * kRows + crow;
+      for (int i = 0; i < kPos; i += kRows) {
+        const int r = i + crow;
         const int pg = __shfl_sync(0xffffffffu, page, r);
-        copy(r, (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)((pos + r) & tmask) * pool.token_stride - (size_t)crow * pool.token_stride +
-                    head_off, pg >= 0);
+        const size_t at = (size_t)(pg < 0 ? 0 : pg) * pool.page_stride + (size_t)((pos + r) & tmask) * pool.token_stride -
+                          (size_t)crow * pool.token_stride + head_off;
+        copy_async16(to(i), k_chunk + at, pg >= 0);
+        copy_async16(to(i) + C::kHalf, v_chunk + at, pg >= 0);
       }
     }
     copies_commit();
