@@ -10,7 +10,10 @@
 // A CTA takes a slice of one row's vocabulary.  Its logits go to registers first, in 16-byte
 // loads; while they are on their way it counts the row's tokens that fall into the slice in
 // shared memory (integer atomics: the result does not depend on their order).  The logits are
-// read and written once; the history is read once for each slice, from L2.
+// read and written once; the history is read once for each slice, from L2.  Bound by bandwidth
+// without tokens (64 rows of 128256: 12 us, 0.85 of the copy rate), else by the chain of loads,
+// counts and barriers that each CTA goes through at 4 CTAs for an SM (with histories of up to
+// 4096, 64 pairs and a mask: 22 us, 0.46).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

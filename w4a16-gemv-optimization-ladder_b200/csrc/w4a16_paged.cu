@@ -37,7 +37,8 @@ __device__ __forceinline__ int page_of(const PagedTables& t, int s, int p, int p
 //
 // Bound by the bytes of q, k and v, read once and written once.  A CTA takes a token at a time;
 // a thread turns 8 pairs (i, i + D/2) of every 16th head with the angles of its pairs in
-// registers, kBatch heads' loads in flight before the token's position and page are known.
+// registers, kBatch heads' loads in flight before the token's position and page are known
+// (16384 tokens of 32 + 16 heads of 128: 65 us, 0.96 of the copy rate).
 template <int D>
 constexpr int append_threads() { return 16 * (D / 16); }
 
@@ -135,23 +136,28 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
 // bank conflicts.  The 8 (NH = 1) or 16 (NH = 2) query heads of a CTA are the n of the products.
 //
 // Work is shared out by a count of units over all (row, kv head, block of query heads) items, in
-// that order: each worker takes an equal run of them, wherever that cuts an item.  With an item for every
-// warp of the grid a worker is a warp and a unit one stage of positions, so the warps run
-// without a barrier; with fewer, which warps would cut into many parts, a worker is a CTA, a
-// unit one stage of each warp, and the CTA joins its warps' parts itself (256 rows of up to 200
-// positions, 2048 items: 34 us by warps, 42 by CTAs; 32 rows of up to 4096, 256 items: 55 and 53).  The lengths are read on the device, so every CTA first sums them up.  An item
-// that lies within one worker is finished there; the parts of one that was cut go to the
-// workspace (slot 2w + 1 if the part begins the item, else 2w) and are joined by k_paged_join.
+// that order: each worker takes an equal run of them, wherever that cuts an item.  With an item
+// for every warp of the grid a worker is a warp and a unit one stage of positions, so the warps
+// run without a barrier; with fewer, which warps would cut into many parts, a worker is a CTA,
+// a unit one stage of each warp, and the CTA joins its warps' parts itself (256 rows of up to
+// 200 positions, 2048 items: 31 us by warps, 36 by CTAs; 32 rows of up to 4096, 256 items: 54
+// and 50).  The lengths are read on the device, so every CTA first sums them up.  An item that
+// lies within one worker is finished there; the parts of one that was cut go to the workspace
+// (slot 2w + 1 if the part begins the item, else 2w) and are joined by k_paged_join.
+//
+// Measured: 72 rows of up to 8191 positions, 8 kv heads of 128: 168 us, 0.98 of the copy rate;
+// 32 rows of up to 4096: 50 us, 0.85, of which about 7 us are the two launches and the way to
+// the first key (lengths, table, page) that a single short row takes as well.
 constexpr int kAttnWarps = 4;
 constexpr int kAttnMaxSms = 148;  // bounds the workspace
 // What it costs to begin and end an item, in units of a warp's and of a CTA's work (256 rows of
-// up to 200 positions: 30 us with it, 34 without; 32 rows of up to 4096: 52 and 53).
+// up to 200 positions: 31 us with it, 36 without; 32 rows of up to 4096: 50 and 52).
 constexpr int kItemCost = 2, kItemCostCta = 1;
 // Workers for each item at most: more cost more to join than they save (one sequence of 30000
-// positions with one kv head: 16.5 us with 64, 20.9 with 32, 17.9 with 128, 28.6 without a bound).
+// positions with one kv head: 16.9 us with 64, 21.9 with 32, 27.9 without a bound).
 constexpr int kMaxParts = 64;
 // CTAs of an SM.  head_dim 64 has more to compute for a byte and wants more warps, with two
-// stages each (64 rows of up to 2048 positions: 31 us with 3 CTAs of 2 stages, 35 with 2 of 3).
+// stages each (64 rows of up to 8000 positions: 86 us with 3 CTAs of 2 stages, 94 with 2 of 3).
 constexpr int attn_per_sm(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
 
 template <int D, int NH>
@@ -686,9 +692,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
 
 // Joins the parts of the item that worker blockIdx.x began.  A thread adds up four dimensions of
 // one head.  Few parts: kJoinFew in a round trip to memory, after the description's.  Many
-// (compiled in for calls of few items: up to kMaxParts parts of a long sequence): groups of threads take every G-th part, in a fixed order, and the maxima and
-// weights come first, so that the long sums are plain multiply-adds of independent loads (one
-// sequence of 8000 positions, 8 kv heads of 64: 12.7 us with the attention, 20 with one group).
+// (compiled in for calls of few items: up to kMaxParts parts of a long sequence): groups of
+// threads take every G-th part, in a fixed order, and the maxima and weights come first, so that
+// the long sums are plain multiply-adds of independent loads (one sequence of 8000 positions, 8
+// kv heads of 64: 13.4 us with the attention, 17.1 by the path for few).
 constexpr int kJoinChunk = 128, kJoinFew = 4;
 template <int D, int NH>
 constexpr int join_lanes() { return 8 * NH * D / 4; }

@@ -225,8 +225,9 @@ struct TableWork {
 // Copies whole pages of every layer, k and v: moves are pairs (src, dst), or two lists.  A pair
 // with an index outside [0, pages) is skipped.  Bound by the bytes, read once and written once:
 // a CTA takes one page of one layer and pool at a time, a thread kFlight 16-byte words in flight.
-// More CTAs than fit at once let the faster SMs take more (2 GB moved: 570 us with 32 for each
-// SM, 640 with 4; a fixed number, since only the device knows how many pages move).
+// More CTAs than fit at once let the faster SMs take more (3.5 GB in all: 570 us, 0.96 of the copy
+// rate, with 32 for each SM, 649 with 4; a fixed number, since only the device knows how many
+// pages move).
 __global__ void __launch_bounds__(256) k_pages_apply(const PageBlocks b, const int2* pairs, const int* src, const int* dst, int n,
                                                      const int* count, const TableWork t) {
   constexpr int kFlight = 8;
