@@ -10,10 +10,17 @@ through w4a16.kernels, on the current stream.
     torch.ops.w4a16.gemv_rmsnorm(packed, scale, h, gamma, eps, group) -> fp32 [rows]
     torch.ops.w4a16.gemv_swiglu(packed, scale, gate_up, group) -> fp32 [rows]
     torch.ops.w4a16.dequant(packed, scale, group) -> fp16 [rows, cols]
+    torch.ops.w4a16.paged_attention(q, k_pages, v_pages, tables, lengths, seqs, scale) -> [rows, heads, head_dim]
+    torch.ops.w4a16.process_logits(logits, tokens, prompt_lens, total_lens, repetition, frequency, presence, bias,
+                                   bias_ids, bias_values, mask) -> like logits
 """
+from typing import Optional
+
 import torch
 
 from . import kernels as K
+from . import logits as _logits
+from . import paged as _paged
 
 
 @torch.library.custom_op("w4a16::gemv", mutates_args=())
@@ -57,3 +64,31 @@ def dequant(packed: torch.Tensor, scale: torch.Tensor, group: int) -> torch.Tens
 @dequant.register_fake
 def _(packed, scale, group):
     return packed.new_empty((packed.shape[0], packed.shape[1] * 2), dtype=torch.float16)
+
+
+@torch.library.custom_op("w4a16::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                    lengths: torch.Tensor, seqs: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    return _paged.paged_attention(q, k_pages, v_pages, tables, lengths, seqs=seqs, scale=scale)
+
+
+@paged_attention.register_fake
+def _(q, k_pages, v_pages, tables, lengths, seqs=None, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("w4a16::process_logits", mutates_args=())
+def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
+                   total_lens: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                   frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                   bias_values: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return _logits.process_logits(logits, tokens=tokens, prompt_lens=prompt_lens, total_lens=total_lens, repetition=repetition,
+                                  frequency=frequency, presence=presence, bias=bias, bias_ids=bias_ids, bias_values=bias_values,
+                                  mask=mask)
+
+
+@process_logits.register_fake
+def _(logits, tokens=None, prompt_lens=None, total_lens=None, repetition=None, frequency=None, presence=None, bias=None,
+      bias_ids=None, bias_values=None, mask=None):
+    return logits.new_empty(logits.shape)

@@ -17,6 +17,10 @@ times and synchronises; the first launch is the warm-up, so a capture takes
     gemm            prefill: 2048 activation rows x 4096 x 4096, group-128 (k_gemm_tc)
     g128_f32        one vector, 65536 x 2048 group-128, fp32 scales    (k_gemv_tma)
     g128_f16        the same with fp16 scales                           (k_gemv_tma)
+    paged_attention 32 rows of up to 4096 positions, 32/8 heads of 128   (k_paged_attention, k_paged_join)
+    paged_append    16384 tokens, 32/8 heads of 128                      (k_paged_append)
+    compact         half of 1200 pages live, 16 layers                   (k_compact_plan, k_pages_apply)
+    logits          64 rows of 128256, 2048 tokens each, mask            (k_process_logits)
 """
 import sys
 
@@ -108,6 +112,52 @@ def case_g128_f32():
 
 def case_g128_f16():
     _g128(torch.float16, 8)
+
+
+def _cache(lengths, seed, layers=1, head_dim=128, spare=0):
+    from .paged import PagedKVCache
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pages = sum(-(-n // 16) for n in lengths)
+    c = PagedKVCache(layers, pages + spare, len(lengths), max(lengths), kv_heads=8, head_dim=head_dim)
+    c.k.normal_(generator=g)
+    c.v.normal_(generator=g)
+    seqs = torch.arange(len(lengths), device="cuda", dtype=torch.int32)
+    c.extend(seqs, torch.tensor(lengths, device="cuda", dtype=torch.int32))
+    return c, seqs
+
+
+def case_paged_attention():
+    c, _ = _cache([128 * (i + 1) for i in range(32)], 9)
+    q = torch.randn(32, 32, 128, device="cuda").half()
+    _three(lambda: c.attention(0, q, c.lengths))
+
+
+def case_paged_append():
+    c, seqs = _cache([1024] * 16, 10)
+    qkv = torch.randn(16384, 48, 128, device="cuda").half()
+    angles = torch.randn(1024, 128, device="cuda")
+    at = torch.arange(1024, device="cuda", dtype=torch.int32).repeat(16)
+    rows = seqs.repeat_interleave(1024)
+    _three(lambda: c.append(0, *qkv.split([32, 8, 8], 1), at, cos=angles, sin=angles, seqs=rows))
+
+
+def case_compact():
+    from .paged import compact_pages
+
+    c, seqs = _cache([32] * 600, 11, layers=16, head_dim=64)
+    c.free(seqs[::2].contiguous())
+    _three(lambda: compact_pages(c.k, c.v, c.tables, c.refs, inplace=False))
+
+
+def case_logits():
+    from .logits import process_logits
+
+    x = torch.randn(64, 128256, device="cuda")
+    tokens = torch.randint(0, 128256, (64, 2048), device="cuda", dtype=torch.int32)
+    mask = torch.randint(-2 ** 31, 2 ** 31, (64, 4008), device="cuda").int()
+    r = torch.full((64,), 1.2, device="cuda")
+    _three(lambda: process_logits(x, tokens=tokens, repetition=r, frequency=r, presence=r, mask=mask))
 
 
 CASES = {n[len("case_"):]: f for n, f in globals().items() if n.startswith("case_")}
