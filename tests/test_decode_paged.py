@@ -51,9 +51,9 @@ def _near(a, b):
     assert (a - b).abs().max().item() <= 2e-2 * b.abs().max().item()
 
 
-@pytest.mark.parametrize("fused", [True, False])
-def test_several_sequences_match_one_at_a_time(fused):
-    dec = _decoder(fused=fused)
+@pytest.mark.parametrize("kw", [dict(fused=True), dict(fused=False), dict(dense=True)], ids=["fused", "unfused", "dense"])
+def test_several_sequences_match_one_at_a_time(kw):
+    dec = _decoder(**kw)
     cache = _cache(dec)
     g = torch.Generator().manual_seed(0)
     texts = {s: torch.randint(0, 4096, (n,), generator=g).tolist() for s, n in ((0, 37), (3, 1), (5, 90))}
