@@ -428,7 +428,8 @@ int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* leng
 /* The bookkeeping of a paged cache, all int32 device memory:
  *   tables  [sequences][width] (stride elements between rows), lengths [sequences],
  *   refs    [pages]: the number of table entries that hold the page, 0 for a free one.
- * Whole pages may be shared between sequences; a partly filled page belongs to one. */
+ * Whole pages may be shared between sequences; a partly filled page belongs to one.
+ * A row's width * page_size is at most 2^30. */
 typedef struct {
   int32_t* tables;
   int32_t* lengths;
@@ -451,8 +452,8 @@ typedef struct {
  * that it needs for them.  fork: sequence dst[i], which must be empty, becomes a copy of
  * src[i]: whole pages are shared, a partly filled last page is copied (in every layer) to the
  * lowest free page.  free: sequence seqs[i] gives up every page in its row and becomes empty
- * (pages whose refs reach 0 are free).  n requests (0..1024; free: 0..65536), served in
- * order; all of them see the state from before the call.  ok[i] (int32) is 1, or 0 for a
+ * (pages whose refs reach 0 are free).  n requests (0..1024, extend: n * width at most 2^30;
+ * free: 0..65536), served in order; all of them see the state from before the call.  ok[i] (int32) is 1, or 0 for a
  * request that was refused and changed nothing: an index out of range, a negative count, more
  * positions than the table row holds, the same seqs / dst index as an earlier request, a dst
  * that is not empty or equals its src, or, from the first request on that no longer fits the free pages, every

@@ -87,6 +87,10 @@ def test_pages(lib):
         assert lib.w4a16_pages_compact(blocks(**change), P, P, 12, P, P, P, P, 1 << 20, None) == status, change
     assert lib.w4a16_pages_extend(state(), P, P, 1025, P, None) == -2 and lib.w4a16_pages_extend(state(), None, P, 1, P, None) == -1
     assert lib.w4a16_pages_extend(state(), None, None, 0, None, None) == 0
+    wide = state(width=1 << 27, table_stride=1 << 27)  # 2^31 positions
+    assert lib.w4a16_pages_extend(wide, P, P, 1, P, None) == -2 and lib.w4a16_pages_fork(wide, blocks(), P, P, 1, P, P, 64, None) == -2
+    many = state(width=1 << 21, table_stride=1 << 21)  # 2^31 pages over 1024 rows
+    assert lib.w4a16_pages_extend(many, P, P, 1024, P, None) == -2
     assert lib.w4a16_pages_free(state(), P, -1, P, None) == -2 and lib.w4a16_pages_free(state(), P + 1, 1, P, None) == -3
     assert lib.w4a16_pages_fork(state(pages=9), blocks(), P, P, 2, P, P, 64, None) == -2
     assert lib.w4a16_pages_fork(state(), blocks(), P, P, 9, P, P, 64, None) == -5

@@ -188,8 +188,9 @@ int check_state(const w4a16_page_state* s, w4a16::PagesState* out) {
     return W4A16_ERR_NULL;
   }
   if (s->sequences <= 0 || s->width <= 0 || s->pages <= 0 || s->page_size <= 0 || s->page_size > 4096 ||
-      (s->page_size & (s->page_size - 1)) != 0 || s->table_stride < s->width) {
-    set_error("bad page state: %d sequences, width %d, stride %lld, %d pages of %d (page_size a power of two up to 4096)",
+      (s->page_size & (s->page_size - 1)) != 0 || s->table_stride < s->width || (long long)s->width * s->page_size > (1 << 30)) {
+    set_error("bad page state: %d sequences, width %d, stride %lld, %d pages of %d (page_size a power of two up to 4096, at "
+              "most 2^30 positions a row)",
               s->sequences, s->width, s->table_stride, s->pages, s->page_size);
     return W4A16_ERR_SHAPE;
   }
@@ -853,6 +854,10 @@ int w4a16_pages_extend(const w4a16_page_state* state, const int32_t* seqs, const
   int rc = check_state(state, &st);
   if (rc == W4A16_OK) rc = check_requests(n, w4a16::kPagesMaxRequests, seqs, counts, ok);
   if (rc != W4A16_OK || n == 0) return rc;
+  if ((long long)n * st.width > (1 << 30)) {  // the pages that the call may ask for are summed in 32 bits
+    set_error("%d requests on rows of %d pages are too many for one call (2^30 pages)", n, st.width);
+    return W4A16_ERR_SHAPE;
+  }
   return w4a16::launch_pages_extend(st, seqs, counts, n, ok, reinterpret_cast<cudaStream_t>(stream));
 }
 
