@@ -69,6 +69,22 @@ def test_several_sequences_match_one_at_a_time(kw):
         _near(out[s], _one_by_one(dec, texts[s]))
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(dense=True)], ids=["int4", "dense"])
+def test_any_number_of_tokens(kw):
+    """None, one, the most that go through the GEMV, and one more, each with as many padding tokens as it
+    takes after one real token: that token's logits are the same within the products' rounding."""
+    dec = _decoder(**kw)
+    want = _one_by_one(dec, [7])
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert dec.step_paged(none.long(), none, none, _cache(dec)).shape == (0, want.shape[-1])
+    for n in (1, 2, 64, 65):
+        cache = _cache(dec)
+        cache.extend(_i32([2]), _i32([1]))
+        got = dec.step_paged(torch.full((n,), 7, device=DEV), _i32([2] * n), _i32([0] + [-1] * (n - 1)), cache)
+        assert got.shape[0] == n
+        _near(got[0], want)
+
+
 def test_fork_free_and_compact_change_no_result():
     dec = _decoder()
     cache, plain = _cache(dec), _cache(dec)

@@ -415,6 +415,8 @@ class W4A16LlamaDecoder:
         cfg, D = self.cfg, self.cfg.head_dim
         if cache.k.dtype != torch.float16 or tuple(cache.k.shape[i] for i in (0, 2, 4)) != (cfg.layers, cfg.kv_heads, D):
             raise ValueError(f"the cache must be fp16 with {cfg.layers} layers, {cfg.kv_heads} kv heads and head_dim {D}")
+        if tokens.numel() == 0:
+            return self.embed.new_empty((0, cfg.vocab), dtype=torch.float32)
         lengths = positions + 1
         h = self.embed.index_select(0, tokens).float()
 
