@@ -92,6 +92,27 @@ def test_attention_batches(rows, top):
         assert torch.equal(out, K.paged_attention(q, k, v, tables, lengths))
 
 
+@pytest.mark.parametrize("rows,kv_heads,heads", [(1, 1, 1), (1, 8, 32), (3, 8, 32), (7, 8, 24), (18, 8, 8), (40, 8, 16), (2, 2, 32), (5, 1, 9)])
+@pytest.mark.parametrize("head_dim,dtype", [(64, torch.float16), (128, torch.bfloat16), (256, torch.float16)])
+def test_attention_of_few_rows_in_tables_of_any_width(rows, kv_heads, heads, head_dim, dtype):
+    # the widths around which a row goes to 1, 2, 4 or 8 CTAs together, or is cut into parts
+    lens = [0 if i % 5 == 3 else (i * 389) % 4097 for i in range(1, rows + 1)]
+    lens[0] = 4096
+    k, v, tables, _ = _cache(lens, kv_heads, 16, head_dim, dtype, seed=rows)
+    q = torch.randn(rows, heads, head_dim, device=DEV).to(dtype)
+    some = [0, rows - 1, rows // 2]
+    for cap in (16, 128, 144, 256, 272, 512, 528, 1024, 1040, 2048, 2064, 4096, 4112):
+        short = [min(n, cap) for n in lens]
+        table = torch.full((rows, cap // 16), -1, dtype=torch.int32, device=DEV)
+        n = min(cap // 16, tables.shape[1])
+        table[:, :n] = tables[:, :n]
+        lengths = torch.tensor(short, dtype=torch.int32, device=DEV)
+        out = K.paged_attention(q, k, v, table, lengths)
+        _check(out[some], q[some], k, v, table[some], [short[i] for i in some])
+        assert not out[lengths == 0].any()
+        assert torch.equal(out, K.paged_attention(q, k, v, table, lengths))
+
+
 @pytest.mark.parametrize("head_dim,rows,top", [(64, 8, 200000), (128, 1500, 60000), (256, 3, 30000)])
 def test_attention_one_long_row_among_short_ones(head_dim, rows, top):
     # nearly all work in one item, cut into hundreds of parts (by CTAs, by warps; 12 query heads of one

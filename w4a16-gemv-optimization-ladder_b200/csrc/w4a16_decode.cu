@@ -49,19 +49,6 @@ __device__ __forceinline__ void rope_pair(float& a, float& b, const float* cos_r
   b = rb;
 }
 
-// Thread-block cluster helpers (the CL variant of k_decode_attention: one cluster per kv head).
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// A float of CTA `rank`'s shared memory at the offset of `local` in this CTA's.
-__device__ __forceinline__ float ld_cluster_f32(const float* local, unsigned rank) {
-  uint32_t a = (uint32_t)__cvta_generic_to_shared(local), ra;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ra) : "memory");
-  return v;
-}
-
 // CL: the kv head's splits form one thread-block cluster; each CTA leaves its partial
 // softmaxes in its own shared memory and split 0 combines them through distributed shared
 // memory between two cluster barriers (no global round trips, fence or counter).

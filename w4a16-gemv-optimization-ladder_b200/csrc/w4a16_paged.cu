@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
 // 200 positions, 2048 items: 31 us by warps, 36 by CTAs; 32 rows of up to 4096, 256 items: 54
 // and 50).  The lengths are read on the device, so every CTA first sums them up.  An item that
 // lies within one worker is finished there; the parts of one that was cut go to the workspace
-// (slot 2w + 1 if the part begins the item, else 2w) and are joined by k_paged_join.
+// (slot 2w + 1 if the part begins the item, else 2w) and are joined by k_paged_join.  Calls of few
+// rows go another way (kClusterMax).
 //
 // Measured: 72 rows of up to 8191 positions, 8 kv heads of 128: 168 us, 0.98 of the copy rate;
 // 32 rows of up to 4096: 50 us, 0.85, of which about 7 us are the two launches and the way to
@@ -156,6 +157,14 @@ constexpr int kItemCost = 2, kItemCostCta = 1;
 // Workers for each item at most: more cost more to join than they save (one sequence of 30000
 // positions with one kv head: 16.9 us with 64, 21.9 with 32, 27.9 without a bound).
 constexpr int kMaxParts = 64;
+// Calls of few rows in short tables: a cluster of CTAs takes one item (the kernel's kCluster form),
+// each warp every (4 * cluster)-th stage of it, and joins its warps' parts through distributed shared
+// memory, without a look at the other rows, parts in the workspace or a second launch.  A cluster
+// has up to 8 CTAs: as many as the device runs at once, and as have 128 positions of a full table
+// row each.  Past 512 positions for each the equal shares of all SMs win.  (32 query heads over 8
+// kv heads.  head_dim 64: 1 row of 512 positions 4.2 us, cut into parts 6.9; of 4096 7.6 and 9.9;
+// of 16384 22.6 and 15.6.  head_dim 128: 8 rows of 512 7.2 and 9.7; 16 rows of 64 4.2 and 8.3.)
+constexpr int kClusterMax = 8, kClusterLeast = 128, kClusterMost = 512;
 // CTAs of an SM.  head_dim 64 has more to compute for a byte and wants more warps, with two
 // stages each (64 rows of up to 8000 positions: 86 us with 3 CTAs of 2 stages, 94 with 2 of 3).
 constexpr int attn_per_sm(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
@@ -225,16 +234,19 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
   return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
 }
 
-template <typename T, int D, int NH>
+template <typename T, int D, int NH, bool kCluster>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     k_paged_attention(const PagedAttention a, const PagedPool pool, const PagedTables tab, const int group, const int blocks,
-                      const bool coop, const int cost) {
+                      const bool coop, const int cost, const int cluster) {
   using C = AttnCfg<D, NH>;
   constexpr int kB = D / 32, kVB = D / 64, kU = C::kTiles, kHeads = C::kHeads, kThreads = kAttnWarps * 32, kPos = C::kPos;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  const int rank = blockIdx.x & (cluster - 1);
   const int workers = coop ? gridDim.x : gridDim.x * kAttnWarps;
   const int worker = coop ? blockIdx.x : blockIdx.x * kAttnWarps + warp;
-  const int unit = coop ? kPos * kAttnWarps : kPos, shift = coop ? warp * kPos : 0;  // this warp's stage of a unit
+  // positions of a unit, and where this warp's stage of them lies
+  const int unit = kCluster ? kPos * kAttnWarps * cluster : coop ? kPos * kAttnWarps : kPos;
+  const int shift = kCluster ? (rank * kAttnWarps + warp) * kPos : coop ? warp * kPos : 0;
   const int items = pool.kv_heads * blocks;
   const float nan = __int_as_float(0x7fc00000);
   __shared__ long long sh_base[kAttnWarps], sh_warp[kAttnWarps];
@@ -258,69 +270,93 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   // and end one
   auto tiles = [&](int len) { return len == 0 ? 0 : (len + unit - 1) / unit + cost; };
 
-  // the units of all rows, and the row that holds each worker's first one
-  const int per = (a.rows + kThreads - 1) / kThreads;
-  const int r0 = min(a.rows, (int)threadIdx.x * per), r1 = min(a.rows, r0 + per);
-  long long sum = 0;
-  for (int r = r0; r < r1; ++r) sum += tiles(length(r));
-  sum *= items;
-  long long inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long n = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += n;
-  }
-  if (lane == 31) sh_warp[warp] = inc;
-  __syncthreads();
-  long long before = inc - sum, total = 0;
-  for (int w = 0; w < kAttnWarps; ++w) {
-    if (w < warp) before += sh_warp[w];
-    total += sh_warp[w];
-  }
-  // every worker in use has a unit, so the parts of an item lie with consecutive workers: the
-  // first `more` of them take each + 1 units, the others each
-  const long long most = min((long long)workers, (long long)a.rows * items * kMaxParts);
-  const int used = (int)min(total, most);
-  const long long each = used ? divide(total, used) : 0;
-  const int more = (int)(total - each * used);
-  auto first_unit = [&](int w) { return w < used ? w * each + min(w, more) : total; };
-  for (int w = 0; w < (coop ? 1 : kAttnWarps); ++w) {
-    const long long u = first_unit(coop ? blockIdx.x : blockIdx.x * kAttnWarps + w);
-    if (u < total && before <= u && u < before + sum) {  // one thread
-      long long base = before;
-      int r = r0;
-      for (;; ++r) {
-        const long long n = (long long)tiles(length(r)) * items;
-        if (u < base + n) break;
-        base += n;
-      }
-      sh_row[w] = r;
-      sh_base[w] = base;
-    }
-  }
-  if (coop ? threadIdx.x == 0 : lane == 0) desc[worker].parts = 0;
-  // rows of no positions are zero
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x)
-    if (length(r) == 0)
-      for (int e = threadIdx.x; e < a.heads * D / 8; e += kThreads)
-        reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)r * a.out_stride)[e] = make_uint4(0u, 0u, 0u, 0u);
-  __syncthreads();
-  const long long u0 = first_unit(worker), u1 = worker + 1 < used ? first_unit(worker + 1) : total;
-  if (u0 >= u1) return;  // the whole CTA if it works as one
-  const float scale = a.scale * 1.4426950408889634f;  // probabilities as powers of two
-
   // A span: the tiles [t0, t1) of one item that the worker takes in a row.
   struct Span {
     int row, len, nt, item, t0, t1;
   };
   Span cur;
-  long long base = sh_base[coop ? 0 : warp];  // units before the row of cur
-  cur.row = sh_row[coop ? 0 : warp];
-  cur.len = length(cur.row);
-  cur.nt = tiles(cur.len);
-  cur.item = (int)divide(u0 - base, cur.nt);
-  cur.t0 = (int)(u0 - base - (long long)cur.item * cur.nt);
-  cur.t1 = (int)min((long long)cur.nt, cur.t0 + (u1 - u0));
+  long long u0, u1, each = 0;  // this worker's units; units of a worker
+  int more = 0, first_page = -2;
+  if constexpr (kCluster) {  // one item
+    const int at = blockIdx.x / cluster;
+    cur.row = at / items;
+    cur.item = at - cur.row * items;
+    // the sequence's first pages are looked up while its length is on its way
+    const int seq = a.seqs ? fetch(a.seqs + cur.row) : cur.row, col = (shift + (lane & (kPos - 1))) >> pool.page_shift;
+    cur.len = length(cur.row);
+    if (seq >= 0 && seq < tab.rows && col < tab.width) first_page = fetch(tab.ids + (size_t)seq * tab.stride + col);
+    cur.nt = tiles(cur.len);
+    cur.t0 = 0;
+    cur.t1 = cur.nt;
+    u0 = 0;
+    u1 = cur.nt;
+    if (cur.len == 0) {  // a row of no positions is zero
+      const int h0 = cur.item / blocks * group + cur.item % blocks * kHeads, n = min(kHeads, group - cur.item % blocks * kHeads) * D / 8;
+      for (int e = rank * kThreads + threadIdx.x; e < n; e += kThreads * cluster)
+        reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)cur.row * a.out_stride + (size_t)h0 * D)[e] = make_uint4(0u, 0u, 0u, 0u);
+      return;  // the whole cluster
+    }
+  } else {
+    // the units of all rows, and the row that holds each worker's first one
+    const int per = (a.rows + kThreads - 1) / kThreads;
+    const int r0 = min(a.rows, (int)threadIdx.x * per), r1 = min(a.rows, r0 + per);
+    long long sum = 0;
+    for (int r = r0; r < r1; ++r) sum += tiles(length(r));
+    sum *= items;
+    long long inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long n = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += n;
+    }
+    if (lane == 31) sh_warp[warp] = inc;
+    __syncthreads();
+    long long before = inc - sum, total = 0;
+    for (int w = 0; w < kAttnWarps; ++w) {
+      if (w < warp) before += sh_warp[w];
+      total += sh_warp[w];
+    }
+    // every worker in use has a unit, so the parts of an item lie with consecutive workers: the
+    // first `more` of them take each + 1 units, the others each
+    const long long most = min((long long)workers, (long long)a.rows * items * kMaxParts);
+    const int used = (int)min(total, most);
+    each = used ? divide(total, used) : 0;
+    more = (int)(total - each * used);
+    auto first_unit = [&](int w) { return w < used ? w * each + min(w, more) : total; };
+    for (int w = 0; w < (coop ? 1 : kAttnWarps); ++w) {
+      const long long u = first_unit(coop ? blockIdx.x : blockIdx.x * kAttnWarps + w);
+      if (u < total && before <= u && u < before + sum) {  // one thread
+        long long base = before;
+        int r = r0;
+        for (;; ++r) {
+          const long long n = (long long)tiles(length(r)) * items;
+          if (u < base + n) break;
+          base += n;
+        }
+        sh_row[w] = r;
+        sh_base[w] = base;
+      }
+    }
+    if (coop ? threadIdx.x == 0 : lane == 0) desc[worker].parts = 0;
+    // rows of no positions are zero
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x)
+      if (length(r) == 0)
+        for (int e = threadIdx.x; e < a.heads * D / 8; e += kThreads)
+          reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)r * a.out_stride)[e] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+    u0 = first_unit(worker);
+    u1 = worker + 1 < used ? first_unit(worker + 1) : total;
+    if (u0 >= u1) return;  // the whole CTA if it works as one
+    const long long base = sh_base[coop ? 0 : warp];  // units before the row of cur
+    cur.row = sh_row[coop ? 0 : warp];
+    cur.len = length(cur.row);
+    cur.nt = tiles(cur.len);
+    cur.item = (int)divide(u0 - base, cur.nt);
+    cur.t0 = (int)(u0 - base - (long long)cur.item * cur.nt);
+    cur.t1 = (int)min((long long)cur.nt, cur.t0 + (u1 - u0));
+  }
+  const float scale = a.scale * 1.4426950408889634f;  // probabilities as powers of two
+
   auto next_span = [&](Span& sp, long long u) {  // the span that begins at unit u < u1, where sp ends
     sp.t0 = 0;
     if (++sp.item == items) {
@@ -364,7 +400,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     ahead_len = ahead.len;
     const int at = pos + (lane & (kPos - 1));
     if (at < ahead.len) {
-      if (seq_ok && (at >> pool.page_shift) < tab.width) page = fetch(ids + (at >> pool.page_shift));
+      if (kCluster && ahead_t == 0)
+        page = first_page;
+      else if (seq_ok && (at >> pool.page_shift) < tab.width)
+        page = fetch(ids + (at >> pool.page_shift));
       if (page < 0 || page >= pool.pages) page = -2;
     }
     ++ahead_t;
@@ -595,6 +634,78 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     for (int n = 0; n < NH; ++n) {  // from here on maxima of the scaled scores, as powers of two
       m[n][0] *= scale;
       m[n][1] *= scale;
+    }
+    if constexpr (kCluster) {
+      // the warps' parts (o, m, l), each where its warp's ring was, joined by the cluster
+      auto part = [&](int w) { return reinterpret_cast<const float*>(sh_raw + w * C::kRing); };
+      float* mine = reinterpret_cast<float*>(sh_raw + warp * C::kRing);
+      copies_wait<0>();
+      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int head = 8 * n + 2 * j + c;
+          if (g == 0) {
+            mine[kHeads * D + head] = m[n][c];
+            mine[kHeads * (D + 1) + head] = l[n][c];
+          }
+#pragma unroll
+          for (int b = 0; b < kVB; ++b) {
+            float4* dst = reinterpret_cast<float4*>(mine + head * D + 64 * b + 8 * g);
+            dst[0] = make_float4(o[n][4 * b][c], o[n][4 * b][2 + c], o[n][4 * b + 1][c], o[n][4 * b + 1][2 + c]);
+            dst[1] = make_float4(o[n][4 * b + 2][c], o[n][4 * b + 2][2 + c], o[n][4 * b + 3][c], o[n][4 * b + 3][2 + c]);
+          }
+        }
+      __syncwarp();
+      cluster_sync_all();
+      // an equal share of the heads' dimensions for each CTA: `cluster` neighbouring threads add up
+      // four of them, each its CTA's warps
+      const int all = nheads * (D / 4);
+#pragma unroll 1
+      for (int e0 = warp * 32; e0 < all; e0 += kThreads) {
+        const int e = min(e0 + lane, all - 1), c = e & (cluster - 1), at = (rank * all + e) / cluster, h = at / (D / 4), d = at % (D / 4) * 4;
+        float top = -INFINITY, ms[kAttnWarps], ls[kAttnWarps], ll = 0.f;
+        float4 x[kAttnWarps], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+          ms[w] = ld_cluster_f32(part(w) + kHeads * D + h, c);
+          ls[w] = ld_cluster_f32(part(w) + kHeads * (D + 1) + h, c);
+          x[w] = ld_cluster_f32x4(part(w) + h * D + d, c);
+          top = fmaxf(top, ms[w]);
+        }
+#pragma unroll
+        for (int o = 1; o < kClusterMax; o <<= 1)
+          if (o < cluster) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float low = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+          const float f = exp2_fast(ms[w] - low);
+          ll = fmaf(ls[w], f, ll);
+          acc.x = fmaf(x[w].x, f, acc.x);
+          acc.y = fmaf(x[w].y, f, acc.y);
+          acc.z = fmaf(x[w].z, f, acc.z);
+          acc.w = fmaf(x[w].w, f, acc.w);
+        }
+#pragma unroll
+        for (int o = 1; o < kClusterMax; o <<= 1)
+          if (o < cluster) {
+            ll += __shfl_xor_sync(0xffffffffu, ll, o);
+            acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+            acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+            acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+            acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+          }
+        if (c == 0 && e == e0 + lane) {
+          uint2 r;
+          r.x = pack2<T>(acc.x / ll, acc.y / ll);
+          r.y = pack2<T>(acc.z / ll, acc.w / ll);
+          *reinterpret_cast<uint2*>(out + h * D + d) = r;
+        }
+      }
+      __syncwarp();
+      cluster_sync_all();  // no CTA leaves while another reads its memory
+      return;
     }
     if (!coop) {
 #pragma unroll
@@ -865,6 +976,41 @@ namespace {
 bool attn_wide(int group, int head_dim) { return group > 8 && head_dim <= 128; }
 
 template <typename T, int D, int NH>
+struct ClusterLaunch {  // n clusters, with programmatic stream serialisation
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attrs[2];
+  ClusterLaunch(unsigned n, int cluster, cudaStream_t stream) {
+    cfg.gridDim = dim3(n * cluster);
+    cfg.blockDim = dim3(kAttnWarps * 32);
+    cfg.dynamicSmemBytes = kAttnWarps * AttnCfg<D, NH>::kRing;
+    cfg.stream = stream;
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = cluster;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
+  }
+};
+
+// How many clusters of this size the device runs at once (asked once for each device and size).
+template <typename T, int D, int NH>
+int resident_clusters(int dev, int cluster) {
+  static std::atomic<int> known[64][kClusterMax + 1];  // that number and 1; 0: not asked yet
+  std::atomic<int>& mine = known[dev & 63][cluster];
+  int n = mine.load(std::memory_order_acquire);
+  if (n == 0 || dev >= 64) {
+    ClusterLaunch<T, D, NH> l(1, cluster, nullptr);
+    l.cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, k_paged_attention<T, D, NH, true>, &l.cfg) != cudaSuccess) n = 0;
+    (void)cudaGetLastError();
+    mine.store(++n, std::memory_order_release);
+  }
+  return n - 1;
+}
+
+template <typename T, int D, int NH>
 int launch_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream) {
   using C = AttnCfg<D, NH>;
   int sms = 0;
@@ -880,12 +1026,22 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(configured.load(std::memory_order_acquire) >> (dev & 63) & 1ull)) {
-    e = cudaFuncSetAttribute(k_paged_attention<T, D, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    e = cudaFuncSetAttribute(k_paged_attention<T, D, NH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_paged_attention<T, D, NH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnWarps * C::kRing);
     if (e == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev, std::memory_order_acq_rel);
   }
   if (e != cudaSuccess) return launched("configuring k_paged_attention,", e);
-  const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
-                                                                 stream, true, a, pool, tab, group, blocks, coop, cost));
+  const long long all = (long long)a.rows * pool.kv_heads * blocks;
+  const long long cap = (long long)tab.width << pool.page_shift;
+  int cluster = kClusterMax;
+  while (cluster > 1 && (cap <= (long long)cluster / 2 * kClusterLeast || all > resident_clusters<T, D, NH>(dev, cluster))) cluster /= 2;
+  if (all * cluster <= ctas && cap <= (long long)cluster * kClusterMost) {
+    ClusterLaunch<T, D, NH> l((unsigned)all, cluster, stream);
+    return launched("k_paged_attention", cudaLaunchKernelEx(&l.cfg, k_paged_attention<T, D, NH, true>, a, pool, tab, group, blocks, true, 0, cluster));
+  }
+  const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH, false>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
+                                                                 stream, true, a, pool, tab, group, blocks, coop, cost, 1));
   if (rc2 != W4A16_OK) return rc2;
   // Items few enough to be cut into many parts get groups of threads that share them; the rest the
   // kernel without shared memory, whose CTAs do not keep the next attention's off the SMs.
