@@ -148,6 +148,23 @@ def test_strides_and_single_rows():
     assert one.shape == (4099,) and torch.equal(one, (big[0].float() + 1).half())
 
 
+@pytest.mark.parametrize("rows,pairs", [(2, 255), (2, 256), (2, 513), (80, 257), (80, 1500), (2, 5000)])
+def test_many_pairs(rows, pairs):
+    # more than one round of pairs for a slice of the vocabulary (by 80 rows: of the larger slices); ids
+    # named again in the same round and in later ones, one of them by a third of the pairs
+    logits, kw = _inputs(rows, 16001, 200, torch.float32, pairs=pairs)
+    n = pairs // 3
+    kw["bias_ids"][:, n:2 * n] = kw["bias_ids"][:, :n].flip(1)
+    kw["bias_ids"][:, 2 * n::2] = 77
+    out = K.process_logits(logits, **kw)
+    some = [0, rows - 1]
+    part = {name: (t if name == "bias" else t[some]) for name, t in kw.items()}
+    # a rounding for each value of an id
+    _check(out[some], logits[some], extra=8 + max(int(torch.bincount(r[r >= 0]).max()) for r in part["bias_ids"]), **part)
+    assert torch.equal(K.process_logits(logits, **kw), out)
+    assert torch.equal(K.process_logits(logits, **kw, out=logits), out)
+
+
 def test_same_bits_every_time_and_in_a_graph():
     logits, kw = _inputs(9, 60001, 3000, torch.float32, pairs=300)
     kw["bias_ids"][:, 100:200] = kw["bias_ids"][:, :100]  # every id twice

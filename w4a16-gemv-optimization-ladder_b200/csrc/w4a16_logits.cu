@@ -13,7 +13,7 @@
 // read and written once; the history is read once for each slice, from L2.  Bound by bandwidth
 // without tokens (64 rows of 128256: 12 us, 0.85 of the copy rate), else by the chain of loads,
 // counts and barriers that each CTA goes through at 4 CTAs for an SM (with histories of up to
-// 4096, 64 pairs and a mask: 22 us, 0.46).
+// 4096, 64 pairs and a mask: 20 us, 0.51).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -27,7 +27,12 @@ namespace w4a16 {
 
 namespace {
 
-constexpr uint32_t kSeen = 0x80000000u, kPair = 0x40000000u, kCount = 0x3fffffffu;
+constexpr uint32_t kSeen = 0x80000000u, kCount = 0x7fffffffu;
+
+struct Pair {  // a token with bias pairs: the sum of its values, its logit
+  int token;
+  float sum, logit;
+};
 
 // kLoads: 16-byte pieces of the slice a thread holds.
 template <typename T, int kThreads, int kLoads>
@@ -40,14 +45,16 @@ template <typename T, int kThreads, int kLoads>
 __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_logits(const LogitsProblem p, const int slices) {
   using C = LogitsCfg<T, kThreads, kLoads>;
   constexpr int kVec = C::kVec, kSlice = C::kSlice;
-  // word[token of the slice]: seen in the prompt | occurrences after it; or, for a token with bias
-  // pairs: has pairs | its place in paired (its word, the sum of its values)
+  // word[token of the slice]: seen in the prompt | occurrences after it
   extern __shared__ __align__(16) uint32_t word[];
-  uint2* paired = reinterpret_cast<uint2*>(word + kSlice);
+  // places[token of the slice]: of more than one round of pairs, 1 + the place in paired
+  const bool rounds = p.pairs > kThreads;
+  uint32_t* places = word + kSlice;
+  Pair* paired = reinterpret_cast<Pair*>(rounds ? places + kSlice : places);
   __shared__ uint32_t allowed[C::kWords], pairs_here;
-  __shared__ int first_ids[kThreads];  // the row's first pairs
-  __shared__ float first_values[kThreads];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ __align__(16) int ids_here[kThreads];  // a round of the row's pairs
+  __shared__ float values_here[kThreads];
+  const int tid = threadIdx.x;
   grid_dependency_wait();
   grid_launch_dependents();
   const int row = blockIdx.x / slices;
@@ -90,10 +97,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
   }
   const int* ids = p.bias_ids + (size_t)row * p.pairs;
   const float* values = p.bias_values + (size_t)row * p.pairs;
-  if (p.pairs) {
-    first_ids[tid] = tid < p.pairs ? fetch(ids + tid) : -1;
-    first_values[tid] = tid < p.pairs ? fetch(values + tid) : 0.f;
-  }
+  auto pair_at = [&](int k) {
+    ids_here[tid] = k < p.pairs ? fetch(ids + k) : -1;
+    values_here[tid] = k < p.pairs ? fetch(values + k) : 0.f;
+  };
+  if (p.pairs) pair_at(tid);
   const int first_word = lo >> 5;
   if (p.mask)
     for (int i = tid; i <= ((v1 - 1) >> 5) - first_word; i += kThreads)
@@ -108,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
   }
   const bool marks = p.tokens || p.pairs;
   if (marks) {
-    for (int i = tid; i < kSlice / 4; i += kThreads) reinterpret_cast<uint4*>(word)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < (rounds ? kSlice / 2 : kSlice / 4); i += kThreads) reinterpret_cast<uint4*>(word)[i] = make_uint4(0u, 0u, 0u, 0u);
     if (tid == 0) pairs_here = 0u;
     __syncthreads();
     auto count = [&](int t, int j) {
@@ -133,39 +141,50 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
     }
 #pragma unroll 4
     for (int j = done + tid; j < total; j += kThreads) count(token_at(j), j);
-    // the first pair of an id adds up all of the id's values, in the pairs' order: a warp for
-    // each pair that falls into the slice
-    if (p.pairs) __syncthreads();  // the counts are final
-    auto id_at = [&](int k) { return k < kThreads ? first_ids[k] : k < p.pairs ? fetch(ids + k) : -1; };
+    // A thread for each pair, kThreads of them in a round: the first of an id in the round adds up all
+    // of the id's values there, in the pairs' order (nearly always its own).  The token is written
+    // once more at the end, so that the others' way is free of it (64 rows with 64 pairs, histories and
+    // a mask: 20.7 us; 22.5 with the pairs' places looked up by every token and a warp for each pair).
 #pragma unroll 1
-    for (int j = warp; j < p.pairs; j += kThreads / 32) {
-      const int wanted = id_at(j);
-      if (wanted < lo || wanted >= v1) continue;
-      float sum = 0.f;
-      bool first = true;
-      for (int k0 = 0; k0 < p.pairs && first; k0 += 32) {
-        const bool same = id_at(k0 + lane) == wanted;  // an id in the slice is not -1
-        const float value = !same ? 0.f : k0 + lane < kThreads ? first_values[k0 + lane] : fetch(values + k0 + lane);
-        unsigned m = __ballot_sync(0xffffffffu, same);
-        if (m && k0 + __ffs(m) - 1 < j) first = false;
-        for (; m && first; m &= m - 1) sum += __shfl_sync(0xffffffffu, value, __ffs(m) - 1);
+    for (int k0 = 0; k0 < p.pairs; k0 += kThreads) {
+      if (k0) {
+        __syncthreads();
+        pair_at(k0 + tid);
+        __syncthreads();
       }
-      if (first && lane == 0) {
+      const int wanted = ids_here[tid];
+      if (wanted < lo || wanted >= v1) continue;
+      int same = 0;
+      const int end = min(p.pairs - k0, kThreads);
+#pragma unroll 4
+      for (int k = 0; k < end; k += 4) {  // an id in the slice is not -1
+        const int4 x = *reinterpret_cast<const int4*>(ids_here + k);
+        same += (x.x == wanted) + (x.y == wanted) + (x.z == wanted) + (x.w == wanted);
+      }
+      int k = tid;
+      if (same > 1) {
+        k = 0;
+        while (ids_here[k] != wanted) ++k;
+        if (k < tid) continue;
+      }
+      const int at = rounds ? (int)places[wanted - v0] - 1 : -1;
+      float sum = at < 0 ? 0.f : paired[at].sum;
+      for (; same; ++k)
+        if (ids_here[k] == wanted) {
+          sum += values_here[k];
+          --same;
+        }
+      if (at >= 0) {
+        paired[at].sum = sum;
+      } else {
         const uint32_t i = atomicAdd(&pairs_here, 1u);
-        paired[i] = make_uint2(word[wanted - v0], __float_as_uint(sum));
-        word[wanted - v0] = kPair | i;
+        paired[i] = Pair{wanted, sum, to_f32<T>(in[wanted])};
+        if (rounds) places[wanted - v0] = i + 1;
       }
     }
   }
   if (marks || p.mask) __syncthreads();
   const float* bias = p.bias ? p.bias + (size_t)row * p.bias_stride : nullptr;
-  auto resolve = [&](uint32_t& w, float& add) {  // a token with pairs: its own word, and what they add
-    if (w & kPair) {
-      const uint2 it = paired[w & kCount];
-      w = kPair | it.x;
-      add = __uint_as_float(it.y);
-    }
-  };
   auto penalised = [&](float x, uint32_t w) {
     const float by = x > 0.f ? inv_rep : rep, n = (float)(w & kCount);
     x = w & (kSeen | kCount) ? x * by : x;
@@ -180,16 +199,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
 #pragma unroll
     for (int e = 0; e < kVec; ++e) x[e] = to_f32<T>(piece[c].one[e]);
     uint32_t w[kVec], any = 0;
-    float add[kVec];
     if (marks) {
 #pragma unroll
       for (int e = 0; e < kVec; e += 4) *reinterpret_cast<uint4*>(w + e) = *reinterpret_cast<const uint4*>(word + at + e);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) any |= w[e];
-      if (any & kPair) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) resolve(w[e], add[e]);
-      }
       if (any) {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) x[e] = penalised(x[e], w[e]);
@@ -210,11 +224,6 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
         for (int e = 0; e < kVec; ++e) x[e] += fetch(bias + v + e);
       }
     }
-    if (any & kPair) {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        if (w[e] & kPair) x[e] += add[e];
-    }
     if (p.mask) {  // the piece's bits lie in one word or in two neighbours
       const int i = (v >> 5) - first_word;
       const uint32_t bits = __funnelshift_r(allowed[i], allowed[((v + kVec - 1) >> 5) - first_word], v & 31);
@@ -231,22 +240,22 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
       for (int e = 0; e < kVec; ++e) out_mine[c * kThreads * kVec + e] = piece[c].one[e];
     }
   }
-  // the ends of the row that are no whole piece: under 2 kVec tokens
-  auto one = [&](int v) {
-    const int at = v - v0;
-    float x = to_f32<T>(in[v]);
-    uint32_t w = marks ? word[at] : 0u;
-    float add;
-    resolve(w, add);
-    x = penalised(x, w);
+  auto one = [&](int v, float x, float sum) {
+    x = penalised(x, marks ? word[v - v0] : 0u);
     if (bias) x += fetch(bias + v);
-    if (w & kPair) x += add;
+    x += sum;
     if (p.mask && !(allowed[(v >> 5) - first_word] >> (v & 31) & 1u)) x = -INFINITY;
     out[v] = from_f32<T>(x);
   };
-  if (v0 < 0 && tid < min(v0 + kVec, p.vocab)) one(tid);  // the piece around the row's start
+  // the ends of the row that are no whole piece: under 2 kVec tokens
+  auto end = [&](int v) { one(v, to_f32<T>(in[v]), -0.f); };  // x + -0 is x, of either zero
+  if (v0 < 0 && tid < min(v0 + kVec, p.vocab)) end(tid);  // the piece around the row's start
   const int tail = v1 - (v1 - v0) % kVec;                 // the piece around its end
-  if (tail >= max(v0, 0) && tail + tid < v1) one(tail + tid);
+  if (tail >= max(v0, 0) && tail + tid < v1) end(tail + tid);
+  if (p.pairs) {
+    __syncthreads();  // the plain values are written
+    for (int i = tid; i < (int)pairs_here; i += kThreads) one(paired[i].token, paired[i].logit, paired[i].sum);
+  }
 }
 
 template <typename T, int kThreads, int kLoads>
@@ -258,14 +267,15 @@ int launch_loads(const LogitsProblem& p, cudaStream_t stream) {
     set_error("%d rows of %d logits are too many for one call", p.rows, p.vocab);
     return W4A16_ERR_SHAPE;
   }
-  const size_t smem = p.pairs || p.tokens ? (size_t)C::kSlice * 4 + (size_t)(p.pairs < C::kSlice ? p.pairs : C::kSlice) * 8 : 0;
+  const size_t smem = p.pairs || p.tokens ? (size_t)C::kSlice * (p.pairs > kThreads ? 8 : 4) +
+                                                (size_t)(p.pairs < C::kSlice ? p.pairs : C::kSlice) * sizeof(Pair) : 0;
   cudaError_t e = cudaSuccess;
   if (smem > 40960) {
     static std::atomic<uint64_t> configured{0};  // one bit per device
     int dev = 0;
     e = cudaGetDevice(&dev);
     if (e == cudaSuccess && !(configured.load(std::memory_order_acquire) >> (dev & 63) & 1ull)) {
-      e = cudaFuncSetAttribute(k_process_logits<T, kThreads, kLoads>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSlice * 12);
+      e = cudaFuncSetAttribute(k_process_logits<T, kThreads, kLoads>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSlice * (8 + sizeof(Pair)));
       if (e == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev, std::memory_order_acq_rel);
     }
   }
@@ -285,7 +295,7 @@ int launch_type(const LogitsProblem& p, cudaStream_t stream) {
   const int rc = current_sm_count(&sms);
   if (rc != W4A16_OK) return rc;
   // Slices of 8192 tokens, whose history is read fewer times; of 2048 where those would leave SMs
-  // without one (1 row of 128256: 2.6 us by slices of 2048, 4.2 by 8192; 64 rows: 54 and 22.5).
+  // without one (1 row of 128256: 2.6 us by slices of 2048, 4.2 by 8192; 64 rows: 54 and 20).
   constexpr int kSize = sizeof(T);
   const long long blocks = ((long long)p.vocab + 8191) / 8192 * p.rows;
   return blocks < sms ? launch_loads<T, 128 * kSize, 1>(p, stream) : launch_loads<T, 256, kSize * 2>(p, stream);
