@@ -155,16 +155,21 @@ constexpr int kAttnMaxSms = 148;  // bounds the workspace
 // up to 200 positions: 31 us with it, 36 without; 32 rows of up to 4096: 50 and 52).
 constexpr int kItemCost = 2, kItemCostCta = 1;
 // Workers for each item at most: more cost more to join than they save (one sequence of 30000
-// positions with one kv head: 16.9 us with 64, 21.9 with 32, 27.9 without a bound).
-constexpr int kMaxParts = 64;
+// positions with one kv head of 64: 9.4 us with 128, 10.6 with 64 or 256).
+constexpr int kMaxParts = 128;
 // Calls of few rows in short tables: a cluster of CTAs takes one item (the kernel's kCluster form),
 // each warp every (4 * cluster)-th stage of it, and joins its warps' parts through distributed shared
 // memory, without a look at the other rows, parts in the workspace or a second launch.  A cluster
 // has up to 8 CTAs: as many as the device runs at once, and as have 128 positions of a full table
-// row each.  Past 512 positions for each the equal shares of all SMs win.  (32 query heads over 8
-// kv heads.  head_dim 64: 1 row of 512 positions 4.2 us, cut into parts 6.9; of 4096 7.6 and 9.9;
-// of 16384 22.6 and 15.6.  head_dim 128: 8 rows of 512 7.2 and 9.7; 16 rows of 64 4.2 and 8.3.)
-constexpr int kClusterMax = 8, kClusterLeast = 128, kClusterMost = 512;
+// row each.  It is not for rows longer than cluster_most() for each CTA, where equal shares for all SMs win.
+// (32 query heads over 8 kv heads.  head_dim 64: 1 row of 512 positions 4.2 us, cut into parts 7.6; of
+// 4096 7.5 and 8.4; of 8192 11.5 and 9.9.  head_dim 128: 16 rows of 64 4.1 and 8.3; 8 rows of 512 7.2
+// and 9.7; 1 row of 4096 11.8 and 9.8, 4 rows, whose clusters fill the device, 18.0 and 20.1.)
+constexpr int kClusterMax = 8, kClusterLeast = 128;
+constexpr int cluster_most(int head_dim, int nh, bool fill) {
+  const int n = 32768 / (head_dim * nh) * (fill ? 2 : 1);
+  return n < 512 ? n : 512;
+}
 // CTAs of an SM.  head_dim 64 has more to compute for a byte and wants more warps, with two
 // stages each (64 rows of up to 8000 positions: 86 us with 3 CTAs of 2 stages, 94 with 2 of 3).
 constexpr int attn_per_sm(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
@@ -183,8 +188,10 @@ struct AttnCfg {
   static constexpr int kSmem = kAttnWarps * (kRing + 8 * D * 4);  // the rings, then the warps' parts of 8 heads
 };
 
-struct __align__(16) AttnDesc {  // the item that worker w began and did not finish
-  int row, item, parts, pad;
+// An item cut into parts (parts 0: none): at the place of the worker that began it, or in calls of
+// few items (by_item) at the item's own.
+struct __align__(16) AttnDesc {
+  int row, item, parts, first;  // first: the worker that began it
 };
 
 template <typename T>
@@ -237,7 +244,8 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
 template <typename T, int D, int NH, bool kCluster>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
     k_paged_attention(const PagedAttention a, const PagedPool pool, const PagedTables tab, const int group, const int blocks,
-                      const bool coop, const int cost, const int cluster) {
+                      const bool coop, const int cost, const int cluster,
+                      const bool by_item) {
   using C = AttnCfg<D, NH>;
   constexpr int kB = D / 32, kVB = D / 64, kU = C::kTiles, kHeads = C::kHeads, kThreads = kAttnWarps * 32, kPos = C::kPos;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
@@ -337,12 +345,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
         sh_base[w] = base;
       }
     }
-    if (coop ? threadIdx.x == 0 : lane == 0) desc[worker].parts = 0;
+    if (!by_item && (coop ? threadIdx.x == 0 : lane == 0)) desc[worker].parts = 0;
     // rows of no positions are zero
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x)
-      if (length(r) == 0)
+      if (length(r) == 0) {
         for (int e = threadIdx.x; e < a.heads * D / 8; e += kThreads)
           reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)r * a.out_stride)[e] = make_uint4(0u, 0u, 0u, 0u);
+        if (by_item)
+          for (int e = threadIdx.x; e < items; e += kThreads) desc[r * items + e].parts = 0;
+      }
     __syncthreads();
     u0 = first_unit(worker);
     u1 = worker + 1 < used ? first_unit(worker + 1) : total;
@@ -787,14 +798,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       }
       __syncthreads();  // the parts' memory is free again
     }
-    if (!whole && t0 == 0 && (coop ? threadIdx.x == 0 : lane == 0)) {
+    if (t0 == 0 && (!whole || by_item) && (coop ? threadIdx.x == 0 : lane == 0)) {
       // the worker of the item's last unit, which lies nt - t1 units past this span
-      const long long last = begun + nt - 1;
-      desc[worker].row = row;
-      desc[worker].item = item;
-      const long long whole_ones = more * (each + 1);
+      const long long last = begun + nt - 1, whole_ones = more * (each + 1);
       const int w = last < whole_ones ? (int)divide(last, each + 1) : more + (int)divide(last - whole_ones, each);
-      desc[worker].parts = w - worker + 1;
+      AttnDesc& d = desc[by_item ? row * items + item : worker];
+      d.row = row;
+      d.item = item;
+      d.first = worker;
+      d.parts = whole ? 0 : w - worker + 1;
     }
     if (u >= u1) break;
   }
@@ -802,129 +814,55 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
 }
 
 // Joins the parts of the item that worker blockIdx.x began.  A thread adds up four dimensions of
-// one head.  Few parts: kJoinFew in a round trip to memory, after the description's.  Many
-// (compiled in for calls of few items: up to kMaxParts parts of a long sequence): groups of
-// threads take every G-th part, in a fixed order, and the maxima and weights come first, so that
-// the long sums are plain multiply-adds of independent loads (one sequence of 8000 positions, 8
-// kv heads of 64: 13.4 us with the attention, 17.1 by the path for few).
-constexpr int kJoinChunk = 128, kJoinFew = 4;
+// one head, kJoinFew parts in a round trip to memory, after the description's.
+constexpr int kJoinFew = 4;
 template <int D, int NH>
 constexpr int join_lanes() { return 8 * NH * D / 4; }
 
-template <typename T, int D, int NH, bool kMany>
-__global__ void __launch_bounds__(kMany ? 1024 : join_lanes<D, NH>()) k_paged_join(const PagedAttention a, const int group, const int blocks) {
+template <typename T, int D, int NH>
+__global__ void __launch_bounds__(join_lanes<D, NH>()) k_paged_join(const PagedAttention a, const int group, const int blocks) {
   using C = AttnCfg<D, NH>;
-  constexpr int kLanes = join_lanes<D, NH>(), kHeads = C::kHeads;
+  constexpr int kHeads = C::kHeads;
   grid_dependency_wait();  // and no early launch after this: the next attention fills the GPU, and is the slower for odd places
   const AttnDesc* desc = static_cast<const AttnDesc*>(a.workspace);
   const float* slots = reinterpret_cast<const float*>(desc + C::kMaxWorkers);
   const AttnDesc it = desc[blockIdx.x];
   if (it.parts == 0) return;
-  const int head = threadIdx.x % kLanes / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  const int head = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
   auto part = [&](int i) { return slots + (size_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::kSlot; };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  if (!kMany || it.parts <= 2 * kJoinFew) {
-    if (threadIdx.x >= kLanes) return;
-    float top = -INFINITY;
-    for (int i0 = 0; i0 < it.parts; i0 += kJoinFew) {
-      float m[kJoinFew], l[kJoinFew];
-      float4 x[kJoinFew];
-      const float old = top;
+  float sum = 0.f, top = -INFINITY;
+  for (int i0 = 0; i0 < it.parts; i0 += kJoinFew) {
+    float m[kJoinFew], l[kJoinFew];
+    float4 x[kJoinFew];
+    const float old = top;
 #pragma unroll
-      for (int i = 0; i < kJoinFew; ++i) {
-        m[i] = -INFINITY;
-        if (i0 + i < it.parts) {
-          const float* p = part(i0 + i);
-          m[i] = p[head];
-          l[i] = p[kHeads + head];
-          x[i] = *reinterpret_cast<const float4*>(p + 2 * kHeads + head * D + d);
-        }
-        top = fmaxf(top, m[i]);
+    for (int i = 0; i < kJoinFew; ++i) {
+      m[i] = -INFINITY;
+      if (i0 + i < it.parts) {
+        const float* p = part(i0 + i);
+        m[i] = p[head];
+        l[i] = p[kHeads + head];
+        x[i] = *reinterpret_cast<const float4*>(p + 2 * kHeads + head * D + d);
       }
-      const float low = top == -INFINITY ? 0.f : top, corr = exp2_fast(old - low);
-      sum *= corr;
-      acc.x *= corr;
-      acc.y *= corr;
-      acc.z *= corr;
-      acc.w *= corr;
+      top = fmaxf(top, m[i]);
+    }
+    const float low = top == -INFINITY ? 0.f : top, corr = exp2_fast(old - low);
+    sum *= corr;
+    acc.x *= corr;
+    acc.y *= corr;
+    acc.z *= corr;
+    acc.w *= corr;
 #pragma unroll
-      for (int i = 0; i < kJoinFew; ++i)
-        if (i0 + i < it.parts) {
-          const float f = exp2_fast(m[i] - low);
-          sum = fmaf(l[i], f, sum);
-          acc.x = fmaf(x[i].x, f, acc.x);
-          acc.y = fmaf(x[i].y, f, acc.y);
-          acc.z = fmaf(x[i].z, f, acc.z);
-          acc.w = fmaf(x[i].w, f, acc.w);
-        }
-    }
-  } else if constexpr (kMany) {
-    __shared__ float sh_w[kJoinChunk][kHeads], sh_l[kJoinChunk][kHeads], sh_max[kHeads], sh_sum[kHeads], sh_corr[kHeads];
-    __shared__ float4 sh_acc[1024];
-    const int grp = threadIdx.x / kLanes, groups = blockDim.x / kLanes;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    if (threadIdx.x < kHeads) {
-      sh_max[threadIdx.x] = -INFINITY;
-      sh_sum[threadIdx.x] = 0.f;
-    }
-    for (int c0 = 0; c0 < it.parts; c0 += kJoinChunk) {
-      const int n = min(kJoinChunk, it.parts - c0);
-      for (int e = threadIdx.x; e < n * kHeads; e += blockDim.x) {
-        const float* p = part(c0 + e / kHeads);
-        sh_w[e / kHeads][e % kHeads] = p[e % kHeads];
-        sh_l[e / kHeads][e % kHeads] = p[kHeads + e % kHeads];
+    for (int i = 0; i < kJoinFew; ++i)
+      if (i0 + i < it.parts) {
+        const float f = exp2_fast(m[i] - low);
+        sum = fmaf(l[i], f, sum);
+        acc.x = fmaf(x[i].x, f, acc.x);
+        acc.y = fmaf(x[i].y, f, acc.y);
+        acc.z = fmaf(x[i].z, f, acc.z);
+        acc.w = fmaf(x[i].w, f, acc.w);
       }
-      __syncthreads();
-      for (int h = warp; h < kHeads; h += warps) {
-        float top = sh_max[h];
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, sh_w[i][h]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float low = top == -INFINITY ? 0.f : top;
-        float t = 0.f;
-        for (int i = lane; i < n; i += 32) {
-          const float f = exp2_fast(sh_w[i][h] - low);
-          sh_w[i][h] = f;
-          t = fmaf(sh_l[i][h], f, t);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        if (lane == 0) {
-          const float corr = exp2_fast(sh_max[h] - low);
-          sh_corr[h] = corr;
-          sh_sum[h] = sh_sum[h] * corr + t;
-          sh_max[h] = top;
-        }
-      }
-      __syncthreads();
-      const float corr = sh_corr[head];
-      acc.x *= corr;
-      acc.y *= corr;
-      acc.z *= corr;
-      acc.w *= corr;
-#pragma unroll 8
-      for (int i = grp; i < n; i += groups) {
-        const float4 x = *reinterpret_cast<const float4*>(part(c0 + i) + 2 * kHeads + head * D + d);
-        const float f = sh_w[i][head];
-        acc.x = fmaf(x.x, f, acc.x);
-        acc.y = fmaf(x.y, f, acc.y);
-        acc.z = fmaf(x.z, f, acc.z);
-        acc.w = fmaf(x.w, f, acc.w);
-      }
-      __syncthreads();  // the weights' memory is free again
-    }
-    sh_acc[threadIdx.x] = acc;
-    __syncthreads();
-    if (grp > 0) return;
-    for (int i = 1; i < groups; ++i) {
-      const float4 x = sh_acc[threadIdx.x + i * kLanes];
-      acc.x += x.x;
-      acc.y += x.y;
-      acc.z += x.z;
-      acc.w += x.w;
-    }
-    sum = sh_sum[head];
   }
   if (head >= group - it.item % blocks * kHeads) return;  // a head block's empty places
   uint2 r;
@@ -932,6 +870,94 @@ __global__ void __launch_bounds__(kMany ? 1024 : join_lanes<D, NH>()) k_paged_jo
   r.y = pack2<T>(acc.z / sum, acc.w / sum);
   const int h = it.item / blocks * group + it.item % blocks * kHeads + head;
   *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (size_t)it.row * a.out_stride + (size_t)h * D + d) = r;
+}
+
+// The same for calls of few items, which may have a hundred parts: a CTA for 64 dimensions of a head
+// of an item, groups of threads that take every G-th part, the parts' values on their way while
+// the weights are worked out (1 sequence of 104000 positions, 2 kv heads of 128: 26.5 us with the
+// attention; 37 with a CTA for all of an item, bound by what one SM can load).
+constexpr int kJoinThreads = 256, kJoinDims = 64;
+template <typename T, int D, int NH>
+__global__ void __launch_bounds__(kJoinThreads) k_paged_join_heads(const PagedAttention a, const int group, const int blocks, const int items) {
+  using C = AttnCfg<D, NH>;
+  constexpr int kHeads = C::kHeads, kLanes = kJoinDims / 4, kGroups = kJoinThreads / kLanes, kAhead = 8, kWarps = kJoinThreads / 32;
+  __shared__ float sh_w[kJoinThreads], sh_top[kWarps], sh_sum[kWarps];
+  __shared__ float4 sh_acc[kJoinThreads];
+  grid_dependency_wait();
+  const int share = blockIdx.x % (D / kJoinDims), head = blockIdx.x / (D / kJoinDims) % kHeads, at = blockIdx.x / (D / kJoinDims * kHeads);
+  const int item = at % items;
+  if (head >= group - item % blocks * kHeads) return;  // a head block's empty places
+  const AttnDesc* desc = static_cast<const AttnDesc*>(a.workspace);
+  const float* slots = reinterpret_cast<const float*>(desc + C::kMaxWorkers);
+  const AttnDesc it = desc[at];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid / kLanes, d = share * kJoinDims + tid % kLanes * 4;
+  auto part = [&](int i) { return slots + (size_t)(2 * (it.first + i) + (i == 0 ? 1 : 0)) * C::kSlot; };
+  auto value = [&](int i) { return *reinterpret_cast<const float4*>(part(i) + 2 * kHeads + head * D + d); };
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f, top = -INFINITY;
+  for (int c0 = 0; c0 < it.parts; c0 += kJoinThreads) {
+    const int n = min(kJoinThreads, it.parts - c0);
+    float m = -INFINITY, l = 0.f;
+    if (tid < n) {
+      m = part(c0 + tid)[head];
+      l = part(c0 + tid)[kHeads + head];
+    }
+    float4 x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (grp + k * kGroups < n) x[k] = value(c0 + grp + k * kGroups);
+    float most = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) sh_top[warp] = most;
+    __syncthreads();
+    const float old = top;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh_top[w]);
+    const float low = top == -INFINITY ? 0.f : top, corr = exp2_fast(old - low), f = exp2_fast(m - low);
+    sh_w[tid] = f;
+    float t = l * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) sh_sum[warp] = t;
+    __syncthreads();
+    sum *= corr;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sum += sh_sum[w];
+    acc.x *= corr;
+    acc.y *= corr;
+    acc.z *= corr;
+    acc.w *= corr;
+    auto add = [&](const float4& v, float by) {
+      acc.x = fmaf(v.x, by, acc.x);
+      acc.y = fmaf(v.y, by, acc.y);
+      acc.z = fmaf(v.z, by, acc.z);
+      acc.w = fmaf(v.w, by, acc.w);
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (grp + k * kGroups < n) add(x[k], sh_w[grp + k * kGroups]);
+#pragma unroll 8
+    for (int i = grp + kAhead * kGroups; i < n; i += kGroups) add(value(c0 + i), sh_w[i]);
+    __syncthreads();  // the weights' memory is free again
+  }
+  if (it.parts == 0) return;
+  sh_acc[tid] = acc;
+  __syncthreads();
+  if (grp > 0) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) {
+    const float4 x = sh_acc[tid + i * kLanes];
+    acc.x += x.x;
+    acc.y += x.y;
+    acc.z += x.z;
+    acc.w += x.w;
+  }
+  uint2 r;
+  r.x = pack2<T>(acc.x / sum, acc.y / sum);
+  r.y = pack2<T>(acc.z / sum, acc.w / sum);
+  const int h = item / blocks * group + item % blocks * kHeads + head;
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (size_t)(at / items) * a.out_stride + (size_t)h * D + d) = r;
 }
 
 template <typename F>
@@ -1036,20 +1062,19 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   const long long cap = (long long)tab.width << pool.page_shift;
   int cluster = kClusterMax;
   while (cluster > 1 && (cap <= (long long)cluster / 2 * kClusterLeast || all > resident_clusters<T, D, NH>(dev, cluster))) cluster /= 2;
-  if (all * cluster <= ctas && cap <= (long long)cluster * kClusterMost) {
+  if (all * cluster <= ctas && cap <= (long long)cluster * cluster_most(D, NH, all * cluster * 2 >= ctas)) {
     ClusterLaunch<T, D, NH> l((unsigned)all, cluster, stream);
-    return launched("k_paged_attention", cudaLaunchKernelEx(&l.cfg, k_paged_attention<T, D, NH, true>, a, pool, tab, group, blocks, true, 0, cluster));
+    return launched("k_paged_attention", cudaLaunchKernelEx(&l.cfg, k_paged_attention<T, D, NH, true>, a, pool, tab, group, blocks, true, 0, cluster, false));
   }
+  const bool many = coop && all * 8 < ctas;  // items few enough to be cut into many parts
   const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH, false>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
-                                                                 stream, true, a, pool, tab, group, blocks, coop, cost, 1));
+                                                                 stream, true, a, pool, tab, group, blocks, coop, cost, 1, many));
   if (rc2 != W4A16_OK) return rc2;
-  // Items few enough to be cut into many parts get groups of threads that share them; the rest the
-  // kernel without shared memory, whose CTAs do not keep the next attention's off the SMs.
-  const bool many = coop && (long long)a.rows * pool.kv_heads * blocks * 2 * kJoinFew < ctas;
-  constexpr int lanes = join_lanes<D, NH>(), groups = 1024 / lanes < 4 ? 1024 / lanes : 4;
-  return launched("k_paged_join",
-                  launch_maybe_pdl(many ? k_paged_join<T, D, NH, true> : k_paged_join<T, D, NH, false>, dim3(workers),
-                                   dim3(many ? lanes * groups : lanes), 0, stream, true, a, group, blocks));
+  if (many)
+    return launched("k_paged_join_heads", launch_maybe_pdl(k_paged_join_heads<T, D, NH>, dim3((unsigned)all * C::kHeads * (D / kJoinDims)), dim3(kJoinThreads), 0,
+                                                           stream, true, a, group, blocks, pool.kv_heads * blocks));
+  return launched("k_paged_join", launch_maybe_pdl(k_paged_join<T, D, NH>, dim3(workers), dim3(join_lanes<D, NH>()), 0, stream, true, a, group,
+                                                   blocks));
 }
 
 }  // namespace
