@@ -165,7 +165,10 @@ constexpr int kMaxParts = 128;
 // (32 query heads over 8 kv heads.  head_dim 64: 1 row of 512 positions 4.2 us, cut into parts 7.6; of
 // 4096 7.5 and 8.4; of 8192 11.5 and 9.9.  head_dim 128: 16 rows of 64 4.1 and 8.3; 8 rows of 512 7.2
 // and 9.7; 1 row of 4096 11.8 and 9.8, 4 rows, whose clusters fill the device, 18.0 and 20.1.)
-constexpr int kClusterMax = 8, kClusterLeast = 128;
+// In tables of up to kTwiceMost positions CTAs of an item each are faster even if only half of them
+// fit at once (8 kv heads: 60 rows of up to 30 positions 7.6 and 10.1, of up to 200 9.4 and 10.8; 74
+// rows of exactly 256 with head_dim 128 are the exception, 20.7 and 19.4).
+constexpr int kClusterMax = 8, kClusterLeast = 128, kTwiceMost = 256;
 constexpr int cluster_most(int head_dim, int nh, bool fill) {
   const int n = 32768 / (head_dim * nh) * (fill ? 2 : 1);
   return n < 512 ? n : 512;
@@ -1062,7 +1065,8 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
   const long long cap = (long long)tab.width << pool.page_shift;
   int cluster = kClusterMax;
   while (cluster > 1 && (cap <= (long long)cluster / 2 * kClusterLeast || all > resident_clusters<T, D, NH>(dev, cluster))) cluster /= 2;
-  if (all * cluster <= ctas && cap <= (long long)cluster * cluster_most(D, NH, all * cluster * 2 >= ctas)) {
+  const bool few = all * cluster <= ctas && cap <= (long long)cluster * cluster_most(D, NH, all * cluster * 2 >= ctas);
+  if (few || (all <= 2 * ctas && cap <= kTwiceMost)) {
     ClusterLaunch<T, D, NH> l((unsigned)all, cluster, stream);
     return launched("k_paged_attention", cudaLaunchKernelEx(&l.cfg, k_paged_attention<T, D, NH, true>, a, pool, tab, group, blocks, true, 0, cluster, false));
   }
