@@ -114,6 +114,14 @@ def test_logits(lib):
     assert call(rows=0) == 0 and call(vocab=0) == 0
 
 
+@pytest.mark.parametrize("cls,pack", [(_lib.PagePool, _lib.pack_pool), (_lib.PageTables, _lib.pack_tables), (_lib.PageState, _lib.pack_state),
+                                      (_lib.PageBlocks, _lib.pack_blocks), (_lib.LogitsDesc, _lib.pack_logits)])
+def test_packed_structures_are_the_declared_ones(cls, pack):
+    values = range(1, len(cls._fields_) + 1)
+    packed = cls.from_buffer_copy(pack(*values))
+    assert len(pack(*values)) == ctypes.sizeof(cls) and [getattr(packed, name) for name, _ in cls._fields_] == list(values)
+
+
 def test_python_calls_refuse_tensors_that_are_not_on_a_gpu():
     import torch
 

@@ -8,6 +8,7 @@ There is no fallback: if the library is missing every op raises.
 import ctypes
 import functools
 import os
+import struct
 
 LIB_NAME = "libw4a16_b200.so"
 ENV_LIB = "W4A16_B200_LIB"
@@ -29,7 +30,6 @@ _i = ctypes.c_int
 _u = ctypes.c_uint
 _sz = ctypes.c_size_t
 _ll = ctypes.c_longlong
-
 
 
 class PagePool(ctypes.Structure):
@@ -62,6 +62,16 @@ class LogitsDesc(ctypes.Structure):
                 ("prompt_lens", _p), ("total_lens", _p), ("repetition", _p), ("frequency", _p), ("presence", _p),
                 ("bias", _p), ("bias_stride", _ll), ("bias_ids", _p), ("bias_values", _p), ("pairs", _i),
                 ("mask", _p), ("mask_stride", _ll)]
+
+
+def _packer(cls):
+    """The bytes of a structure from its fields in order (0 for a null pointer), to be passed where a
+    pointer to it is due: filling in a ctypes object takes four times as long."""
+    codes = {_p: "P", _i: "i", _ll: "q"}
+    return struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_)).pack
+
+
+pack_pool, pack_tables, pack_state, pack_blocks, pack_logits = map(_packer, (PagePool, PageTables, PageState, PageBlocks, LogitsDesc))
 
 
 _REF_SIG = [_p, _p, _p, _p, _i, _i, _p]

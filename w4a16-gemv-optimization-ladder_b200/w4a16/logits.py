@@ -4,14 +4,14 @@ benchmarks/end_to_end.py:33-37.)"""
 import torch
 
 from . import _lib
-from .paged import _byref, _call, _refuse
+from .paged import _call, _refuse
 
 _LOGIT_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
 def _per_row(t, rows, dtype, name, dev):
     if t is None:
-        return None
+        return 0
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev and t.dim() == 1 and t.shape[0] == rows
             and t.is_contiguous()):
         _refuse(f"{name} must be a contiguous {dtype} [{rows}] tensor on {dev}")
@@ -54,10 +54,10 @@ def process_logits(logits, *, tokens=None, prompt_lens=None, total_lens=None, re
     dev, shape = logits.device, logits.shape
     rows, vocab = (1, shape[0]) if len(shape) == 1 else shape
     if out is None:
-        out = logits.new_empty(shape)
+        out = logits.new_empty(*shape)
     else:
         _rows(out, (logits.dtype,), (shape,), "out", dev)
-    tp = pl = tl = rp = fp = pp = bp = ip = vp = mp = None
+    tp = pl = tl = rp = fp = pp = bp = ip = vp = mp = 0
     token_bytes = history = token_stride = bias_stride = pairs = mask_stride = 0
     if tokens is not None:
         if not (isinstance(tokens, torch.Tensor) and tokens.dim() == 2):
@@ -88,7 +88,7 @@ def process_logits(logits, *, tokens=None, prompt_lens=None, total_lens=None, re
         mask_stride = mask.stride(0) if mask.dim() == 2 and rows > 1 else 0
     if rows and vocab:
         stride, out_stride = (vocab, vocab) if rows == 1 else (logits.stride(0), out.stride(0))
-        d = _lib.LogitsDesc(logits.data_ptr(), out.data_ptr(), _LOGIT_DTYPES[logits.dtype], rows, vocab, stride, out_stride, tp, token_bytes,
-                            history, token_stride, pl, tl, rp, fp, pp, bp, bias_stride, ip, vp, pairs, mp, mask_stride)
-        _call("w4a16_process_logits", dev, _byref(d))
+        d = _lib.pack_logits(logits.data_ptr(), out.data_ptr(), _LOGIT_DTYPES[logits.dtype], rows, vocab, stride, out_stride, tp, token_bytes,
+                             history, token_stride, pl, tl, rp, fp, pp, bp, bias_stride, ip, vp, pairs, mp, mask_stride)
+        _call("w4a16_process_logits", dev, d)
     return out

@@ -22,7 +22,6 @@ graph; nothing is kept between calls.  Wrong dtypes, devices, shapes or layouts 
 RuntimeError before anything is launched; indices are checked in the kernels (a bad page, position
 or sequence gives NaN, is skipped, or is refused, as each function says).
 """
-import ctypes
 import functools
 
 import torch
@@ -30,7 +29,6 @@ import torch
 from . import _lib
 
 _POOL_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
-_byref = ctypes.byref
 # torch.cuda.current_stream(device).cuda_stream and torch.cuda.current_device(), without the objects
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
@@ -54,7 +52,7 @@ def _call(name, dev, *args):
 
 
 def _pool(k_pages, v_pages):
-    """The C description of one layer's pool, checked."""
+    """One layer's pool, checked: its C description, kv_heads, head_dim."""
     dtype = _POOL_DTYPES.get(getattr(k_pages, "dtype", None))
     if dtype is None or k_pages.dim() != 4 or not k_pages.is_cuda:
         _refuse("k_pages must be an fp16 or bf16 CUDA tensor [pages, kv_heads, page_size, head_dim]")
@@ -67,8 +65,8 @@ def _pool(k_pages, v_pages):
     if sd != 1:
         _refuse("the last dimension of the pages must be contiguous")
     # a dimension of one entry may carry any stride
-    return _lib.PagePool(k_pages.data_ptr(), v_pages.data_ptr(), dtype, pages, kv_heads, page_size, head_dim,
-                         sp if pages > 1 else 8, sh if kv_heads > 1 else 8, st if page_size > 1 else 8)
+    return _lib.pack_pool(k_pages.data_ptr(), v_pages.data_ptr(), dtype, pages, kv_heads, page_size, head_dim, sp if pages > 1 else 8,
+                          sh if kv_heads > 1 else 8, st if page_size > 1 else 8), kv_heads, head_dim
 
 
 @functools.lru_cache(maxsize=64)
@@ -83,7 +81,7 @@ def _tables(tables, dev):
     stride, one = tables.stride()
     if one != 1 and width > 1:
         _refuse("the rows of tables must be contiguous")
-    return _lib.PageTables(tables.data_ptr(), sequences, width, stride)
+    return _lib.pack_tables(tables.data_ptr(), sequences, width, stride)
 
 
 def _index(t, n, name, dev):
@@ -119,11 +117,11 @@ def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=
     Returns out.  A position past the tables' width or the angles, a sequence outside `tables` or a
     page outside the pool writes nothing to the cache and gives NaN.  A (sequence, position) may
     occur once per call."""
-    pool = _pool(k_pages, v_pages)
+    pool, kvh, d = _pool(k_pages, v_pages)
     dev, dtype = k_pages.device, k_pages.dtype
     if not (isinstance(k, torch.Tensor) and k.dim() == 3):
         _refuse("k must be [tokens, kv_heads, head_dim]")
-    n, kvh, d = k.shape[0], pool.kv_heads, pool.head_dim
+    n = k.shape[0]
     kp, ks = _tokens(k, n, kvh, d, dtype, "k", dev)
     vp, vs = _tokens(v, n, kvh, d, dtype, "v", dev)
     pos = _index(positions, n, "positions", dev)
@@ -147,12 +145,12 @@ def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=
         heads = q.shape[1]
         qp, qs = _tokens(q, n, heads, d, dtype, "q", dev)
         if out is None:
-            out = q.new_empty((n, heads, d))
+            out = q.new_empty(n, heads, d)  # (numbers: a tuple costs half as much again)
             op, os_ = out.data_ptr(), heads * d
         else:
             op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
     if n:
-        _call("w4a16_paged_append", dev, qp, qs, kp, ks, vp, vs, pos, sq, n, heads, _byref(tab), cp, sp, angles, _byref(pool), op, os_)
+        _call("w4a16_paged_append", dev, qp, qs, kp, ks, vp, vs, pos, sq, n, heads, tab, cp, sp, angles, pool, op, os_)
     return out
 
 
@@ -170,9 +168,8 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
 
     Returns out [rows, heads, head_dim].  A row of length <= 0 is zero; a length past the tables'
     width, a sequence outside `tables` or a page outside the pool gives NaN."""
-    pool = _pool(k_pages, v_pages)
+    pool, kvh, d = _pool(k_pages, v_pages)
     dev, dtype = k_pages.device, k_pages.dtype
-    kvh, d = pool.kv_heads, pool.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() == 3):
         _refuse("q must be [rows, heads, head_dim]")
     n, heads = q.shape[0], q.shape[1]
@@ -183,7 +180,7 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     sq = _index(seqs, n, "seqs", dev) if seqs is not None else None
     tab = _tables(tables, dev)
     if out is None:
-        out = q.new_empty((n, heads, d))
+        out = q.new_empty(n, heads, d)
         op, os_ = out.data_ptr(), heads * d
     else:
         op, os_ = _tokens(out, n, heads, d, dtype, "out", dev)
@@ -197,7 +194,7 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
                 and workspace.is_contiguous()):
             _refuse(f"workspace must be a contiguous uint8 tensor on {dev}")
         size = workspace.numel()
-    _call("w4a16_paged_attention", dev, qp, qs, lens, sq, n, heads, _byref(tab), _byref(pool), float(d ** -0.5 if scale is None else scale),
+    _call("w4a16_paged_attention", dev, qp, qs, lens, sq, n, heads, tab, pool, float(d ** -0.5 if scale is None else scale),
           op, os_, workspace.data_ptr(), size)
     return out
 
@@ -210,13 +207,13 @@ def _state(tables, lengths, refs, page_size):
         _refuse("tables must be a contiguous int32 [sequences, width] CUDA tensor")
     dev = tables.device
     sequences, width = tables.shape
-    return _lib.PageState(tables.data_ptr(), _index(lengths, sequences, "lengths", dev), _index(refs, None, "refs", dev), sequences,
-                          width, refs.shape[0], page_size, width)
+    return _lib.pack_state(tables.data_ptr(), _index(lengths, sequences, "lengths", dev), _index(refs, None, "refs", dev), sequences,
+                           width, refs.shape[0], page_size, width)
 
 
 def _blocks(k_pages, v_pages):
-    """The C description of the pages' bytes in all layers, checked: [layers, pages, ...] or one
-    layer's [pages, kv_heads, page_size, head_dim], every page one dense block."""
+    """The pages' bytes in all layers, checked ([layers, pages, ...] or one layer's [pages, kv_heads,
+    page_size, head_dim], every page one dense block): their C description, pages."""
     if not (isinstance(k_pages, torch.Tensor) and k_pages.is_cuda and k_pages.dim() in (4, 5)):
         _refuse("k_pages must be a CUDA tensor [layers, pages, kv_heads, page_size, head_dim] or [pages, kv_heads, page_size, head_dim]")
     shape, stride = k_pages.shape, k_pages.stride()
@@ -233,8 +230,8 @@ def _blocks(k_pages, v_pages):
             if n != 1 and st != block:
                 _refuse("a page must be one dense block")
             block *= n
-    return _lib.PageBlocks(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, ls * size if layers > 1 else 0,
-                           (ps if pages > 1 else elements) * size, elements * size)
+    return _lib.pack_blocks(k_pages.data_ptr(), v_pages.data_ptr(), layers, pages, ls * size if layers > 1 else 0,
+                            (ps if pages > 1 else elements) * size, elements * size), pages
 
 
 def extend_sequences(tables, lengths, refs, seqs, counts, *, page_size):
@@ -251,7 +248,7 @@ def extend_sequences(tables, lengths, refs, seqs, counts, *, page_size):
     n = seqs.shape[0]
     c = _index(counts, n, "counts", dev)
     ok = torch.empty_like(seqs)
-    _call("w4a16_pages_extend", dev, _byref(st), s, c, n, ok.data_ptr())
+    _call("w4a16_pages_extend", dev, st, s, c, n, ok.data_ptr())
     return ok
 
 
@@ -262,18 +259,18 @@ def fork_sequences(k_pages, v_pages, tables, lengths, refs, src, dst):
 
     Returns ok, int32 [n], as extend_sequences does; a dst that is not empty, is its own src or was
     named by an earlier request is refused.  All requests see the state from before the call."""
-    b = _blocks(k_pages, v_pages)
+    b, pages = _blocks(k_pages, v_pages)
     st = _state(tables, lengths, refs, k_pages.shape[-2])
     dev = tables.device
-    if k_pages.device != dev or st.pages != b.pages:
-        _refuse(f"refs must have one entry for each of the {b.pages} pages, and k_pages be on {dev}")
+    if k_pages.device != dev or refs.shape[0] != pages:
+        _refuse(f"refs must have one entry for each of the {pages} pages, and k_pages be on {dev}")
     s = _index(src, None, "src", dev)
     n = src.shape[0]
     t = _index(dst, n, "dst", dev)
     ok = torch.empty_like(src)
     need = _lib.lib().w4a16_pages_fork_scratch_bytes(n)
     scratch = src.new_empty((need + 3) // 4)
-    _call("w4a16_pages_fork", dev, _byref(st), _byref(b), s, t, n, ok.data_ptr(), scratch.data_ptr(), need)
+    _call("w4a16_pages_fork", dev, st, b, s, t, n, ok.data_ptr(), scratch.data_ptr(), need)
     return ok
 
 
@@ -284,18 +281,18 @@ def free_sequences(tables, lengths, refs, seqs):
     dev = tables.device
     s = _index(seqs, None, "seqs", dev)
     ok = torch.empty_like(seqs)
-    _call("w4a16_pages_free", dev, _byref(st), s, seqs.shape[0], ok.data_ptr())
+    _call("w4a16_pages_free", dev, st, s, seqs.shape[0], ok.data_ptr())
     return ok
 
 
 def copy_pages(k_pages, v_pages, src, dst):
     """Copies page src[i] to page dst[i] in every layer (int32 [n]).  A pair with an index outside
     the pool is skipped.  No page may be in both lists, or twice in dst."""
-    b = _blocks(k_pages, v_pages)
+    b, _ = _blocks(k_pages, v_pages)
     dev = k_pages.device
     s = _index(src, None, "src", dev)
     n = src.shape[0]
-    _call("w4a16_pages_copy", dev, _byref(b), s, _index(dst, n, "dst", dev), n)
+    _call("w4a16_pages_copy", dev, b, s, _index(dst, n, "dst", dev), n)
 
 
 def compact_pages(k_pages, v_pages, tables, refs, *, inplace=True):
@@ -304,16 +301,16 @@ def compact_pages(k_pages, v_pages, tables, refs, *, inplace=True):
 
     Returns (tables, refs, moved): the tables and refs with the new page numbers (updated in place, or
     new tensors with inplace=False), and the number of pages moved, int32 [1] on the device."""
-    b = _blocks(k_pages, v_pages)
+    b, pages = _blocks(k_pages, v_pages)
     dev = k_pages.device
     if not (isinstance(tables, torch.Tensor) and tables.device == dev and tables.dtype == torch.int32 and tables.is_contiguous()):
         _refuse(f"tables must be a contiguous int32 tensor on {dev}")
-    r = _index(refs, b.pages, "refs", dev)
+    r = _index(refs, pages, "refs", dev)
     new_tables, new_refs = (tables, refs) if inplace else (torch.empty_like(tables), torch.empty_like(refs))
     moved = refs.new_empty(1)
-    need = _lib.lib().w4a16_pages_compact_scratch_bytes(b.pages)
+    need = _lib.lib().w4a16_pages_compact_scratch_bytes(pages)
     scratch = refs.new_empty((need + 3) // 4)
-    _call("w4a16_pages_compact", dev, _byref(b), tables.data_ptr(), new_tables.data_ptr(), tables.numel(), r, new_refs.data_ptr(),
+    _call("w4a16_pages_compact", dev, b, tables.data_ptr(), new_tables.data_ptr(), tables.numel(), r, new_refs.data_ptr(),
           moved.data_ptr(), scratch.data_ptr(), need)
     return new_tables, new_refs, moved
 
