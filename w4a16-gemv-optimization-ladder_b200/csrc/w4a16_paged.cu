@@ -305,7 +305,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
       const int h0 = cur.item / blocks * group + cur.item % blocks * kHeads, n = min(kHeads, group - cur.item % blocks * kHeads) * D / 8;
       for (int e = rank * kThreads + threadIdx.x; e < n; e += kThreads * cluster)
         reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (size_t)cur.row * a.out_stride + (size_t)h0 * D)[e] = make_uint4(0u, 0u, 0u, 0u);
-      return;  // the whole cluster
+      __syncwarp();
+      cluster_sync_all();  // the join's two, though no CTA of this cluster gets there: each takes every barrier, whatever
+      cluster_sync_all();  // length it read
+      return;
     }
   } else {
     // the units of all rows, and the row that holds each worker's first one
