@@ -165,38 +165,44 @@ __global__ void __launch_bounds__(256) k_pages_free(const PagesState st, const i
 
 // Compaction plan, one CTA: with L live pages, the k-th live page at or above L moves to the
 // k-th free page below it.  Sources and destinations are disjoint, and no page moves that
-// does not have to.
+// does not have to.  One prefix sum of the live pages is all it takes: with n live pages before
+// page p and B live pages below L, a live page p >= L is the (n - B)-th to move, a free page
+// p < L the (p - n)-th to be filled.
 __global__ void __launch_bounds__(1024) k_compact_plan(const int* refs, int pages, int* refs_out, int* where,
                                                        int2* moves, int* moved) {
-  __shared__ int sh[33];
+  __shared__ int sh[33], sh_below;
   grid_dependency_wait();
   grid_launch_dependents();
   const int per = (pages + 1023) / 1024, p0 = min(pages, (int)threadIdx.x * per), p1 = min(pages, p0 + per);
   int live = 0;
+#pragma unroll 4
   for (int p = p0; p < p1; ++p) live += refs[p] > 0;
   int total;
-  block_prefix(live, sh, &total);
-  __syncthreads();
-  int high = 0, holes = 0;
-  for (int p = p0; p < p1; ++p) {
-    const bool l = refs[p] > 0;
-    high += l && p >= total;
-    holes += !l && p < total;
+  const int before = block_prefix(live, sh, &total);
+  if (p0 <= total && total < p1) {  // one thread, unless every page is live
+    int n = before;
+    for (int p = p0; p < total; ++p) n += refs[p] > 0;
+    sh_below = n;
   }
-  int count, same;
-  int hk = block_prefix(high, sh, &count);
+  if (total == pages && threadIdx.x == 0) sh_below = total;
   __syncthreads();
-  int ok = block_prefix(holes, sh, &same);
+  const int below = sh_below, count = total - below;
+  int n = before;
+#pragma unroll 4
   for (int p = p0; p < p1; ++p) {
     const int r = refs[p];
-    if (r > 0 && p >= total) moves[hk++].x = p;
-    if (r <= 0 && p < total) moves[ok++].y = p;
+    if (r > 0 && p >= total) {
+      moves[n - below].x = p;
+    } else {
+      where[p] = p;
+      if (r <= 0 && p < total)
+        moves[p - n].y = p;
+      else if (refs_out != refs)
+        refs_out[p] = r;
+    }
+    n += r > 0;
   }
   __syncthreads();  // the moves are visible to the CTA
-  if (refs_out != refs)
-    for (int p = threadIdx.x; p < pages; p += 1024) refs_out[p] = refs[p];
-  for (int p = threadIdx.x; p < pages; p += 1024) where[p] = p;
-  __syncthreads();
   for (int k = threadIdx.x; k < count; k += 1024) {
     const int2 m = moves[k];
     where[m.x] = m.y;
