@@ -60,7 +60,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
   grid_dependency_wait();
   grid_launch_dependents();
   const int i = threadIdx.x;
+  auto free_of = [&](int p0) {  // which of this thread's 4 pages from p0 on are free
+    unsigned b = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (p0 + 4 * i + k < st.pages && st.refs[p0 + 4 * i + k] == 0) b |= 1u << k;
+    return b;
+  };
   const int seq = i < n ? seqs[i] : -1;
+  const unsigned first_bits = free_of(0);  // asked for along with the requests
   named[i] = seq;
   __syncthreads();
   const int mask = (1 << st.page_shift) - 1;
@@ -104,10 +112,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
   int found = 0, rounds = 0, rank = 0;
   unsigned bits = 0;
   auto look = [&](int p0, int have) {  // free pages of this thread's 4, and their first's rank
-    bits = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (p0 + 4 * i + k < st.pages && st.refs[p0 + 4 * i + k] == 0) bits |= 1u << k;
+    bits = p0 ? free_of(p0) : first_bits;
     int got;
     __syncthreads();
     rank = have + block_prefix(__popc(bits), sh, &got);
