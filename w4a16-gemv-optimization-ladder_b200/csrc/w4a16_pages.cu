@@ -235,13 +235,14 @@ struct TableWork {
 
 // Copies whole pages of every layer, k and v: moves are pairs (src, dst), or two lists.  A pair
 // with an index outside [0, pages) is skipped.  Bound by the bytes, read once and written once:
-// a CTA takes one page of one layer and pool at a time, a thread kFlight 16-byte words in flight.
-// More CTAs than fit at once let the faster SMs take more (3.5 GB in all: 570 us, 0.96 of the copy
-// rate, with 32 for each SM, 649 with 4; a fixed number, since only the device knows how many
-// pages move).
+// a group of 32 to 256 threads (1 << lg) takes one page of one layer and pool at a time, a thread
+// kFlight 16-byte words in flight, so that small pages do not leave threads idle (60 forks in 24
+// layers with pages of 2 KB: 10.8 us with a call of free, 13.5 by 256 threads).  More CTAs than fit at once let the faster SMs
+// take more (3.5 GB in all: 566 us, 0.96 of the copy rate, with 32 for each SM, 649 with 4; a fixed
+// number, since only the device knows how many pages move).
+constexpr int kFlight = 8;
 __global__ void __launch_bounds__(256) k_pages_apply(const PageBlocks b, const int2* pairs, const int* src, const int* dst, int n,
-                                                     const int* count, const TableWork t) {
-  constexpr int kFlight = 8;
+                                                     const int* count, const int lg, const TableWork t) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int tid = threadIdx.x;
@@ -266,21 +267,24 @@ __global__ void __launch_bounds__(256) k_pages_apply(const PageBlocks b, const i
   if (count) n = min(n, *count);
   const long long items = 2LL * n * b.layers;
   const int words = (int)(b.page_bytes / 16);
-  for (long long e = blockIdx.x - t.ctas; e < items; e += gridDim.x - t.ctas) {
-    const int which = (int)(e & 1), layer = (int)((e >> 1) % b.layers), i = (int)((e >> 1) / b.layers);
+  const int group = 1 << lg, at = tid & (group - 1), groups = 256 >> lg;  // this thread's place in its group
+  const int step = (gridDim.x - t.ctas) * groups;
+  for (long long e = (int)((blockIdx.x - t.ctas) * groups + (tid >> lg)); e < items; e += step) {
+    const int which = (int)(e & 1), i = e >> 33 ? (int)((e >> 1) / b.layers) : (int)((uint32_t)(e >> 1) / (uint32_t)b.layers);
+    const int layer = (int)((e >> 1) - (long long)i * b.layers);
     const int f = pairs ? pairs[i].x : src[i], d = pairs ? pairs[i].y : dst[i];
     if (f < 0 || f >= b.pages || d < 0 || d >= b.pages || f == d) continue;
     uint8_t* base = static_cast<uint8_t*>(which ? b.v : b.k) + (size_t)layer * b.layer_stride;
     const uint4* from = reinterpret_cast<const uint4*>(base + (size_t)f * b.page_stride);
     uint4* to = reinterpret_cast<uint4*>(base + (size_t)d * b.page_stride);
-    for (int w0 = tid; w0 < words; w0 += 256 * kFlight) {
+    for (int w0 = at; w0 < words; w0 += group * kFlight) {
       uint4 x[kFlight];
 #pragma unroll
       for (int k = 0; k < kFlight; ++k)
-        if (w0 + 256 * k < words) x[k] = __ldcs(from + w0 + 256 * k);
+        if (w0 + group * k < words) x[k] = __ldcs(from + w0 + group * k);
 #pragma unroll
       for (int k = 0; k < kFlight; ++k)
-        if (w0 + 256 * k < words) __stcs(to + w0 + 256 * k, x[k]);
+        if (w0 + group * k < words) __stcs(to + w0 + group * k, x[k]);
     }
   }
 }
@@ -297,9 +301,11 @@ int launch_apply(const PageBlocks& b, const int2* pairs, const int* src, const i
   int sms = 0;
   const int rc = current_sm_count(&sms);
   if (rc != W4A16_OK) return rc;
-  const long long items = 2LL * n * b.layers, most = (long long)sms * 32;
-  return launched("k_pages_apply", launch_maybe_pdl(k_pages_apply, dim3((unsigned)(t.ctas + (items < most ? items : most))), dim3(256), 0,
-                                                    stream, true, b, pairs, src, dst, n, count, t));
+  int group = 32;
+  while (group < 256 && group * kFlight * 16LL < b.page_bytes) group *= 2;
+  const long long ctas = (2LL * n * b.layers + 256 / group - 1) / (256 / group), most = (long long)sms * 32;
+  return launched("k_pages_apply", launch_maybe_pdl(k_pages_apply, dim3((unsigned)(t.ctas + (ctas < most ? ctas : most))), dim3(256), 0,
+                                                    stream, true, b, pairs, src, dst, n, count, __builtin_ctz(group), t));
 }
 
 }  // namespace

@@ -69,9 +69,10 @@ def _pool(k_pages, v_pages):
                           sh if kv_heads > 1 else 8, st if page_size > 1 else 8), kv_heads, head_dim
 
 
-@functools.lru_cache(maxsize=64)
-def _attention_workspace(heads, kv_heads, head_dim):
-    return _lib.lib().w4a16_paged_attention_workspace_bytes(heads, kv_heads, head_dim)
+@functools.lru_cache(maxsize=256)
+def _bytes(name, *args):
+    """The scratch that a C entry asks for: a function of the sizes alone."""
+    return getattr(_lib.lib(), name)(*args)
 
 
 def _tables(tables, dev):
@@ -187,7 +188,7 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     if n == 0:
         return out
     if workspace is None:
-        size = _attention_workspace(heads, kvh, d)
+        size = _bytes("w4a16_paged_attention_workspace_bytes", heads, kvh, d)
         workspace = q.new_empty((size + 1) // 2)
     else:
         if not (isinstance(workspace, torch.Tensor) and workspace.device == dev and workspace.dtype == torch.uint8
@@ -268,7 +269,7 @@ def fork_sequences(k_pages, v_pages, tables, lengths, refs, src, dst):
     n = src.shape[0]
     t = _index(dst, n, "dst", dev)
     ok = torch.empty_like(src)
-    need = _lib.lib().w4a16_pages_fork_scratch_bytes(n)
+    need = _bytes("w4a16_pages_fork_scratch_bytes", n)
     scratch = src.new_empty((need + 3) // 4)
     _call("w4a16_pages_fork", dev, st, b, s, t, n, ok.data_ptr(), scratch.data_ptr(), need)
     return ok
@@ -308,7 +309,7 @@ def compact_pages(k_pages, v_pages, tables, refs, *, inplace=True):
     r = _index(refs, pages, "refs", dev)
     new_tables, new_refs = (tables, refs) if inplace else (torch.empty_like(tables), torch.empty_like(refs))
     moved = refs.new_empty(1)
-    need = _lib.lib().w4a16_pages_compact_scratch_bytes(pages)
+    need = _bytes("w4a16_pages_compact_scratch_bytes", pages)
     scratch = refs.new_empty((need + 3) // 4)
     _call("w4a16_pages_compact", dev, b, tables.data_ptr(), new_tables.data_ptr(), tables.numel(), r, new_refs.data_ptr(),
           moved.data_ptr(), scratch.data_ptr(), need)
