@@ -414,12 +414,17 @@ int w4a16_paged_append(const void* q, long long q_stride, const void* k, long lo
  * elements (multiples of 8) between rows, 16-byte aligned; heads a multiple of kv_heads.
  * Several rows may name one sequence (a prompt's tokens with growing lengths).  A length <= 0
  * gives zeros; a length past the tables, a sequence outside them or a page outside the pool
- * gives NaN.  scale is positive.  Scores, softmax and sums in fp32, rounded once.  workspace: w4a16_paged_attention_workspace_bytes bytes of
- * scratch, 16-byte aligned, whose content does not matter before or after the call; calls that
- * may overlap on the GPU need their own.  The length of each row is read on the device and the
+ * gives NaN.  scale is positive.  Scores, softmax and sums in fp32, rounded once.  workspace:
+ * w4a16_paged_attention_workspace_bytes bytes of scratch, 16-byte aligned, whose content does not
+ * matter before or after the call; calls that may overlap on the GPU need their own.  Calls of few
+ * rows in short tables take none and may be given null and 0: w4a16_paged_attention_call_bytes is
+ * what a call of this pool type, these sizes and tables of this width takes on the current device,
+ * 0 or all.  The length of each row is read on the device and the
  * rows' positions are shared out evenly over the GPU, so neither the tables' width nor unequal
  * lengths cost time. */
 size_t w4a16_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+size_t w4a16_paged_attention_call_bytes(int dtype, int rows, int heads, int kv_heads, int head_dim,
+                                        int width, int page_size);
 int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* lengths,
                           const int32_t* seqs, int rows, int heads, const w4a16_page_tables* tables,
                           const w4a16_page_pool* pool, float scale, void* out, long long out_stride,

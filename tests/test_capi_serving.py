@@ -53,6 +53,9 @@ def test_attention(lib):
     need = lib.w4a16_paged_attention_workspace_bytes(4, 2, 64)
     assert need > 0
     assert attention(lib, ws=None) == -1 and attention(lib, ws=P + 4) == -3 and attention(lib, wsb=need - 1) == -5
+    assert lib.w4a16_paged_attention_call_bytes(_lib.DTYPE_F16, 4, 4, 2, 64, 100000, 16) == need
+    for bad in ((0, 4, 4, 2, 64, 3, 16), (1, 0, 4, 2, 64, 3, 16), (1, 4, 3, 2, 64, 3, 16), (1, 4, 4, 2, 96, 3, 16), (1, 4, 4, 2, 64, 0, 16)):
+        assert lib.w4a16_paged_attention_call_bytes(*bad) == 0
     assert attention(lib, rows=0) == 0
     assert lib.w4a16_paged_attention_workspace_bytes(3, 2, 64) == 0
     assert lib.w4a16_last_error_string()

@@ -143,6 +143,28 @@ def test_attention_padded_batches(rows):
     assert not K.paged_attention(q, k, v, tables, torch.zeros(rows, dtype=torch.int32, device=DEV)).any()
 
 
+def test_attention_workspace_of_a_call():
+    # what a call takes is nothing or all; a smaller one than all is refused
+    from w4a16 import _lib
+
+    lens = [300, 7]
+    for width, heads in ((20, 8), (20, 32), (5000, 8)):
+        k, v, tables, _ = _cache(lens, 4, 16, 64, torch.float16)
+        wide = torch.full((2, width), -1, dtype=torch.int32, device=DEV)
+        wide[:, : tables.shape[1]] = tables
+        q = torch.randn(2, heads, 64, device=DEV).half()
+        n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        want = K.paged_attention(q, k, v, wide, n)
+        _check(want, q, k, v, wide, lens)
+        need = _lib.lib().w4a16_paged_attention_call_bytes(_lib.DTYPE_F16, 2, heads, 4, 64, width, 16)
+        full = _lib.lib().w4a16_paged_attention_workspace_bytes(heads, 4, 64)
+        assert need == (full if width == 5000 else 0)
+        assert torch.equal(K.paged_attention(q, k, v, wide, n, workspace=torch.empty(full, dtype=torch.uint8, device=DEV)), want)
+        small = torch.empty(16, dtype=torch.uint8, device=DEV)
+        with pytest.raises(RuntimeError):
+            K.paged_attention(q, k, v, wide, n, workspace=small)
+
+
 def test_attention_strides_and_scale():
     lens = [130, 77, 5]
     k, v, tables, _ = _cache(lens, 8, 16, 64, torch.float16, nhd=True)  # [pages, page_size, kv_heads, head_dim] storage

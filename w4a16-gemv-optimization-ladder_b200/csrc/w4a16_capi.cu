@@ -803,6 +803,15 @@ size_t w4a16_paged_attention_workspace_bytes(int heads, int kv_heads, int head_d
   return w4a16::paged_attention_workspace_bytes(heads, kv_heads, head_dim);
 }
 
+size_t w4a16_paged_attention_call_bytes(int dtype, int rows, int heads, int kv_heads, int head_dim, int width, int page_size) {
+  if ((dtype != W4A16_DTYPE_F16 && dtype != W4A16_DTYPE_BF16) || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256) || width <= 0 || page_size <= 0)
+    return 0;
+  return w4a16::paged_attention_needs_workspace(dtype, rows, heads, kv_heads, head_dim, (long long)width * page_size)
+             ? w4a16::paged_attention_workspace_bytes(heads, kv_heads, head_dim)
+             : 0;
+}
+
 int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* lengths,
                           const int32_t* seqs, int rows, int heads, const w4a16_page_tables* tables,
                           const w4a16_page_pool* pool, float scale, void* out, long long out_stride,
@@ -831,7 +840,9 @@ int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* leng
     set_error("q and out must be 16-byte aligned with strides of multiples of 8 elements, indices 4");
     return W4A16_ERR_ALIGN;
   }
-  rc = check_scratch(workspace, workspace_bytes, w4a16::paged_attention_workspace_bytes(heads, pl.kv_heads, pl.head_dim));
+  const bool none = !workspace && workspace_bytes == 0 &&
+                    w4a16_paged_attention_call_bytes(pl.dtype, rows, heads, pl.kv_heads, pl.head_dim, tb.width, 1 << pl.page_shift) == 0;
+  if (!none) rc = check_scratch(workspace, workspace_bytes, w4a16::paged_attention_workspace_bytes(heads, pl.kv_heads, pl.head_dim));
   if (rc != W4A16_OK) return rc;
   w4a16::PagedAttention a;
   a.q = q;

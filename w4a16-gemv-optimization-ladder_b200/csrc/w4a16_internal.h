@@ -168,6 +168,8 @@ struct PagedAttention {
 };
 int launch_paged_append(const PagedAppend& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream);
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+// whether a call on the current device takes it (cap: positions of a full table row)
+bool paged_attention_needs_workspace(int dtype, int rows, int heads, int kv_heads, int head_dim, long long cap);
 int launch_paged_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream);
 
 constexpr int kPagesMaxRequests = 1024;  // requests of one extend / fork call

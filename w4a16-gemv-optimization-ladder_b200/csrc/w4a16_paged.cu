@@ -1042,18 +1042,15 @@ int resident_clusters(int dev, int cluster) {
   return n - 1;
 }
 
+// CTAs that fill the current device, and those of the cluster that takes an item, 0 for a call that
+// is shared out in parts.  all: items; cap: positions of a full table row.
 template <typename T, int D, int NH>
-int launch_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream) {
+int plan_attention(long long all, long long cap, int* ctas, int* cluster) {
   using C = AttnCfg<D, NH>;
   int sms = 0;
   const int rc = current_sm_count(&sms);
   if (rc != W4A16_OK) return rc;
-  const int group = a.heads / pool.kv_heads, blocks = (group + C::kHeads - 1) / C::kHeads;
-  const int ctas = (sms < kAttnMaxSms ? sms : kAttnMaxSms) * C::kPerSm;
-  const bool coop = (long long)a.rows * pool.kv_heads * blocks < ctas * kAttnWarps;
-  const int workers = coop ? ctas : ctas * kAttnWarps;
-  // with far fewer items than CTAs a CTA has one at most, and the cost of beginning it is no matter of balance
-  const int cost = !coop ? kItemCost : (long long)a.rows * pool.kv_heads * blocks * 4 >= ctas ? kItemCostCta : 0;
+  *ctas = (sms < kAttnMaxSms ? sms : kAttnMaxSms) * C::kPerSm;
   static std::atomic<uint64_t> configured{0};  // one bit per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1064,15 +1061,29 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
     if (e == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev, std::memory_order_acq_rel);
   }
   if (e != cudaSuccess) return launched("configuring k_paged_attention,", e);
+  int n = kClusterMax;
+  while (n > 1 && (cap <= (long long)n / 2 * kClusterLeast || all > resident_clusters<T, D, NH>(dev, n))) n /= 2;
+  const bool few = all * n <= *ctas && cap <= (long long)n * cluster_most(D, NH, all * n * 2 >= *ctas);
+  *cluster = few || (all <= 2 * *ctas && cap <= kTwiceMost) ? n : 0;
+  return W4A16_OK;
+}
+
+template <typename T, int D, int NH>
+int launch_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream) {
+  using C = AttnCfg<D, NH>;
+  const int group = a.heads / pool.kv_heads, blocks = (group + C::kHeads - 1) / C::kHeads;
   const long long all = (long long)a.rows * pool.kv_heads * blocks;
-  const long long cap = (long long)tab.width << pool.page_shift;
-  int cluster = kClusterMax;
-  while (cluster > 1 && (cap <= (long long)cluster / 2 * kClusterLeast || all > resident_clusters<T, D, NH>(dev, cluster))) cluster /= 2;
-  const bool few = all * cluster <= ctas && cap <= (long long)cluster * cluster_most(D, NH, all * cluster * 2 >= ctas);
-  if (few || (all <= 2 * ctas && cap <= kTwiceMost)) {
+  int ctas = 0, cluster = 0;
+  const int rc = plan_attention<T, D, NH>(all, (long long)tab.width << pool.page_shift, &ctas, &cluster);
+  if (rc != W4A16_OK) return rc;
+  if (cluster) {
     ClusterLaunch<T, D, NH> l((unsigned)all, cluster, stream);
     return launched("k_paged_attention", cudaLaunchKernelEx(&l.cfg, k_paged_attention<T, D, NH, true>, a, pool, tab, group, blocks, true, 0, cluster, false));
   }
+  const bool coop = all < ctas * kAttnWarps;
+  const int workers = coop ? ctas : ctas * kAttnWarps;
+  // with far fewer items than CTAs a CTA has one at most, and the cost of beginning it is no matter of balance
+  const int cost = !coop ? kItemCost : all * 4 >= ctas ? kItemCostCta : 0;
   const bool many = coop && all * 8 < ctas;  // items few enough to be cut into many parts
   const int rc2 = launched("k_paged_attention", launch_maybe_pdl(k_paged_attention<T, D, NH, false>, dim3(ctas), dim3(kAttnWarps * 32), C::kSmem,
                                                                  stream, true, a, pool, tab, group, blocks, coop, cost, 1, many));
@@ -1084,7 +1095,26 @@ int launch_attention(const PagedAttention& a, const PagedPool& pool, const Paged
                                                    blocks));
 }
 
+template <typename F>
+int by_form(int dtype, int head_dim, int group, F&& f) {  // of the kernel: type, head_dim, 8 or 16 heads
+  return by_type(dtype, head_dim, [&](auto t, auto d) {
+    if constexpr (decltype(d)::value <= 128) {
+      if (attn_wide(group, head_dim)) return f(t, d, std::integral_constant<int, 2>());
+    }
+    return f(t, d, std::integral_constant<int, 1>());
+  });
+}
+
 }  // namespace
+
+bool paged_attention_needs_workspace(int dtype, int rows, int heads, int kv_heads, int head_dim, long long cap) {
+  int ctas = 0, cluster = 0;
+  const int rc = by_form(dtype, head_dim, heads / kv_heads, [&](auto t, auto d, auto nh) {
+    const int block = 8 * decltype(nh)::value, blocks = (heads / kv_heads + block - 1) / block;
+    return plan_attention<decltype(t), decltype(d)::value, decltype(nh)::value>((long long)rows * kv_heads * blocks, cap, &ctas, &cluster);
+  });
+  return rc != W4A16_OK || cluster == 0;
+}
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
   const size_t h = attn_wide(heads / kv_heads, head_dim) ? 16 : 8;
@@ -1092,14 +1122,8 @@ size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
 }
 
 int launch_paged_attention(const PagedAttention& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream) {
-  const bool wide = attn_wide(a.heads / pool.kv_heads, pool.head_dim);
-  return by_type(pool.dtype, pool.head_dim, [&](auto t, auto d) {
-    using T = decltype(t);
-    constexpr int D = decltype(d)::value;
-    if constexpr (D <= 128) {
-      if (wide) return launch_attention<T, D, 2>(a, pool, tab, stream);
-    }
-    return launch_attention<T, D, 1>(a, pool, tab, stream);
+  return by_form(pool.dtype, pool.head_dim, a.heads / pool.kv_heads, [&](auto t, auto d, auto nh) {
+    return launch_attention<decltype(t), decltype(d)::value, decltype(nh)::value>(a, pool, tab, stream);
   });
 }
 

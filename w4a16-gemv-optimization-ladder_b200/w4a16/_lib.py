@@ -113,6 +113,7 @@ SIGNATURES = {
     "w4a16_paged_append": ([_p, _ll, _p, _ll, _p, _ll, _p, _p, _i, _i, _p, _p, _p, _i, _p, _p, _ll, _p], _i),
     "w4a16_paged_attention": ([_p, _ll, _p, _p, _i, _i, _p, _p, ctypes.c_float, _p, _ll, _p, _sz, _p], _i),
     "w4a16_paged_attention_workspace_bytes": ([_i, _i, _i], _sz),
+    "w4a16_paged_attention_call_bytes": ([_i] * 7, _sz),
     "w4a16_pages_extend": ([_p, _p, _p, _i, _p, _p], _i),
     "w4a16_pages_fork": ([_p, _p, _p, _p, _i, _p, _p, _sz, _p], _i),
     "w4a16_pages_fork_scratch_bytes": ([_i], _sz),

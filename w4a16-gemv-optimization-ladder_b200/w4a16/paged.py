@@ -52,7 +52,7 @@ def _call(name, dev, *args):
 
 
 def _pool(k_pages, v_pages):
-    """One layer's pool, checked: its C description, kv_heads, head_dim."""
+    """One layer's pool, checked: its C description, kv_heads, page_size, head_dim."""
     dtype = _POOL_DTYPES.get(getattr(k_pages, "dtype", None))
     if dtype is None or k_pages.dim() != 4 or not k_pages.is_cuda:
         _refuse("k_pages must be an fp16 or bf16 CUDA tensor [pages, kv_heads, page_size, head_dim]")
@@ -66,13 +66,19 @@ def _pool(k_pages, v_pages):
         _refuse("the last dimension of the pages must be contiguous")
     # a dimension of one entry may carry any stride
     return _lib.pack_pool(k_pages.data_ptr(), v_pages.data_ptr(), dtype, pages, kv_heads, page_size, head_dim, sp if pages > 1 else 8,
-                          sh if kv_heads > 1 else 8, st if page_size > 1 else 8), kv_heads, head_dim
+                          sh if kv_heads > 1 else 8, st if page_size > 1 else 8), kv_heads, page_size, head_dim
 
 
 @functools.lru_cache(maxsize=256)
 def _bytes(name, *args):
     """The scratch that a C entry asks for: a function of the sizes alone."""
     return getattr(_lib.lib(), name)(*args)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_bytes(index, *args):
+    with torch.cuda.device(index):
+        return _lib.lib().w4a16_paged_attention_call_bytes(*args)
 
 
 def _tables(tables, dev):
@@ -82,7 +88,7 @@ def _tables(tables, dev):
     stride, one = tables.stride()
     if one != 1 and width > 1:
         _refuse("the rows of tables must be contiguous")
-    return _lib.pack_tables(tables.data_ptr(), sequences, width, stride)
+    return _lib.pack_tables(tables.data_ptr(), sequences, width, stride), width
 
 
 def _index(t, n, name, dev):
@@ -118,7 +124,7 @@ def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=
     Returns out.  A position past the tables' width or the angles, a sequence outside `tables` or a
     page outside the pool writes nothing to the cache and gives NaN.  A (sequence, position) may
     occur once per call."""
-    pool, kvh, d = _pool(k_pages, v_pages)
+    pool, kvh, _, d = _pool(k_pages, v_pages)
     dev, dtype = k_pages.device, k_pages.dtype
     if not (isinstance(k, torch.Tensor) and k.dim() == 3):
         _refuse("k must be [tokens, kv_heads, head_dim]")
@@ -127,7 +133,7 @@ def paged_append(q, k, v, positions, tables, k_pages, v_pages, *, cos=None, sin=
     vp, vs = _tokens(v, n, kvh, d, dtype, "v", dev)
     pos = _index(positions, n, "positions", dev)
     sq = _index(seqs, n, "seqs", dev) if seqs is not None else None
-    tab = _tables(tables, dev)
+    tab, _ = _tables(tables, dev)
     cp = sp = None
     angles = 0
     if cos is not None or sin is not None:
@@ -165,11 +171,11 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
              name one sequence, as the tokens of a prompt do with growing lengths
     scale    a positive number, default head_dim ** -0.5
     workspace  a uint8 CUDA tensor of at least w4a16_paged_attention_workspace_bytes; default: one
-             allocated for the call, so calls on several streams or in several graphs do not share it
+             allocated for a call that takes it, so calls on several streams or in several graphs do not share it
 
     Returns out [rows, heads, head_dim].  A row of length <= 0 is zero; a length past the tables'
     width, a sequence outside `tables` or a page outside the pool gives NaN."""
-    pool, kvh, d = _pool(k_pages, v_pages)
+    pool, kvh, page_size, d = _pool(k_pages, v_pages)
     dev, dtype = k_pages.device, k_pages.dtype
     if not (isinstance(q, torch.Tensor) and q.dim() == 3):
         _refuse("q must be [rows, heads, head_dim]")
@@ -179,7 +185,7 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
         _refuse(f"{heads} query heads are not a multiple of {kvh} kv heads")
     lens = _index(lengths, n, "lengths", dev)
     sq = _index(seqs, n, "seqs", dev) if seqs is not None else None
-    tab = _tables(tables, dev)
+    tab, width = _tables(tables, dev)
     if out is None:
         out = q.new_empty(n, heads, d)
         op, os_ = out.data_ptr(), heads * d
@@ -188,15 +194,16 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     if n == 0:
         return out
     if workspace is None:
-        size = _bytes("w4a16_paged_attention_workspace_bytes", heads, kvh, d)
-        workspace = q.new_empty((size + 1) // 2)
+        size = _attention_bytes(dev.index, _POOL_DTYPES[dtype], n, heads, kvh, d, width, page_size)
+        workspace = q.new_empty((size + 1) // 2) if size else None
+        ws = workspace.data_ptr() if size else None
     else:
         if not (isinstance(workspace, torch.Tensor) and workspace.device == dev and workspace.dtype == torch.uint8
                 and workspace.is_contiguous()):
             _refuse(f"workspace must be a contiguous uint8 tensor on {dev}")
-        size = workspace.numel()
+        size, ws = workspace.numel(), workspace.data_ptr()
     _call("w4a16_paged_attention", dev, qp, qs, lens, sq, n, heads, tab, pool, float(d ** -0.5 if scale is None else scale),
-          op, os_, workspace.data_ptr(), size)
+          op, os_, ws, size)
     return out
 
 
