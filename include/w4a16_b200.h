@@ -419,9 +419,10 @@ int w4a16_paged_append(const void* q, long long q_stride, const void* k, long lo
  * matter before or after the call; calls that may overlap on the GPU need their own.  Calls of few
  * rows in short tables take none and may be given null and 0: w4a16_paged_attention_call_bytes is
  * what a call of this pool type, these sizes and tables of this width takes on the current device,
- * 0 or all.  The length of each row is read on the device and the
- * rows' positions are shared out evenly over the GPU, so neither the tables' width nor unequal
- * lengths cost time. */
+ * 0 or all.  The length of each row is read on the device, and the positions of all rows are shared
+ * out evenly over the GPU (in calls of few rows in short tables, a row's over a cluster of its own),
+ * so neither the tables' width nor unequal lengths cost reads.  The same call gives the same bits
+ * every time; tables of another width may order the sums in another way. */
 size_t w4a16_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
 size_t w4a16_paged_attention_call_bytes(int dtype, int rows, int heads, int kv_heads, int head_dim,
                                         int width, int page_size);

@@ -177,7 +177,7 @@ def test_attention_strides_and_scale():
     assert not big[:, :4].any() and not big[:, 36:].any()
     padded = torch.full((3, tables.shape[1] + 500), -1, dtype=torch.int32, device=DEV)  # a much wider table
     padded[:, : tables.shape[1]] = tables
-    assert torch.equal(K.paged_attention(q, k, v, padded, lengths, scale=0.3), out)
+    _check(K.paged_attention(q, k, v, padded, lengths, scale=0.3), q, k, v, tables, lens, scale=0.3)  # sums in another order
     assert torch.equal(K.paged_attention(q, k, v, padded[:, : tables.shape[1] + 1], lengths, scale=0.3), out)  # rows apart
 
 

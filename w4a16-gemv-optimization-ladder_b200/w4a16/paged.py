@@ -173,7 +173,8 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     workspace  a uint8 CUDA tensor of at least w4a16_paged_attention_workspace_bytes; default: one
              allocated for a call that takes it, so calls on several streams or in several graphs do not share it
 
-    Returns out [rows, heads, head_dim].  A row of length <= 0 is zero; a length past the tables'
+    Returns out [rows, heads, head_dim], the same bits every time for tables of the same width (those of
+    few rows in short tables go a faster way).  A row of length <= 0 is zero; a length past the tables'
     width, a sequence outside `tables` or a page outside the pool gives NaN."""
     pool, kvh, page_size, d = _pool(k_pages, v_pages)
     dev, dtype = k_pages.device, k_pages.dtype
