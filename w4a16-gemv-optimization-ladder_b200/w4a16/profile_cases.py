@@ -18,6 +18,8 @@ times and synchronises; the first launch is the warm-up, so a capture takes
     g128_f32        one vector, 65536 x 2048 group-128, fp32 scales    (k_gemv_tma)
     g128_f16        the same with fp16 scales                           (k_gemv_tma)
     paged_attention 32 rows of up to 4096 positions, 32/8 heads of 128   (k_paged_attention, k_paged_join)
+    paged_attention_short  8 rows of 500 positions: one cluster an item  (k_paged_attention)
+    paged_attention_long   1 row of 100000 positions: parts of few items (k_paged_attention, k_paged_join_heads)
     paged_append    16384 tokens, 32/8 heads of 128                      (k_paged_append)
     compact         half of 1200 pages live, 16 layers                   (k_compact_plan, k_pages_apply)
     logits          64 rows of 128256, 2048 tokens each, mask            (k_process_logits)
@@ -130,6 +132,18 @@ def _cache(lengths, seed, layers=1, head_dim=128, spare=0):
 def case_paged_attention():
     c, _ = _cache([128 * (i + 1) for i in range(32)], 9)
     q = torch.randn(32, 32, 128, device="cuda").half()
+    _three(lambda: c.attention(0, q, c.lengths))
+
+
+def case_paged_attention_short():
+    c, _ = _cache([500] * 8, 9)
+    q = torch.randn(8, 32, 128, device="cuda").half()
+    _three(lambda: c.attention(0, q, c.lengths))
+
+
+def case_paged_attention_long():
+    c, _ = _cache([100000], 9)
+    q = torch.randn(1, 32, 128, device="cuda").half()
     _three(lambda: c.attention(0, q, c.lengths))
 
 
