@@ -238,6 +238,60 @@ def test_attention_bad_pages_give_nan_and_touch_nothing_else():
     assert torch.isnan(out[2:4]).all() and torch.equal(out[[0, 1, 4, 5]], want[[0, 1, 4, 5]])
 
 
+# Rows with a bad page, sequence or length between good ones, in each form of the call: a cluster for an
+# item; CTAs that take several items; warps; parts of few long items, joined by a CTA each and by heads.
+FORMS = [("cluster", 6, 2, 8, 64, torch.float16, 40), ("cluster", 3, 8, 32, 128, torch.bfloat16, 500), ("items", 400, 4, 8, 64, torch.float16, 64),
+         ("items", 32, 8, 32, 128, torch.bfloat16, 4096), ("items", 90, 4, 8, 256, torch.float16, 200), ("items", 100, 4, 64, 128, torch.float16, 300),
+         ("warps", 1500, 4, 4, 64, torch.bfloat16, 60), ("warps", 700, 4, 48, 128, torch.float16, 40), ("parts", 40, 4, 16, 64, torch.float16, 5000),
+         ("parts", 3, 4, 16, 128, torch.bfloat16, 30000), ("parts", 2, 1, 12, 64, torch.float16, 60000)]
+
+
+@pytest.mark.parametrize("form,rows,kv_heads,heads,head_dim,dtype,top", FORMS)
+def test_attention_bad_rows_leave_the_others_as_they_were(form, rows, kv_heads, heads, head_dim, dtype, top):
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(1, top + 1, (rows,), generator=g).tolist()
+    lens[1::3] = [1 + n % 20 for n in lens[1::3]]  # short rows behind long ones
+    lens[0] = top
+    if rows > 3:
+        lens[5::11] = [0] * len(lens[5::11])
+    broken = set(range(0, rows, 6)) if rows > 6 else {0}
+    k, v, tables, free = _cache(lens, kv_heads, 16, head_dim, dtype, seed=rows)
+    q = torch.randn(rows, heads, head_dim, device=DEV).to(dtype)
+    lengths, seqs = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (lens, list(range(rows))))
+    want = K.paged_attention(q, k, v, tables, lengths, seqs=seqs)
+    bad, other, hurt = tables.clone(), seqs.clone(), []
+    for i, r in enumerate(sorted(broken)):
+        pages = -(-lens[r] // 16)
+        if pages == 0:
+            continue
+        hurt.append(r)
+        if i % 4 == 0:
+            bad[r, pages - 1] = -1
+        elif i % 4 == 1:
+            bad[r, :pages] = k.shape[0]
+        elif i % 4 == 2:
+            bad[r, 0] = 2 ** 31 - 1
+        else:
+            other[r] = rows if i % 8 == 3 else -1
+    out = K.paged_attention(q, k, v, bad, lengths, seqs=other)
+    kept = torch.tensor([r not in hurt for r in range(rows)], device=DEV)
+    assert torch.isnan(out[~kept]).all() and torch.equal(out[kept], want[kept])
+    # lengths past the tables: where another table is one page wider, the same lengths are good ones
+    wide = torch.cat([tables, torch.full_like(tables[:, :1], int(free[0]))], 1)
+    wide[hurt] = torch.where(wide[hurt] < 0, free[0].int(), wide[hurt])
+    past = lengths.clone()
+    past[hurt] = tables.shape[1] * 16 + 1
+    want = K.paged_attention(q, k, v, wide, past)
+    assert not torch.isnan(want).any()
+    past[hurt[::2]] = 2 ** 31 - 1
+    out = K.paged_attention(q, k, v, wide[:, :-1], past)
+    assert torch.isnan(out[~kept]).all()
+    if form == "cluster":  # chosen by the tables' width
+        _check(out[kept], q[kept], k, v, tables[kept], [n for r, n in enumerate(lens) if r not in hurt])
+    else:
+        assert torch.equal(out[kept], want[kept])
+
+
 def test_attention_offsets_past_32_bits():
     # the last pages of a pool of more than 2^32 elements
     pages = 2 ** 32 // (8 * 64 * 128) + 8

@@ -435,11 +435,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
   unsigned bad = 0;  // bit: the stage holds a position without a page
   auto load = [&](int stage) {
     const uint32_t dst = ring + stage * 2 * C::kHalf;
-    if (pos >= ahead_len) {  // a unit without positions for this warp
+    bad = (bad & ~(1u << stage)) | (page == -2 ? 1u << stage : 0u);
+    if (pos >= ahead_len) {  // a unit without positions for this warp (and without a bad page)
       copies_commit();
       return;
     }
-    bad = (bad & ~(1u << stage)) | (page == -2 ? 1u << stage : 0u);
     const uint32_t here = dst + crow * (D * 2) + (chunk & ~7) * 16;
     auto to = [&](int r0) {  // where this lane's chunk of row r0 + crow goes (r0 a multiple of kRows)
       return here + r0 * (D * 2) + (((chunk & 7) ^ swizzle(r0 + crow)) * 16);
