@@ -219,6 +219,36 @@ def test_attention_garbage_outside_the_lengths_and_infinities_inside():
     assert torch.isfinite(big[:4]).all()
 
 
+@pytest.mark.parametrize("rows,kv_heads,n", [(1, 2, 500), (60, 4, 3000), (600, 4, 400), (2, 1, 60000)])
+@pytest.mark.parametrize("above", [10, 16, 20])
+@pytest.mark.parametrize("head_dim,dtype", [(64, torch.float16), (128, torch.float16), (64, torch.bfloat16)])
+def test_attention_one_key_far_above_a_long_tail(rows, kv_heads, n, above, head_dim, dtype):
+    """The first key scores about `above` over all others and its value is zero, so the result is what the
+    others leave.  With u half a step of the type the result is rounded once.  A score is off by less than
+    (head_dim / 16 + 16) steps of 2^-22 of sum |q k| * scale <= 32: 2^-12, in numerator and denominator:
+    2^-11; adding up n terms costs n * 2^-27 of sum p |v|; the parts of a probability leave out at most
+    2^-16 of it (bf16), or 2^-38 of the largest one (fp16), which is e^above of the others.  An fp16 result
+    below 2^-14 (e^-20 times 500 values of about 1.3 is 1.3e-6) is a multiple of 2^-24: rounded by up to 2^-25."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    heads = 2 * kv_heads
+    k, v, tables, _ = _cache([n] * rows, kv_heads, 16, head_dim, dtype, seed=n)
+    q = (torch.randn(rows, heads, head_dim, device=DEV, generator=g) * 0.1 + 1).to(dtype)
+    k.mul_(0.1)
+    v.copy_(v.abs() + 0.5)
+    first = tables[:, 0].long()
+    k[first, :, 0] = above * head_dim ** -0.5
+    v[first, :, 0] = 0
+    out = K.paged_attention(q, k, v, tables, torch.full((rows,), n, dtype=torch.int32, device=DEV))
+    for t in sorted({0, rows // 2, rows - 1}):
+        kk, vv = _sequence(k, tables[t], n), _sequence(v, tables[t], n)
+        s = torch.einsum("ghd,gnd->ghn", q[t].double().unflatten(0, (kv_heads, 2)), kk) * head_dim ** -0.5
+        p = torch.softmax(s, dim=2)
+        assert (s[:, :, 0] - s[:, :, 1:].amax(2) > above - 4).all()
+        ref = torch.einsum("ghn,gnd->ghd", p, vv).flatten(0, 1)  # every value is positive
+        lost = n * 2.0 ** -38 * vv.amax() + 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -16 * ref
+        assert ((out[t].double() - ref).abs() <= (HALF[dtype] + 2.0 ** -11 + n * 2.0 ** -27) * ref + lost).all()
+
+
 def test_attention_bad_pages_give_nan_and_touch_nothing_else():
     lens = [40, 40, 40, 40, 40, 40]
     k, v, tables, _ = _cache(lens, 2, 16, 64, torch.float16)

@@ -130,8 +130,8 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
 //   O^T[dimension][head] = V^T P   A = V^T: the lane reads 16 bytes (dimensions 8g) of positions
 //                                  2j, 2j+1, 2j+8, 2j+9 and pairs two positions with one byte
 //                                  permutation per word; P^T comes from S^T by 8 x 8 matrix
-//                                  transpositions, in two 16-bit parts (value and remainder), so
-//                                  that the probabilities lose nothing to the type
+//                                  transpositions, in two 16-bit parts (value and remainder) of
+//                                  kProb times the probability
 // The 16-byte chunks of a row are permuted by swizzle(row), which keeps both reads free of
 // bank conflicts.  The 8 (NH = 1) or 16 (NH = 2) query heads of a CTA are the n of the products.
 //
@@ -176,6 +176,12 @@ constexpr int cluster_most(int head_dim, int nh, bool fill) {
 // CTAs of an SM.  head_dim 64 has more to compute for a byte and wants more warps, with two
 // stages each (64 rows of up to 8000 positions: 86 us with 3 CTAs of 2 stages, 94 with 2 of 3).
 constexpr int attn_per_sm(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
+
+// What the probabilities, their sums and the products with V carry until the last division.  fp16's
+// smallest step is 2^-24: a probability as it is would lose what lies below 2^-25 of the warp's largest one,
+// with 2^14 (the largest is 2^14, of 65504) what lies below 2^-39.  bf16 has fp32's exponents.
+template <typename T>
+constexpr float kProb = std::is_same<T, __half>::value ? 16384.f : 1.f;
 
 template <int D, int NH>
 struct AttnCfg {
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
         for (int t = 0; t < kU; ++t) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            s[n][t][c] = exp2_fast(fmaf(s[n][t][c], scale, -low[c & 1]));
+            s[n][t][c] = exp2_fast(fmaf(s[n][t][c], scale, -low[c & 1])) * kProb<T>;
             l[n][c & 1] += s[n][t][c];
           }
 #pragma unroll
