@@ -249,6 +249,23 @@ def test_attention_one_key_far_above_a_long_tail(rows, kv_heads, n, above, head_
         assert ((out[t].double() - ref).abs() <= (HALF[dtype] + 2.0 ** -11 + n * 2.0 ** -27) * ref + lost).all()
 
 
+@pytest.mark.parametrize("heads,head_dim", [(1, 64), (16, 64), (1, 128), (9, 128), (1, 256)])
+def test_attention_long_sums_have_no_bias(heads, head_dim):
+    """Values of 1, so the result is 1 whatever the probabilities; many rows of one long sequence, so that a warp
+    adds up thousands of tiles.  The result is rounded once (2^-12 below 1).  A sum of N tiles rounded to nearest
+    is off by errors of no preferred sign, each below 2^-24 of it: 8 sqrt(N) 2^-24 is past any chance; the parts of
+    the probabilities leave out 2^-22."""
+    n, rows = 2 ** 24 // head_dim, 1200
+    g = torch.Generator(device=DEV).manual_seed(heads)
+    k = torch.randn(n // 256, 1, 256, head_dim, device=DEV, generator=g).half()
+    v = torch.ones_like(k)
+    q = torch.randn(rows, heads, head_dim, device=DEV, generator=g).half()
+    tables = torch.arange(n // 256, dtype=torch.int32, device=DEV)[None]
+    lengths = torch.full((rows,), n, dtype=torch.int32, device=DEV)
+    out = K.paged_attention(q, k, v, tables, lengths, seqs=torch.zeros_like(lengths))
+    assert ((out.double() - 1).abs() <= 2.0 ** -12 + 8 * (n / 16) ** 0.5 * 2.0 ** -24 + 2.0 ** -22).all()
+
+
 def test_attention_bad_pages_give_nan_and_touch_nothing_else():
     lens = [40, 40, 40, 40, 40, 40]
     k, v, tables, _ = _cache(lens, 2, 16, 64, torch.float16)

@@ -132,6 +132,10 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
 //                                  permutation per word; P^T comes from S^T by 8 x 8 matrix
 //                                  transpositions, in two 16-bit parts (value and remainder) of
 //                                  kProb times the probability
+// A tile's part of O starts from zero and is added to the running sum by an ordinary addition: the
+// products' own additions cut off what is below the sum's last bit, always towards zero (values of
+// 1 over 262144 positions in a warp gave 0.9985 as one long sum; 16 heads of a CTA pay 3% for the
+// additions, 64 rows of up to 2000 with 8 kv heads of 128 65.5 us for 63.7, 8 heads under 1%).
 // The 16-byte chunks of a row are permuted by swizzle(row), which keeps both reads free of
 // bank conflicts.  The 8 (NH = 1) or 16 (NH = 2) query heads of a CTA are the n of the products.
 //
@@ -627,8 +631,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnCfg<D, NH>::kPerSm)
             const uint32_t a2 = prmt(w[2][i], w[3][i], 0x5410u), a3 = prmt(w[2][i], w[3][i], 0x7632u);
 #pragma unroll
             for (int n = 0; n < NH; ++n) {
-              mma16816<T>(o[n][b * 4 + i], a0, a1, a2, a3, ph[n][t][0], ph[n][t][1]);
-              mma16816<T>(o[n][b * 4 + i], a0, a1, a2, a3, pl[n][t][0], pl[n][t][1]);
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816<T>(d, a0, a1, a2, a3, ph[n][t][0], ph[n][t][1]);
+              mma16816<T>(d, a0, a1, a2, a3, pl[n][t][0], pl[n][t][1]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[n][b * 4 + i][c] += d[c];
             }
           }
         }
