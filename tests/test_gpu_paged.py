@@ -266,6 +266,33 @@ def test_attention_long_sums_have_no_bias(heads, head_dim):
     assert ((out.double() - 1).abs() <= 2.0 ** -12 + 8 * (n / 16) ** 0.5 * 2.0 ** -24 + 2.0 ** -22).all()
 
 
+@pytest.mark.parametrize("head_dim,dtype", [(64, torch.float16), (64, torch.bfloat16), (128, torch.bfloat16), (256, torch.bfloat16)])
+@pytest.mark.parametrize("rows,group", [(60, 1), (60, 12), (900, 4)])
+def test_attention_takes_both_parts_of_a_probability(rows, group, head_dim, dtype):
+    """Three keys: two of score 0 with the values -h and -l, the type's nearest to x = e^s and to x - h, and
+    one of score s < 0 with the value 1.  So the result is (x - h - l) / (2 + x), which two parts of the type
+    leave of x: with b bits 2^-(2b + 1) of it (bf16 2^-17, fp16 2^-23), and one part 2^-b.  s is exact (one dimension of
+    q is 1, the others 0); the exponential is off by 2^-22 and by the two roundings of its argument, below
+    1.5 * 2^-24; adding up terms below 1 in fp32 costs less than 2^-23 each, of at most 9."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    k = torch.zeros(rows, 1, 16, head_dim, dtype=dtype, device=DEV)
+    v = torch.zeros_like(k)
+    s = -(torch.rand(rows, device=DEV, generator=g) * 0.9 + 0.1).to(dtype)
+    x = s.double().exp()
+    h = x.to(dtype)
+    low = (x - h.double()).to(dtype)
+    k[:, 0, 2, 0] = s
+    v[:, 0, 0], v[:, 0, 1], v[:, 0, 2] = -h[:, None], -low[:, None], 1
+    q = torch.zeros(rows, group, head_dim, dtype=dtype, device=DEV)
+    q[:, :, 0] = 1
+    tables = torch.arange(rows, dtype=torch.int32, device=DEV)[:, None]
+    out = K.paged_attention(q, k, v, tables, torch.full((rows,), 3, dtype=torch.int32, device=DEV), scale=1.0)
+    ref = ((x - h.double() - low.double()) / (2 + x))[:, None, None]
+    lost = 2.0 ** -23 if dtype == torch.float16 else 2.0 ** -17
+    tol = HALF[dtype] * ref.abs() + (2.0 ** -22 + 1.5 * 2.0 ** -24 + 9 * 2.0 ** -23 + lost) / 2 + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert ((out.double() - ref).abs() <= tol).all()
+
+
 def test_attention_bad_pages_give_nan_and_touch_nothing_else():
     lens = [40, 40, 40, 40, 40, 40]
     k, v, tables, _ = _cache(lens, 2, 16, 64, torch.float16)

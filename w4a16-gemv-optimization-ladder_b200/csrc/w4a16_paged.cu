@@ -131,7 +131,11 @@ __global__ void __launch_bounds__(append_threads<D>(), 1024 / append_threads<D>(
 //                                  2j, 2j+1, 2j+8, 2j+9 and pairs two positions with one byte
 //                                  permutation per word; P^T comes from S^T by 8 x 8 matrix
 //                                  transpositions, in two 16-bit parts (value and remainder) of
-//                                  kProb times the probability
+//                                  kProb times the probability: fp16's 11 bits leave 2^-23 of it,
+//                                  bf16's 8 leave 2^-17, 2^-8 of the rounding of the result.  (With
+//                                  a third part for bf16 one value in 2000 was not the nearest bf16,
+//                                  with two one in 900, of 2 rows of up to 120001; it took 1% more
+//                                  time there and 5% with 16 heads, 64 rows of up to 2000.)
 // A tile's part of O starts from zero and is added to the running sum by an ordinary addition: the
 // products' own additions cut off what is below the sum's last bit, always towards zero (values of
 // 1 over 262144 positions in a warp gave 0.9985 as one long sum; 16 heads of a CTA pay 3% for the
