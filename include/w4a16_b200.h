@@ -499,8 +499,8 @@ int w4a16_pages_compact(const w4a16_page_blocks* blocks, const int32_t* tables, 
  *   x = x + bias[v] + the values of the row's pairs (bias_ids, bias_values) with id v
  *   bit v % 32 of mask[b][v / 32] is 0:       x = -inf
  * NULL leaves a part out (total_lens NULL: all `history` tokens; prompt_lens NULL: no prompt).
- * Tokens and ids outside [0, vocab) are skipped; lengths are clamped to [0, history].  The
- * division is a product with 1 / repetition. */
+ * Tokens and ids outside [0, vocab) are skipped; lengths are clamped to [0, history].  A
+ * repetition between 2^-126 and 2^100 divides with one rounding (past them with more). */
 typedef struct {
   const void* logits;       /* [rows][vocab], row stride `stride` elements */
   void* out;                /* the same layout by out_stride; may be logits itself */

@@ -182,6 +182,27 @@ def test_same_bits_every_time_and_in_a_graph():
     _check(out, logits, extra=24, **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 5003), (130, 10007)])
+def test_repetition_divides(dtype, rows, vocab):
+    """The nearest quotient, but where it lies within 2^-22 of a step of the middle of two neighbours (1 / repetition
+    is known to 2^-47): there the other neighbour, which for 16-bit logits rounds to one step of the type at most."""
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    logits = (torch.randn(rows, vocab, device=DEV, generator=g) * 5).to(dtype)
+    logits[0, :4] = torch.tensor([0.0, -0.0, float("inf"), float("-inf")])
+    tokens = torch.arange(vocab, device=DEV, dtype=torch.int32).repeat(rows, 1)
+    for scale in (1.0, 2.0 ** -126, 2.0 ** 99):  # the ends of the range
+        r = (torch.rand(rows, device=DEV, generator=g) + (0.7 if scale == 1 else 1.0)) * scale
+        r[rows // 2] = 1.1 * scale
+        out = K.process_logits(logits, tokens=tokens, repetition=r)
+        x = logits.float()
+        want = torch.where(x > 0, x / r[:, None], x * r[:, None]).to(dtype)
+        other = out != want
+        assert other.float().mean() <= 4 * 2.0 ** -22 + 1 / other.numel()
+        u = 2 * HALF[dtype]
+        assert ((out.double() - want.double())[other].abs() <= u * want.double()[other].abs()).all()
+
+
 def test_refusals_on_the_host():
     logits, kw = _inputs(3, 100, 10, torch.float32)
     t = kw["tokens"]

@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
     for (int i = tid; i <= ((v1 - 1) >> 5) - first_word; i += kThreads)
       allowed[i] = (uint32_t)fetch(p.mask + (size_t)row * p.mask_stride + first_word + i);
   const float rep = p.repetition ? fetch(p.repetition + row) : 1.f, inv_rep = 1.f / rep;
+  const float inv_rest = fmaf(-rep, inv_rep, 1.f) * inv_rep;  // inv_rep + inv_rest is 1 / rep to 2^-47
   const float freq = p.frequency ? fetch(p.frequency + row) : 0.f;
   const float pres = p.presence ? fetch(p.presence + row) : 0.f;
 
@@ -186,8 +187,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) k_process_l
   if (marks || p.mask) __syncthreads();
   const float* bias = p.bias ? p.bias + (size_t)row * p.bias_stride : nullptr;
   auto penalised = [&](float x, uint32_t w) {
-    const float by = x > 0.f ? inv_rep : rep, n = (float)(w & kCount);
-    x = w & (kSeen | kCount) ? x * by : x;
+    // x / rep as the sum of two products, rounded once (64 rows with 64 pairs, histories and a mask: 20.7 us, with a
+    // division 23.5); of an infinity one of them is NaN, and the other the quotient
+    const float q = x * inv_rep, z = fmaf(x, inv_rep, x * inv_rest), n = (float)(w & kCount);
+    const float y = x > 0.f ? (z == z ? z : q) : x * rep;
+    x = w & (kSeen | kCount) ? y : x;
     return w & kCount ? x - freq * n - pres : x;
   };
   const bool wide_out = reinterpret_cast<uintptr_t>(out + v0) % 16 == 0, wide_bias = reinterpret_cast<uintptr_t>(bias + v0) % 16 == 0;

@@ -42,7 +42,7 @@ def process_logits(logits, *, tokens=None, prompt_lens=None, total_lens=None, re
     tokens       int32 or int64 [rows, history]: prompt, then generated tokens; ids outside the
                  vocabulary (padding) are skipped
     prompt_lens, total_lens  int32 [rows] (default 0 and history; clamped to history)
-    repetition, frequency, presence  fp32 [rows], each optional
+    repetition, frequency, presence  fp32 [rows], each optional; a repetition lies between 2^-126 and 2^100
     bias         fp32 [vocab] or [rows, vocab]
     bias_ids, bias_values  int32 and fp32 [rows, pairs]; an id outside the vocabulary is skipped, the
                  values of an id named twice are added in their order
