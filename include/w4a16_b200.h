@@ -464,8 +464,8 @@ typedef struct {
  * free: 0..65536), served in order; all of them see the state from before the call.  ok[i] (int32) is 1, or 0 for a
  * request that was refused and changed nothing: an index out of range, a negative count, more
  * positions than the table row holds, the same seqs / dst index as an earlier request, a dst
- * that is not empty or equals its src, or, from the first request on that no longer fits the free pages, every
- * request that needs one.  scratch: w4a16_pages_fork_scratch_bytes(n), 16-byte aligned. */
+ * that is not empty or equals its src, a src whose partly filled page is none of the pool, or, from the
+ * first request on that no longer fits the free pages, every request that needs one.  scratch: w4a16_pages_fork_scratch_bytes(n), 16-byte aligned. */
 int w4a16_pages_extend(const w4a16_page_state* state, const int32_t* seqs, const int32_t* counts,
                        int n, int32_t* ok, w4a16_stream_t stream);
 size_t w4a16_pages_fork_scratch_bytes(int n);

@@ -140,6 +140,24 @@ def test_random_life(sequences, width, pages, page_size, seed):
         model.check(cache)
 
 
+@pytest.mark.parametrize("page_size", [2, 16])
+def test_fork_of_a_sequence_whose_last_page_is_bad_is_refused(page_size):
+    # there is nothing to copy: a child with a free page's old contents would answer in earnest
+    cache, model = _pair(8, 4, 30, page_size)
+    n = 3 * page_size - 1
+    for x in (cache, model):
+        x.extend(*((_i32([0, 1, 2]), _i32([n] * 3)) if x is cache else ([0, 1, 2], [n] * 3)))
+    for entry in (-1, 30, 2 ** 31 - 1):
+        cache.tables[1, 2] = entry
+        before = [t.clone() for t in (cache.tables, cache.lengths, cache.refs, cache.k, cache.v)]
+        assert cache.fork(_i32([1, 1]), _i32([4, 5])).tolist() == [0, 0]
+        assert all(torch.equal(a, b) for a, b in zip(before, (cache.tables, cache.lengths, cache.refs, cache.k, cache.v)))
+    assert cache.fork(_i32([1, 0, 1, 2]), _i32([4, 5, 6, 7])).tolist() == [0, 1, 0, 1]  # the others' pages are as if it were not there
+    model.fork([0, 2], [5, 7])
+    cache.tables[1, 2] = model.tables[1][2]
+    model.check(cache)
+
+
 def test_requests_past_the_free_pages_are_refused_in_order():
     cache, model = _pair(6, 4, 5, 16)
     seqs, counts = [0, 1, 2, 3, 4], [33, 16, 17, 0, 1]  # 3 + 1 pages, then 2 do not fit, 0 needed, 1 would

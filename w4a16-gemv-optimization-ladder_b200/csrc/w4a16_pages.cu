@@ -51,12 +51,12 @@ __device__ __forceinline__ int block_prefix(int v, int* sh, int* total) {
 // Serves the requests of one call in order.  extend (src == nullptr): sequence seqs[i] grows by
 // counts[i] positions.  fork: seqs[i] (empty) becomes a copy of src[i]; it needs a page of its
 // own for src's partly filled one.  Request i is refused (ok 0, nothing changed) when its
-// arguments are out of range, when an earlier request names the same seqs[i], or when the
-// free pages do not suffice for all requests up to it.
+// arguments are out of range, when an earlier request names the same seqs[i], when the page that a fork
+// would copy is none of the pool, or when the free pages do not suffice for all requests up to it.
 __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st, const int* seqs,
                                                              const int* src, const int* counts,
                                                              int n, int* ok, int2* moves) {
-  __shared__ int sh[33], named[kPlanThreads], cum[kPlanThreads], first[kPlanThreads];
+  __shared__ int sh[33], named[kPlanThreads], cum[kPlanThreads], first[kPlanThreads], copied[kPlanThreads];
   grid_dependency_wait();
   grid_launch_dependents();
   const int i = threadIdx.x;
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
 #pragma unroll 8
     for (int j = 0; j < i; ++j) valid &= named[j] != seq;
   }
-  int need = 0, length = 0, from = 0, grown = 0;
+  int need = 0, length = 0, from = 0, grown = 0, last = -1;
   if (valid) {
     length = st.lengths[seq];
     if (src) {
@@ -89,6 +89,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
         valid = grown >= 0 && grown <= cap;
         need = valid && (grown & mask) ? 1 : 0;
         length = grown & ~mask;  // the first position that needs a page of its own
+        if (need) {
+          last = st.tables[(size_t)from * st.table_stride + (length >> st.page_shift)];  // the page to be copied
+          valid = last >= 0 && last < st.pages;
+        }
       }
     } else {
       const int c = counts[i];
@@ -103,6 +107,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
   int wanted;
   const int before = block_prefix(need, sh, &wanted);
   cum[i] = before + need;
+  copied[i] = last;
   first[i] = (int)(((long long)length + mask) >> st.page_shift);  // table column of the request's first new page
   __syncthreads();
   // the lowest free pages, as many as are wanted, 4 for a thread at a time: rank -> request ->
@@ -133,7 +138,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(const PagesState st
       if (cum[lo] <= found) {
         const int p = r * kRound + 4 * i + k, nth = rank - (lo ? cum[lo - 1] : 0);
         st.refs[p] = 1;
-        if (moves) moves[lo] = make_int2(st.tables[(size_t)src[lo] * st.table_stride + first[lo]], p);
+        if (moves) moves[lo] = make_int2(copied[lo], p);
         st.tables[(size_t)named[lo] * st.table_stride + first[lo] + nth] = p;
       }
       ++rank;

@@ -267,7 +267,8 @@ def fork_sequences(k_pages, v_pages, tables, lengths, refs, src, dst):
     k_pages, v_pages: [layers, pages, kv_heads, page_size, head_dim] (or one layer's four dimensions).
 
     Returns ok, int32 [n], as extend_sequences does; a dst that is not empty, is its own src or was
-    named by an earlier request is refused.  All requests see the state from before the call."""
+    named by an earlier request is refused, and so is a src whose partly filled page is outside the
+    pool.  All requests see the state from before the call."""
     b, pages = _blocks(k_pages, v_pages)
     st = _state(tables, lengths, refs, k_pages.shape[-2])
     dev = tables.device
