@@ -85,6 +85,23 @@ def test_any_number_of_tokens(kw):
         _near(got[0], want)
 
 
+@pytest.mark.parametrize("kw,n", [(dict(), 6), (dict(dense=True), 6), (dict(), 70)], ids=["int4", "dense", "gemm"])
+def test_tokens_outside_the_vocabulary(kw, n):
+    """Of padding they are nobody's; of a real position they give NaN in their own sequence."""
+    dec = _decoder(**kw)
+    cache, clean = _cache(dec), _cache(dec)
+    for c in (cache, clean):
+        assert c.extend(_i32([0, 1]), _i32([2, 2])).tolist() == [1, 1]
+    seqs, at = _i32([0, 0, 1] + [0] * (n - 3)), _i32([0, 1, 0] + [-1] * (n - 3))
+    want = dec.step_paged(torch.tensor([5, 6, 7] + [0] * (n - 3), device=DEV), seqs, at, clean)
+    pad = ([-1, 4096, 2 ** 62, -2 ** 63] * n)[:n - 3]
+    out = dec.step_paged(torch.tensor([5, 6, 7] + pad, device=DEV), seqs, at, cache)
+    assert torch.equal(out[:3], want[:3]) and torch.equal(cache.k, clean.k) and torch.equal(cache.v, clean.v)
+    for bad in (-1, 4096):
+        out = dec.step_paged(torch.tensor([5, bad, 7] + pad, device=DEV), seqs, at, cache)
+        assert torch.equal(out[[0, 2]], want[[0, 2]]) and torch.isnan(out[1]).all()
+
+
 def test_fork_free_and_compact_change_no_result():
     dec = _decoder()
     cache, plain = _cache(dec), _cache(dec)

@@ -410,15 +410,16 @@ class W4A16LlamaDecoder:
         """Logits (fp32 [T, vocab]) of T tokens of any sequences of a paged cache, prompts' tokens and
         single new ones mixed: token t (tokens int64 [T]) is position positions[t] (int32) of sequence
         seqs[t] (int32), for which cache.extend has made room, and attends to the positions up to
-        its own.  A negative position is padding.  cache: a PagedKVCache of this model's layers,
-        kv heads and head_dim, in fp16."""
+        its own.  A negative position is padding, whose token may be any number; a real token outside the
+        vocabulary gives NaN.  cache: a PagedKVCache of this model's layers, kv heads and head_dim, in fp16."""
         cfg, D = self.cfg, self.cfg.head_dim
         if cache.k.dtype != torch.float16 or tuple(cache.k.shape[i] for i in (0, 2, 4)) != (cfg.layers, cfg.kv_heads, D):
             raise ValueError(f"the cache must be fp16 with {cfg.layers} layers, {cfg.kv_heads} kv heads and head_dim {D}")
         if tokens.numel() == 0:
             return self.embed.new_empty((0, cfg.vocab), dtype=torch.float32)
         lengths = positions + 1
-        h = self.embed.index_select(0, tokens).float()
+        outside = ((tokens < 0) | (tokens >= cfg.vocab)) & (positions >= 0)
+        h = self.embed.index_select(0, tokens.clamp(0, cfg.vocab - 1)).float().masked_fill_(outside[:, None], float("nan"))
 
         def norm(w):
             return (h * torch.rsqrt(h.pow(2).mean(1, keepdim=True) + cfg.eps) * w).half()
