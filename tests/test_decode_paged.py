@@ -159,6 +159,39 @@ def test_decode_step_in_a_graph_with_the_cache_growing():
     assert torch.equal(cache.tables, eager.tables) and torch.equal(cache.refs, eager.refs)
 
 
+def test_a_captured_step_keeps_its_workspaces_when_larger_steps_follow(monkeypatch):
+    """The products' split-K workspaces grow with the number of tokens.  A graph captured before holds the addresses of
+    the smaller ones, which must not go back to the allocator."""
+    from w4a16 import kernels
+
+    for name, empty in (("_WORKSPACE", {}), ("_GEMM_WS", {}), ("_OUTGROWN", [])):
+        monkeypatch.setattr(kernels, name, empty)
+    dec = _decoder()
+    graphs = []
+    for n in (2, 5, 65, 200):
+        cache = _cache(dec)
+        cache.extend(_i32([1]), _i32([150]))
+        args = torch.arange(n, device=DEV), _i32([1] * n), _i32([i if i < 150 else -1 for i in range(n)]), cache
+        want = dec.step_paged(*args)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = dec.step_paged(*args)
+        used = list(kernels._WORKSPACE.values()) + list(kernels._GEMM_WS.values())
+        graphs.append((graph, out, want, used, args))
+    held = {b.data_ptr() for b in list(kernels._WORKSPACE.values()) + list(kernels._GEMM_WS.values()) + kernels._OUTGROWN}
+    assert len(kernels._OUTGROWN) >= 1
+    for _, _, _, used, _ in graphs:
+        assert {b.data_ptr() for b in used} <= held
+    sizes = sum(b.numel() for b in kernels._OUTGROWN)
+    assert sizes <= sum(b.numel() for b in list(kernels._WORKSPACE.values()) + list(kernels._GEMM_WS.values()))
+    del used
+    junk = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=DEV) for _ in range(64)]
+    for graph, out, want, _, _ in graphs:
+        graph.replay()
+        assert torch.equal(out, want)
+    assert len(junk) == 64
+
+
 def test_step_paged_refuses_another_models_cache():
     import w4a16 as K
 

@@ -68,6 +68,7 @@ def _check_vec(vec, cols, device):
 # ------------------------------------------------------------------ workspace
 
 _WORKSPACE = {}
+_OUTGROWN = []  # smaller workspaces that larger ones took the place of: captured graphs still use them
 
 
 def _workspace(device, batch, rows, cols):
@@ -81,6 +82,9 @@ def _workspace(device, batch, rows, cols):
     if buf is None or buf.numel() < need:
         if torch.cuda.is_current_stream_capturing():
             return buf
+        if buf is not None:
+            _OUTGROWN.append(buf)
+            need = max(need, 2 * buf.numel())  # all of them together stay below the newest
         buf = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=device)
         _WORKSPACE[key] = buf
     return buf
@@ -396,6 +400,9 @@ def _gemm_workspace(dev, m, n, k):
     if ws is None or ws.numel() < need:
         if torch.cuda.is_current_stream_capturing():
             return None  # no allocation during capture: that call runs unsplit
+        if ws is not None:
+            _OUTGROWN.append(ws)
+            need = max(need, 2 * ws.numel())
         ws = torch.zeros(need, dtype=torch.uint8, device=dev)
         _GEMM_WS[dev] = ws
     return ws
@@ -481,7 +488,7 @@ def read_device_error(device=None):
         _lib.check(_lib.lib().w4a16_read_device_error(ctypes.byref(code), _stream(dev)),
                    "w4a16_read_device_error")
         if code.value:
-            for buf in (_WORKSPACE.get(dev.index), _GEMM_WS.get(dev)):
-                if buf is not None:
+            for buf in (_WORKSPACE.get(dev.index), _GEMM_WS.get(dev), *_OUTGROWN):
+                if buf is not None and buf.device == dev:
                     buf.zero_()
     return code.value
