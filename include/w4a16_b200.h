@@ -414,7 +414,7 @@ int w4a16_paged_append(const void* q, long long q_stride, const void* k, long lo
  * elements (multiples of 8) between rows, 16-byte aligned; heads a multiple of kv_heads.
  * Several rows may name one sequence (a prompt's tokens with growing lengths).  A length <= 0
  * gives zeros; a length past the tables, a sequence outside them or a page outside the pool
- * gives NaN.  scale is positive.  Scores, softmax and sums in fp32, rounded once; a probability
+ * gives NaN.  scale is positive, at most 2^127.  Scores, softmax and sums in fp32, rounded once; a probability
  * enters the product with V as two values of the pool's type, which leave out at most 2^-23 (fp16)
  * or 2^-17 (bf16) of it and, in fp16, what is below 2^-39 of the largest one.  workspace:
  * w4a16_paged_attention_workspace_bytes bytes of scratch, 16-byte aligned, whose content does not

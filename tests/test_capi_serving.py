@@ -61,6 +61,13 @@ def test_attention(lib):
     assert lib.w4a16_last_error_string()
 
 
+def test_attention_scale_times_log2_e_is_a_number(lib):
+    # the kernel's exponentials are powers of two: 2.5e38 * log2(e) is past fp32, and infinity times a score of 0 NaN
+    for scale in (2.4e38, 3e38, 3.4e38):
+        assert attention(lib, scale=scale) == -2, scale
+    assert attention(lib, scale=2.0 ** 127, rows=0) == 0 and attention(lib, scale=2.0 ** -149, rows=0) == 0
+
+
 def test_append(lib):
     for change, status in BAD_POOLS:
         assert append(lib, p=pool(**change)) == status, change

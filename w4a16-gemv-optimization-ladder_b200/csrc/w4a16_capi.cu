@@ -826,8 +826,8 @@ int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* leng
               pl.kv_heads, tb.width);
     return W4A16_ERR_SHAPE;
   }
-  if (!(scale > 0.f) || scale > 3e38f) {
-    set_error("scale %g is not a positive number", scale);
+  if (!(scale > 0.f) || scale > 0x1p127f) {  // times log2(e) it has to stay a number
+    set_error("scale %g is not a positive number up to 2^127", scale);
     return W4A16_ERR_SHAPE;
   }
   if (rows == 0) return W4A16_OK;

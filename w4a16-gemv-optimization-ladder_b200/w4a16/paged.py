@@ -169,7 +169,7 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     lengths  int32 [rows]: positions each row attends to, its own token's included
     seqs     int32 [rows]: each row's row of `tables` (default: row t is sequence t); several rows may
              name one sequence, as the tokens of a prompt do with growing lengths
-    scale    a positive number, default head_dim ** -0.5
+    scale    a positive number up to 2^127, default head_dim ** -0.5
     workspace  a uint8 CUDA tensor of at least w4a16_paged_attention_workspace_bytes; default: one
              allocated for a call that takes it, so calls on several streams or in several graphs do not share it
 
