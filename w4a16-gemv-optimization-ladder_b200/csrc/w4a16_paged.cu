@@ -11,7 +11,8 @@
 //
 // Every kernel here is launched with programmatic stream serialisation: its CTAs may be placed
 // while the kernel before it in the stream ends, and wait for that one before they read or
-// write anything.  What that kernel may have written is read by the coherent path only.
+// write anything.  What that kernel may have written is read by ordinary loads through pointers
+// without __restrict__ (fetch says why).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
