@@ -124,6 +124,17 @@ def test_logits(lib):
     assert call(rows=0) == 0 and call(vocab=0) == 0
 
 
+def test_workspace_bytes_from_python(lib):
+    import w4a16 as K
+
+    for heads, kv_heads, head_dim in ((32, 8, 64), (9, 1, 128), (24, 2, 256), (1, 1, 64)):
+        need = K.paged_attention_workspace_bytes(heads, kv_heads, head_dim)
+        assert need == lib.w4a16_paged_attention_workspace_bytes(heads, kv_heads, head_dim) > 0
+    for bad in ((3, 2, 64), (0, 1, 64), (4, 0, 64), (4, 2, 96)):
+        with pytest.raises(RuntimeError):
+            K.paged_attention_workspace_bytes(*bad)
+
+
 @pytest.mark.parametrize("cls,pack", [(_lib.PagePool, _lib.pack_pool), (_lib.PageTables, _lib.pack_tables), (_lib.PageState, _lib.pack_state),
                                       (_lib.PageBlocks, _lib.pack_blocks), (_lib.LogitsDesc, _lib.pack_logits)])
 def test_packed_structures_are_the_declared_ones(cls, pack):

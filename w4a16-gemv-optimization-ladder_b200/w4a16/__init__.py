@@ -38,6 +38,7 @@ from .paged import (
     free_sequences,
     paged_append,
     paged_attention,
+    paged_attention_workspace_bytes,
 )
 from .linear import W4A16Linear, replace_linear_with_w4a16
 from .quant import (
@@ -63,5 +64,5 @@ __all__ = [
     "read_device_error",
     # serving several sequences
     "PagedKVCache", "paged_append", "paged_attention", "extend_sequences", "fork_sequences", "free_sequences",
-    "compact_pages", "copy_pages", "process_logits",
+    "compact_pages", "copy_pages", "paged_attention_workspace_bytes", "process_logits",
 ]

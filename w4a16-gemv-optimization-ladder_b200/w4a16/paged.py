@@ -170,8 +170,8 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     seqs     int32 [rows]: each row's row of `tables` (default: row t is sequence t); several rows may
              name one sequence, as the tokens of a prompt do with growing lengths
     scale    a positive number up to 2^127, default head_dim ** -0.5
-    workspace  a uint8 CUDA tensor of at least w4a16_paged_attention_workspace_bytes; default: one
-             allocated for a call that takes it, so calls on several streams or in several graphs do not share it
+    workspace  a uint8 CUDA tensor of at least paged_attention_workspace_bytes(heads, kv_heads, head_dim); default:
+             one allocated for a call that takes it, so calls on several streams or in several graphs do not share it
 
     Returns out [rows, heads, head_dim], the same bits every time for tables of the same width (those of
     few rows in short tables go a faster way).  A row of length <= 0 is zero; a length past the tables'
@@ -206,6 +206,14 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, seqs=None, scale=No
     _call("w4a16_paged_attention", dev, qp, qs, lens, sq, n, heads, tab, pool, float(d ** -0.5 if scale is None else scale),
           op, os_, ws, size)
     return out
+
+
+def paged_attention_workspace_bytes(heads, kv_heads, head_dim):
+    """Bytes of a workspace for any paged_attention call of these heads.  Its content does not matter; calls that may
+    run at the same time (on two streams, in two graphs) need one each."""
+    if head_dim not in (64, 128, 256) or heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        _refuse(f"no paged attention of {heads} query heads over {kv_heads} kv heads of {head_dim} (64, 128 or 256)")
+    return _bytes("w4a16_paged_attention_workspace_bytes", heads, kv_heads, head_dim)
 
 
 # ------------------------------------------------------------------------------ page bookkeeping
