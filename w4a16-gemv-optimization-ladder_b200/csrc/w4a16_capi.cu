@@ -855,7 +855,6 @@ int w4a16_paged_attention(const void* q, long long q_stride, const int32_t* leng
   a.heads = heads;
   a.scale = scale;
   a.workspace = workspace;
-  a.workspace_bytes = workspace_bytes;
   return w4a16::launch_paged_attention(a, pl, tb, reinterpret_cast<cudaStream_t>(stream));
 }
 

@@ -164,7 +164,6 @@ struct PagedAttention {
   int rows = 0, heads = 0;
   float scale = 0.f;
   void* workspace = nullptr;
-  size_t workspace_bytes = 0;
 };
 int launch_paged_append(const PagedAppend& a, const PagedPool& pool, const PagedTables& tab, cudaStream_t stream);
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
