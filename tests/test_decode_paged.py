@@ -247,3 +247,13 @@ def test_generation_under_rules_matches_an_eager_loop():
     assert dec.generate(token=11, pos=20, n=12, repetition=1.0).tolist() == plain.tolist()  # rules that change nothing
     with pytest.raises(ValueError):
         dec.generate(token=1, pos=0, n=2, prompt=[1] * 161)
+
+
+def test_generation_refuses_rules_of_other_shapes():
+    # a mask of truth values or of one word would be taken for other words, a bias of one value for all tokens'
+    dec = _decoder(seed=7)
+    for bad in (dict(mask=torch.ones(128, device=DEV, dtype=torch.bool)), dict(mask=torch.ones(1, device=DEV, dtype=torch.int32)),
+                dict(mask=torch.ones(4096, device=DEV, dtype=torch.bool)), dict(bias=torch.ones(1, device=DEV)),
+                dict(bias=torch.ones(1, 4096, device=DEV))):
+        with pytest.raises(ValueError):
+            dec.generate(token=1, pos=0, n=2, **bad)

@@ -517,6 +517,10 @@ class W4A16LlamaDecoder:
             prompt = [int(token)] if prompt is None else [int(x) for x in prompt]
             if len(prompt) > self.cfg.max_len:
                 raise ValueError(f"a prompt of {len(prompt)} ids exceeds the cache length {self.cfg.max_len}")
+            for name, t, size in (("bias", bias, self.cfg.vocab), ("mask", mask, -(-self.cfg.vocab // 32))):
+                # what copy_ would broadcast or convert to other words
+                if isinstance(t, torch.Tensor) and not (tuple(t.shape) == (size,) and (name == "bias" or t.dtype in (torch.int32, torch.int64))):
+                    raise ValueError(f"{name} must be a [{size}] tensor{' of int32 words' if name == 'mask' else ''}")
             if self.gen_rules_graph is None:
                 self.capture_generate(rules=True)
             r = self.gen_rules
