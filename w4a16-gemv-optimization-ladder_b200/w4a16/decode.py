@@ -411,7 +411,8 @@ class W4A16LlamaDecoder:
         single new ones mixed: token t (tokens int64 [T]) is position positions[t] (int32) of sequence
         seqs[t] (int32), for which cache.extend has made room, and attends to the positions up to
         its own.  A negative position is padding, whose token may be any number; a real token outside the
-        vocabulary gives NaN.  cache: a PagedKVCache of this model's layers, kv heads and head_dim, in fp16."""
+        vocabulary gives NaN.  cache: a PagedKVCache of this model's layers, kv heads and head_dim, in fp16.
+        The products use this device's shared split-K workspaces: order the calls on one stream."""
         cfg, D = self.cfg, self.cfg.head_dim
         if cache.k.dtype != torch.float16 or tuple(cache.k.shape[i] for i in (0, 2, 4)) != (cfg.layers, cfg.kv_heads, D):
             raise ValueError(f"the cache must be fp16 with {cfg.layers} layers, {cfg.kv_heads} kv heads and head_dim {D}")
